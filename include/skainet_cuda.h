@@ -329,6 +329,76 @@ int32_t skn_kv_append_many_dev(skn_kvcache *kv, const float *k_new_dev, const fl
 int32_t skn_attn_causal_dev(skn_kvcache *kv, const float *q_dev, int32_t n_q_heads, int32_t T, float scale,
                             float *out_dev, void *scratch_dev);
 
+/* ---- Paged KV cache ---------------------------------------------------------------------------------
+ * Keys and values of many sequences of unequal lengths in two pools of pages, for servers that cannot give every
+ * sequence a ring of its own.  No counterpart in the reference (it has no KV cache at all).  The cache counts nothing and owns no
+ * page: which page holds what comes with every call (skn_paged_batch), so pages can be shared between sequences (a common
+ * prefix), given back and used again without telling the cache.
+ *
+ * K and V pool, one page of one head after the other:  [n_pages][n_kv_heads], page_tokens rows each.
+ *   SKN_KV_F16, SKN_KV_BF16: [page_tokens][head_dim]
+ *   SKN_KV_Q4_0: quants [head_dim / 32][page_tokens][16 bytes], then scales [page_tokens][head_dim / 32] fp16.  Per 32 dims, with m their
+ *     value of largest size (the first of equals): d = m / -8, q = trunc(x * fp32(1 / d) + 8.5) in 64 bits, at most 15, read back as
+ *     (q - 8) * fp16(d); byte j holds q[j] and, in its upper half, q[j + 16] (GGUF's Q4_0).  An all-zero block has d = 0.
+ * Rows are rounded once, to nearest even, from fp32.  Rotated keys are formed in 64 bits and rounded to fp32 first. */
+typedef struct skn_paged skn_paged;
+#define SKN_KV_Q4_0 4       /* paged caches only */
+#define SKN_ROT_ADJACENT 0  /* dimension 2 i turns with 2 i + 1 */
+#define SKN_ROT_HALVES 1    /* dimension i turns with i + rot_dims / 2 */
+typedef struct skn_paged_spec {
+    int32_t n_kv_heads, head_dim;    /* head_dim 64 or 128 */
+    int32_t page_tokens;             /* 16, 32, 64 or 128 */
+    int32_t kv_dtype;                /* SKN_KV_F16, SKN_KV_BF16, SKN_KV_Q4_0 */
+    int32_t n_pages;
+    int32_t rot_dims;                /* first dimensions of keys and queries that turn with the position: a multiple of 16; 0: none */
+    int32_t rot_pairs;               /* SKN_ROT_*; pair i turns by position * rot_base^(-2 i / rot_dims) */
+    int32_t reserved;
+    double rot_base;
+} skn_paged_spec;
+/* One step's sequences.  Sequence s has the rows token_start[s] .. token_start[s + 1] - 1 of the step's tokens; they are the last of the
+ * lengths[s] tokens that it has with them, so row i is at position lengths[s] - token_start[s + 1] + i.  Position p lies in row
+ * p % page_tokens of page page_table[s * max_pages + p / page_tokens].  Rows at negative positions (a sequence with more rows than
+ * lengths[s]) are padding: they are not appended or gathered, and their attention output is zero.  Rows before token_start[0] and from
+ * token_start[n_seqs] on belong to nobody and are left as they are.  Entries of pages that no call needs (beyond the
+ * length, or outside every query's window) may hold anything.  The arrays are on the device for `_dev` calls, whose kernels check
+ * what they use of them: a sequence or a page out of range is skipped, and the next skn_sync returns SKN_ERR_ARG. */
+typedef struct skn_paged_batch {
+    int32_t n_seqs, n_tokens;        /* n_tokens: rows of k, v, q and out */
+    int32_t max_new;                 /* no sequence has more new tokens */
+    int32_t max_pages;               /* columns of the page table */
+    const int32_t *page_table;       /* [n_seqs][max_pages] */
+    const int32_t *token_start;      /* [n_seqs + 1], not decreasing */
+    const int32_t *lengths;          /* [n_seqs] */
+} skn_paged_batch;
+/* bytes of one pool of this specification (host arithmetic; the message of a refusal is read with skn_last_error(NULL)) */
+int32_t skn_paged_pool_bytes(const skn_paged_spec *spec, int64_t *bytes);
+/* k_pool_dev, v_pool_dev: device memory of skn_paged_pool_bytes bytes each, 16-byte aligned, that outlives the cache; or both NULL: the
+ * cache allocates them, filled with zeros.  The workspace of attention is allocated here, so every `_dev` call below can be captured
+ * into a CUDA graph; calls on one cache share it and have to be ordered on the device (one stream, or events). */
+int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_dev, void *v_pool_dev, skn_paged **out);
+int32_t skn_paged_destroy(skn_paged *pc);
+int32_t skn_paged_info(const skn_paged *pc, void **k_pool_dev, void **v_pool_dev, int64_t *pool_bytes);
+/* Append the step's keys and values, the keys rotated to their positions; q (optional) is rotated into q_out, which may be q.
+ * `_dev`: io is the element type of k, v, q and q_out (SKN_KV_F32 or SKN_KV_BF16), a row [heads][head_dim]; strides are the elements from one
+ * row to the next (rows of a joint projection need no copy).  Pointers and rows are 16-byte aligned.  A page that a step appends to belongs to
+ * one of its sequences only.  The host form takes dense fp32 rows and answers every mistake before anything has run. */
+int32_t skn_paged_append(skn_paged *pc, const skn_paged_batch *batch, const float *k_host, const float *v_host, const float *q_host,
+                         int32_t n_q_heads, float *q_out_host);
+int32_t skn_paged_append_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, const void *k_dev, int64_t k_stride, const void *v_dev,
+                             int64_t v_stride, const void *q_dev, int64_t q_stride, int32_t n_q_heads, void *q_out_dev, int64_t q_out_stride);
+/* The reverse of append: the cached rows at the positions of the step's tokens (all tokens of a sequence, where token_start says so), dense
+ * [n_tokens][n_kv_heads][head_dim], fp32 (host) or io (device). */
+int32_t skn_paged_gather(skn_paged *pc, const skn_paged_batch *batch, float *k_out_host, float *v_out_host);
+int32_t skn_paged_gather_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, void *k_out_dev, void *v_out_dev);
+/* out = softmax(scale * q . K^T) . V of every row over the cached tokens at its own position and before: all of them (window 0), or the last
+ * `window`, its own included, and the first `sinks` of the sequence.  Query head h reads kv head h / (n_q_heads / n_kv_heads).  What is not
+ * visible has no influence, whatever it holds.  fp32 rows: fp32 accuracy.  bf16 rows: queries exact, softmax weights rounded to
+ * fp16 (bf16 caches: bf16), fp32 sums. */
+int32_t skn_paged_attn(skn_paged *pc, const skn_paged_batch *batch, const float *q_host, int32_t n_q_heads, float scale, int32_t window,
+                       int32_t sinks, float *out_host);
+int32_t skn_paged_attn_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, const void *q_dev, int64_t q_stride, int32_t n_q_heads,
+                           float scale, int32_t window, int32_t sinks, void *out_dev, int64_t out_stride);
+
 /* Host arithmetic only (no device is touched, no context needed): the launch geometry the many-row
  * matvec (3 to 16 activation rows, weights streamed once) would get for n_groups sixteen-row groups of
  * n_cols columns on a GPU of sm_count SMs; swiglu: the interleaved gate / up form.  No reference

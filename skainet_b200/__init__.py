@@ -16,5 +16,6 @@ from .lugasun import LugasunConfig, LugasunDecoder  # noqa: E402
 from .tutezen import TutezenConfig, TutezenDecoder  # noqa: E402
 from .registry import ARCHITECTURES, load_model  # noqa: E402
 from .generate import generate  # noqa: E402
+from .paged import PagedBatch, PagedKVCache  # noqa: E402
 
-__all__ += ["ARCHITECTURES", "LugasunConfig", "LugasunDecoder", "TutezenConfig", "TutezenDecoder", "generate", "load_model"]
+__all__ += ["ARCHITECTURES", "LugasunConfig", "LugasunDecoder", "PagedBatch", "PagedKVCache", "TutezenConfig", "TutezenDecoder", "generate", "load_model"]

@@ -69,6 +69,16 @@ class TutezenWeights(ctypes.Structure):
                                     "out_norm", "q_gain", "kv_gain", "sink")]
 
 
+class PagedSpec(ctypes.Structure):
+    _fields_ = [("n_kv_heads", c_i32), ("head_dim", c_i32), ("page_tokens", c_i32), ("kv_dtype", c_i32), ("n_pages", c_i32),
+                ("rot_dims", c_i32), ("rot_pairs", c_i32), ("reserved", c_i32), ("rot_base", ctypes.c_double)]
+
+
+class PagedBatchSpec(ctypes.Structure):
+    _fields_ = [("n_seqs", c_i32), ("n_tokens", c_i32), ("max_new", c_i32), ("max_pages", c_i32), ("page_table", c_vp),
+                ("token_start", c_vp), ("lengths", c_vp)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "skn_version": (c_i32, []),
@@ -149,6 +159,16 @@ SIGNATURES = {
     "skn_decoder_forward": (c_i32, [c_vp, c_i32, c_i32, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp]),
     "skn_decoder_forward_dev": (c_i32, [c_vp, c_i32, c_i32, c_vp, c_i32, c_i32]),
     "skn_decoder_trace": (c_i32, [c_vp, c_i32, c_i32, c_vp]),
+    "skn_paged_pool_bytes": (c_i32, [P(PagedSpec), P(c_i64)]),
+    "skn_paged_create": (c_i32, [c_vp, P(PagedSpec), c_vp, c_vp, P(c_vp)]),
+    "skn_paged_destroy": (c_i32, [c_vp]),
+    "skn_paged_info": (c_i32, [c_vp, P(c_vp), P(c_vp), P(c_i64)]),
+    "skn_paged_append": (c_i32, [c_vp, P(PagedBatchSpec), c_vp, c_vp, c_vp, c_i32, c_vp]),
+    "skn_paged_append_dev": (c_i32, [c_vp, P(PagedBatchSpec), c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_i64]),
+    "skn_paged_gather": (c_i32, [c_vp, P(PagedBatchSpec), c_vp, c_vp]),
+    "skn_paged_gather_dev": (c_i32, [c_vp, P(PagedBatchSpec), c_i32, c_vp, c_vp]),
+    "skn_paged_attn": (c_i32, [c_vp, P(PagedBatchSpec), c_vp, c_i32, ctypes.c_float, c_i32, c_i32, c_vp]),
+    "skn_paged_attn_dev": (c_i32, [c_vp, P(PagedBatchSpec), c_i32, c_vp, c_i64, c_i32, ctypes.c_float, c_i32, c_i32, c_vp, c_i64]),
     "skn_gguf_open": (c_i32, [ctypes.c_char_p, P(c_vp)]),
     "skn_gguf_close": (c_i32, [c_vp]),
     "skn_gguf_counts": (c_i32, [c_vp, P(c_i32), P(c_i64), P(c_i64), P(c_i64), P(c_i64)]),

@@ -293,7 +293,8 @@ int32_t skn_status_check(skn_ctx *ctx) {
         return skn_fail(ctx, st, "a kernel reported device-side status %d (%s)", st,
                         st == SKN_ERR_TIMEOUT ? "a bounded wait ran out"
                         : st == SKN_ERR_SHAPE ? "a KV cache was asked to hold more tokens than its capacity; nothing was overwritten"
-                                              : "see status codes");
+                        : st == SKN_ERR_ARG ? "a step over a paged cache named rows or pages out of range; they were skipped"
+                                            : "see status codes");
     }
     return SKN_OK;
 }

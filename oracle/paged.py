@@ -88,10 +88,10 @@ class Pages:
         return pool[table[s, p // self.page], :, p % self.page].transpose(1, 0, 2)
 
     def attend(self, q, table, token_start, lengths, scale, window=0, sinks=0, given=None):
-        """(out, bound): outputs fp64 (rows of nobody as in `given`), and per output sum p |v| and the largest scale * sum |q k| of its row"""
+        """outputs fp64 (rows of nobody as in `given`); per output sum p |v|; per row the largest scale * sum |q k|, then the dims' sums of |v|"""
         q = np.asarray(q, dtype=np.float64)
         out = np.zeros_like(q) if given is None else np.asarray(given, dtype=np.float64).copy()
-        mass, reach = np.zeros_like(q), np.zeros(q.shape[:2] + (1,))
+        mass, reach = np.zeros_like(q), np.zeros(q.shape[:2] + (1 + q.shape[2],))
         first = int(token_start[0])
         for i, (s, p) in enumerate(positions(token_start, lengths)):
             i += first
@@ -109,5 +109,6 @@ class Pages:
                 w /= w.sum()
                 out[i, h] = w @ v
                 mass[i, h] = w @ np.abs(v)
-                reach[i, h] = abs(scale) * (np.abs(k) @ np.abs(q[i, h])).max()
+                reach[i, h, 0] = abs(scale) * (np.abs(k) @ np.abs(q[i, h])).max()
+                reach[i, h, 1:] = np.abs(v).sum(axis=0)
         return out, mass, reach

@@ -357,6 +357,8 @@ int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_
     *out = nullptr;
     const int32_t rc = check_spec(ctx, spec);
     if (rc) return rc;
+    if ((int64_t)spec->n_pages * spec->n_kv_heads * spec->page_tokens > INT32_MAX)
+        return skn_fail(ctx, SKN_ERR_SHAPE, "%d pages of %d tokens and %d heads are more than 2^31 rows", spec->n_pages, spec->page_tokens, spec->n_kv_heads);
     if (!k_pool_dev != !v_pool_dev) return skn_fail(ctx, SKN_ERR_ARG, "one pool is NULL");
     if (((uintptr_t)k_pool_dev | (uintptr_t)v_pool_dev) & 15) return skn_fail(ctx, SKN_ERR_ALIGN, "pools must be 16-byte aligned");
     skn_paged *pc = new (std::nothrow) skn_paged();
@@ -381,6 +383,7 @@ int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_
     }
     if (e == cudaSuccess) e = cudaMalloc((void **)&pc->d_turns, sizeof(turns));
     if (e == cudaSuccess) e = cudaMemcpyAsync(pc->d_turns, turns, sizeof(turns), cudaMemcpyHostToDevice, ctx->stream);
+    if (e == cudaSuccess) e = skn_paged_attn_prepare(pc);
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     if (e != cudaSuccess) {
         skn_paged_destroy(pc);
@@ -401,6 +404,8 @@ int32_t skn_paged_destroy(skn_paged *pc) {
         if (pc->v) cudaFree(pc->v);
     }
     if (pc->d_turns) cudaFree(pc->d_turns);
+    if (pc->d_parts) cudaFree(pc->d_parts);
+    if (pc->d_tickets) cudaFree(pc->d_tickets);
     pc->magic = 0;
     delete pc;
     return SKN_OK;

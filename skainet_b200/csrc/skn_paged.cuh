@@ -3,7 +3,9 @@
 #include "skn_internal.cuh"
 
 #include <cuda.h>
+#include <type_traits>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #define SKN_MAGIC_PAGED 0x736b6e70u   // 'sknp'
 
@@ -17,7 +19,13 @@ struct skn_paged {
     int64_t head_bytes;          // one page of one head
     int64_t pool_bytes;
     double *d_turns;             // [rot_dims / 2] half turns per position
+    // Attention's workspace (skn_paged_attn.cu): tensor maps of the pools and, for rows whose keys several CTAs share, their partial results
+    CUtensorMap map[4];          // K, V; of Q4_0 their quants, then their scales
+    int n_parts;                 // CTAs that share a launch's work
+    float *d_parts;              // [2 n_parts][SKN_PAGED_PART_ROWS][head_dim + 4]: output, maximum, sum
+    unsigned *d_tickets;         // [2 n_parts], zero between launches
 };
+constexpr int SKN_PAGED_PART_ROWS = 32;
 
 // A step as the kernels see it
 struct PagedStep {
@@ -108,6 +116,7 @@ template <int D> __device__ __forceinline__ void paged_load8(const skn_q4 *at, i
 #endif
 
 bool skn_paged_ok(const skn_paged *pc);
+cudaError_t skn_paged_attn_prepare(skn_paged *pc);
 // attention over `batch` (device arrays) on the context's stream; arguments checked by the caller
 int32_t skn_paged_attn_launch(skn_paged *pc, const skn_paged_batch *batch, int32_t io, const void *q, int64_t q_stride, int32_t n_q_heads, float scale,
                               int32_t window, int32_t sinks, void *out, int64_t out_stride);

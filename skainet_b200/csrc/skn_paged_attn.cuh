@@ -1,0 +1,945 @@
+// Attention over the paged KV cache: rows of few tokens (decoding), and every row of fp32.  A translation unit per cache type.
+//
+// Work.  A segment is a sequence's new rows (up to 8 NB of them: tokens x query heads of one kv head) over the keys that some of them sees,
+// in units of 16 (fp16, bf16) or 32 (Q4_0) keys.  The units of all segments form one line, which the CTAs share out evenly, so that a batch of
+// unequal lengths keeps every SM at work to the end; a segment that lies in several CTAs leaves partial results (maximum, sum,
+// unnormalised output), which the last of them to finish joins in order.
+//
+// A unit.  Each of a CTA's eight warps takes every eighth unit through a ring of its own, filled by TMA.  S^T = K q^T with mma.sync (m16n8k16: 16 keys
+// x 8 rows): keys are the operand of 16 so that up to eight query heads waste nothing.  Scores go through one running maximum per row that
+// moves only when a weight would exceed 2^SLACK (one vote a unit instead of six shuffles).  Weights are transposed by movmatrix into the second
+// operand of O^T = V^T p^T.  fp32 rows: queries and weights as sums of two fp16 (fp16 and Q4_0 caches) or three bf16 terms.
+//
+// Q4_0.  K: a nibble masked out of a word is an fp16 subnormal, q 2^-24 (or 16 q 2^-24), which the tensor cores multiply exactly, so quants need
+// no conversion; one accumulator per block of 32 dims starts at -8 sum q and is scaled by the key's d.  V: weights are multiplied by the
+// key's d of the block, in fp16 relative to a power of two 2^E that follows the largest d, and meet q - 8 (one packed instruction for two): with
+// the 8 taken off at the end, a dimension of zeros would come out as the rounding of two large sums.
+//
+// Infinities and NaN.  Scores of hidden keys are replaced, not added to.  A hidden row of V meets a weight of zero, and zero times infinity is no
+// zero: in units with hidden keys, rows that nobody sees are cleared if they are not finite.  Whatever else goes wrong with such values
+// (a key that some rows see and others do not; an infinity that meets the two terms of a weight) leaves a result that is not finite,
+// and a segment with one is computed again straight from the definition (paged_redo).
+#pragma once
+#include "skn_paged.cuh"
+#include "skn_mma.cuh"
+#include "skn_tc.cuh"
+
+#include <math.h>
+
+constexpr int PA_WARPS = 8, PA_THREADS = 32 * PA_WARPS;
+constexpr int PA_MAX_SEQS = 1024;            // sequences whose work is shared out; more of them take a CTA per segment
+constexpr float PA_NONE = -1e30f;            // running maximum before the first score
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <class CT> __device__ __forceinline__ void mma_as(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<CT, __nv_bfloat16>::value) mma_bf16(c, a, b0, b1);
+    else mma_f16(c, a, b0, b1);
+}
+__device__ __forceinline__ uint32_t movm(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// two values -> NT packed terms of the product's type
+template <class CT, int NT> __device__ __forceinline__ void terms_of(float x, float y, uint32_t (&w)[NT]) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        if constexpr (std::is_same<CT, __nv_bfloat16>::value) {
+            w[i] = pack_bf16(x, y);
+            if (i + 1 < NT) less_bf16(x, y, w[i]);
+        } else {
+            w[i] = pack_f16(x, y);
+            if (i + 1 < NT) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                x -= f.x;
+                y -= f.y;
+            }
+        }
+    }
+}
+__device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(skn_smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(skn_smem_u32(bar))
+                 : "memory");
+}
+
+struct PagedAttn {
+    PagedStep st;
+    const uint8_t *k_pool, *v_pool;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    int group, window, sinks;
+    float scale;                  // times log2(e)
+    int direct;                   // a CTA per segment: no sharing (rows in blocks of 8 NB)
+    float *parts;
+    unsigned *tickets;
+};
+
+// The keys that a segment's rows see, as units: 0 .. a - 1 (first tokens), then from unit a + gap on
+struct PagedSpan { int units, a, gap; };
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttn &p, int pmin, int pmax, int unit) {
+    const int lo = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
+    const int a = (min(p.sinks, lo) + unit - 1) / unit, b = lo / unit;
+    PagedSpan s = {(pmax + unit) / unit, 0, 0};
+    if (pmax < 0) s.units = 1;                       // rows without a key still have an output
+    if (p.window && b > a) {
+        s.a = a;
+        s.gap = b - a;
+        s.units -= s.gap;
+    }
+    return s;
+}
+__device__ __forceinline__ bool paged_sees(const PagedAttn &p, int key, int pos) {
+    return key <= pos && (!p.window || key > pos - p.window || key < p.sinks);
+}
+
+struct PagedSegment {
+    int seq, head, first, rows, row0;     // its rows of the step: token first + r / group, query head head * group + r % group, r = row0 ..
+    int n, len;                           // of the sequence
+    PagedSpan span;
+    int u0, u1;                           // this CTA's units
+    int c0, n_parts, slot;                // CTAs that have some of it: c0 .. c0 + n_parts - 1
+};
+
+// A segment from the definition: for rows in turn, a thread per key and then a thread per dimension.  Results as the warps' are: maximum (base 2), sum and
+// unnormalised output in `comb`.
+template <class CT, int D, class IO>
+__device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &g, int unit, float *comb, float *ml, float *scratch) {
+    float *qs = scratch, *ps = scratch + D, *red = ps + PA_THREADS;
+    const int tid = threadIdx.x;
+    for (int r = 0; r < g.rows; ++r) {
+        const int t = (g.row0 + r) / p.group, pos = g.len - g.n + t;
+        const IO *q = static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + r) % p.group) * D;
+        __syncthreads();
+        if (tid < D / 8) {
+            float x[8];
+            io_load8(q + 8 * tid, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qs[8 * tid + i] = x[i];
+        }
+        __syncthreads();
+        float m = PA_NONE, l = 0.f, acc = 0.f;
+        for (int b = g.u0 * unit; b < g.u1 * unit; b += PA_THREADS) {
+            auto key_of = [&](int i) { const int u = i / unit; return (u < g.span.a ? u : u + g.span.gap) * unit + i % unit; };
+            const int i = b + tid, key = key_of(i);
+            float z = -INFINITY;
+            bool seen = i < g.u1 * unit && paged_sees(p, key, pos);
+            if (seen) {
+                const int page = paged_page(p.st, g.seq, key), row = key & ((1 << p.st.page_shift) - 1);
+                seen = page >= 0;
+                if (seen) {
+                    const CT *at = reinterpret_cast<const CT *>(p.k_pool + paged_at(p.st, page, g.head));
+                    float dot[8] = {};
+                    for (int c = 0; c < D / 8; ++c) {
+                        float x[8];
+                        paged_load8<D>(at, p.st.page_shift, row, c, x);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) dot[j] = fmaf(x[j], qs[8 * c + j], dot[j]);
+                    }
+                    z = (((dot[0] + dot[1]) + (dot[2] + dot[3])) + ((dot[4] + dot[5]) + (dot[6] + dot[7]))) * p.scale;
+                }
+            }
+            float top = z;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if ((tid & 31) == 0) red[tid >> 5] = top;
+            __syncthreads();
+            top = m;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, red[w]);
+            const float fix = exp2f(m - top), w = seen ? exp2f(z - top) : 0.f;
+            ps[tid] = seen ? w : -1.f;                   // -1: hidden, its row of V is not touched
+            float sum = w;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            __syncthreads();
+            if ((tid & 31) == 0) red[tid >> 5] = sum;
+            __syncthreads();
+            l *= fix;
+#pragma unroll
+            for (int k = 0; k < PA_WARPS; ++k) l += red[k];
+            acc *= fix;
+            m = top;
+            if (tid < D)
+                for (int j = 0; j < PA_THREADS && b + j < g.u1 * unit; ++j) {
+                    if (ps[j] < 0.f) continue;
+                    const int kj = key_of(b + j), page = p.st.table[(int64_t)g.seq * p.st.max_pages + (kj >> p.st.page_shift)];
+                    const CT *at = reinterpret_cast<const CT *>(p.v_pool + paged_at(p.st, page, g.head));
+                    float x[8];
+                    paged_load8<D>(at, p.st.page_shift, kj & ((1 << p.st.page_shift) - 1), tid >> 3, x);
+                    float v = x[0];
+#pragma unroll
+                    for (int e = 1; e < 8; ++e) v = (tid & 7) == e ? x[e] : v;
+                    acc = fmaf(ps[j], v, acc);
+                }
+            __syncthreads();
+        }
+        if (tid < D) comb[r * (D + 4) + tid] = acc;
+        if (tid == 0) {
+            ml[2 * r] = m;
+            ml[2 * r + 1] = l;
+        }
+    }
+    __syncthreads();
+}
+
+template <class CT, int D, int NB, bool EX> struct PaTraits {
+    static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
+    static constexpr int UNIT = Q4 ? 32 : 16;
+    static constexpr int NT = EX ? (BF ? 3 : 2) : 1;
+    static constexpr int ROW = Q4 ? D / 2 + D / 16 : 2 * D;
+    static constexpr int HALF = (16 * ROW + 127) / 128 * 128;                     // 16 rows, where TMA may put them
+    static constexpr int TILE = UNIT / 16 * HALF, STAGE = 2 * TILE;               // K, then V
+    // eight warps' rings: about 190 KB of 16-bit rows in one CTA per SM; of 4 bits 74 KB (D = 128) in each of two
+    static constexpr int STAGES = Q4 ? (D == 128 ? 2 : 4) : D == 128 ? (NB == 4 ? 2 : 3) : 6;
+    static constexpr int PER_SM = Q4 && NB == 1 ? 2 : 1;
+    static constexpr int ROWS = 8 * NB;
+    // Weights reach 2^SLACK before the maximum moves.  In fp16 they are lifted to 2^15 at most, so that a weight of 2^-24 - 15 + SLACK of its row's largest is
+    // the last one there; fp32 rows, whose second term ends there too, pay for a smaller SLACK with more moves
+    static constexpr int SLACK = EX ? 1 : 4;
+    static constexpr float LIFT = BF ? 1.f : EX ? 16384.f : 2048.f;
+    static constexpr int V_UP = EX ? 12 : 7;                                      // Q4_0: the largest d, times 2^-E, is 2^V_UP .. 2^(V_UP + 1) when E is set
+    static constexpr bool Q_SMEM = NB > 1 || (Q4 && EX);                          // query fragments in shared memory instead of registers
+    static constexpr int KS = D / 16;
+    static constexpr int RING = PA_WARPS * STAGES * STAGE;
+    static constexpr int COMB = PA_WARPS * ROWS * (D + 4) * 4;                    // lies over the ring between segments
+    static constexpr int BODY = (RING > COMB ? RING : COMB);
+    static constexpr int Q_BYTES = Q_SMEM ? NT * NB * KS * 32 * 8 : 0;
+    static constexpr size_t SMEM = 1024 + BODY + Q_BYTES;
+};
+
+template <class CT, int D, int NB, bool EX>
+__global__ void __launch_bounds__(PA_THREADS, (PaTraits<CT, D, NB, EX>::PER_SM))
+skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                      const __grid_constant__ CUtensorMap mks, const __grid_constant__ CUtensorMap mvs) {
+    using T = PaTraits<CT, D, NB, EX>;
+    using IO = typename std::conditional<EX, float, __nv_bfloat16>::type;
+    constexpr int UNIT = T::UNIT, NT = T::NT, KS = T::KS, STAGES = T::STAGES, ROWS = T::ROWS, NBLK = D / 32;
+    extern __shared__ uint8_t raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    uint2 *qf = reinterpret_cast<uint2 *>(ring + T::BODY);
+    __shared__ uint64_t full[PA_WARPS * STAGES];
+    __shared__ long long before[PA_MAX_SEQS + 1];
+    __shared__ float wml[PA_WARPS][2 * ROWS], rml[2 * ROWS];
+    __shared__ float scratch[D + PA_THREADS + PA_WARPS];
+    __shared__ long long wsum_s[PA_WARPS];
+    __shared__ int flags[2];                   // [0] a result is not finite, [1] a wait ran out
+    __shared__ unsigned ticket;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
+    const PagedStep &st = p.st;
+
+    if (tid < PA_WARPS * STAGES) skn_mbar_init(&full[tid], 1);
+    if (tid < 2) flags[tid] = 0;
+    skn_fence_mbar_init();
+
+    // ---- the line of units -----------------------------------------------------------------------------------------------
+    long long u = 0, u_end = 1, total = 1;
+    int n_cta = 1;
+    if (!p.direct) {
+        long long run = 0;
+        for (int b = 0; b < st.n_seqs; b += PA_THREADS) {
+            const int s = b + tid;
+            long long x = 0;
+            if (s < st.n_seqs) {
+                const PagedSeq sq = paged_seq(st, s);
+                if (sq.n > 0) x = paged_span(p, sq.len - sq.n, sq.len - 1, UNIT).units;
+            }
+            long long inc = x;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
+            }
+            if (lane == 31) wsum_s[warp] = inc;
+            __syncthreads();
+            long long base = run;
+            for (int w = 0; w < PA_WARPS; ++w) {
+                if (w < warp) base += wsum_s[w];
+                run += wsum_s[w];
+            }
+            if (s < st.n_seqs) before[s] = (base + inc - x) * st.heads;
+            __syncthreads();
+        }
+        total = run * st.heads;
+        if (tid == 0) before[st.n_seqs] = total;
+        __syncthreads();
+        if (total == 0) return;
+        // fewer CTAs where each would get less than a unit per warp
+        const long long want = (total + PA_WARPS - 1) / PA_WARPS;
+        n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
+        if ((int)blockIdx.x >= n_cta) return;
+        u = total * blockIdx.x / n_cta;
+        u_end = total * (blockIdx.x + 1) / n_cta;
+    } else __syncthreads();
+
+    int stage = 0, parity = 0;                 // of the warp's next unit
+    const long long u_begin = u;
+    int s_at = 0;
+    while (u < u_end) {
+        // ---- which segment ------------------------------------------------------------------------------------------------
+        PagedSegment g;
+        if (p.direct) {
+            g.seq = blockIdx.z;
+            g.head = blockIdx.y;
+            const PagedSeq sq = paged_seq(st, g.seq);
+            g.n = sq.n; g.len = sq.len; g.first = sq.first;
+            const int n_blocks = (sq.n * p.group + ROWS - 1) / ROWS;
+            const int rb = n_blocks - 1 - (int)blockIdx.x;              // the longest rows first
+            if (rb < 0) return;
+            g.row0 = rb * ROWS;
+            g.rows = min(ROWS, sq.n * p.group - g.row0);
+            g.span = paged_span(p, sq.len - sq.n + g.row0 / p.group, sq.len - sq.n + (g.row0 + g.rows - 1) / p.group, UNIT);
+            g.u0 = 0; g.u1 = g.span.units;
+            g.n_parts = 1; g.c0 = 0; g.slot = 0;
+            u = u_end;
+        } else {
+            int lo = s_at, hi = st.n_seqs - 1;                          // the last sequence that begins at or before u and has units
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (before[mid] <= u) lo = mid; else hi = mid - 1;
+            }
+            s_at = g.seq = lo;
+            const PagedSeq sq = paged_seq(st, g.seq);
+            g.n = sq.n; g.len = sq.len; g.first = sq.first;
+            g.row0 = 0; g.rows = sq.n * p.group;
+            g.span = paged_span(p, sq.len - sq.n, sq.len - 1, UNIT);
+            const long long off = u - before[lo];
+            g.head = (int)(off / g.span.units);
+            g.u0 = (int)(off - (long long)g.head * g.span.units);
+            const long long left = u_end - u;
+            g.u1 = left < g.span.units - g.u0 ? g.u0 + (int)left : g.span.units;
+            const long long a = u - g.u0;
+            g.c0 = (int)(((a + 1) * n_cta - 1) / total);
+            g.n_parts = (int)(((a + g.span.units) * n_cta - 1) / total) - g.c0 + 1;
+            g.slot = 2 * (int)blockIdx.x + (u == u_begin ? 0 : 1);
+            u += g.u1 - g.u0;
+        }
+        const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
+        const int n_mine = (g.u1 - g.u0 - warp + PA_WARPS - 1) / PA_WARPS;         // units g.u0 + warp + PA_WARPS j
+
+        // ---- loads of the warp's units: lane j of `pages` holds the pages of unit j (mod 32) ---------------------------------
+        int page0 = -1, page1 = -1;
+        auto key_of = [&](int j) {
+            const int i = g.u0 + warp + PA_WARPS * j;
+            return (i < g.span.a ? i : i + g.span.gap) * UNIT;
+        };
+        const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
+        auto needed = [&](int k) { return k <= pmax && (k + 15 >= seen_from || k < p.sinks); };     // some row sees some of 16 keys
+        auto look_up = [&](int j0) {               // pages of units j0 .. j0 + 31; the table is asked for none that nobody needs
+            const int j = j0 + lane;
+            page0 = page1 = -1;
+            if (j < n_mine) {
+                const int k = key_of(j);
+                if (needed(k)) page0 = paged_page(st, g.seq, k);
+                if (T::Q4) {
+                    if (needed(k + 16)) page1 = st.page_shift > 4 && page0 >= 0 ? page0 : paged_page(st, g.seq, k + 16);
+                }
+            }
+        };
+        look_up(0);
+        uint8_t *const mine = ring + warp * STAGES * T::STAGE;
+        uint32_t there = 0;                        // two bits a stage: which 16 keys of its unit have a page
+        auto issue = [&](int j, int at) {          // every lane calls it, the first one works
+            const int pg0 = __shfl_sync(0xffffffffu, page0, j & 31), pg1 = T::Q4 ? __shfl_sync(0xffffffffu, page1, j & 31) : -1;
+            there = (there & ~(3u << (2 * at))) | ((uint32_t)(pg0 >= 0) << (2 * at)) | ((uint32_t)(pg1 >= 0) << (2 * at + 1));
+            if (lane == 0) {
+                uint64_t *bar = &full[warp * STAGES + at];
+                uint8_t *k = mine + at * T::STAGE, *v = k + T::TILE;
+                const int row = key_of(j) & ((1 << st.page_shift) - 1);
+                if constexpr (!T::Q4) {
+                    if (pg0 < 0) skn_mbar_arrive(bar);
+                    else {
+                        skn_mbar_expect_tx(bar, 2 * UNIT * T::ROW);
+                        const int y = ((pg0 * st.heads + g.head) << st.page_shift) + row;
+                        tma_3d(k, &mk, 0, y, 0, bar);
+                        tma_3d(v, &mv, 0, y, 0, bar);
+                    }
+                } else {
+                    // pages of 16: a box each for the two halves; else one box of 32 rows.  Quants [D / 32][rows][16], then scales [rows][D / 32]
+                    const bool two = st.page_shift == 4;
+                    const int bytes = (two ? 16 : 32) * T::ROW * 2;
+                    const int n = two ? (pg0 >= 0) + (pg1 >= 0) : (pg0 >= 0 || pg1 >= 0);
+                    if (n == 0) skn_mbar_arrive(bar);
+                    else {
+                        skn_mbar_expect_tx(bar, n * bytes);
+                        for (int h = 0; h < (two ? 2 : 1); ++h) {
+                            const int pg = h || (!two && pg0 < 0) ? pg1 : pg0;
+                            if (pg < 0) continue;
+                            const int z = pg * st.heads + g.head, off = h * T::HALF, sc = (two ? 16 : 32) * (D / 2);
+                            tma_3d(k + off, &mk, row * 4, 0, z, bar);
+                            tma_3d(v + off, &mv, row * 4, 0, z, bar);
+                            tc_tma_load_2d(k + off + sc, &mks, row * (D / 64), z, bar);
+                            tc_tma_load_2d(v + off + sc, &mvs, row * (D / 64), z, bar);
+                        }
+                    }
+                }
+            }
+        };
+        const bool dead = flags[1] != 0;
+        int issued = dead ? n_mine : 0;
+        for (int i = 0; i < STAGES && issued < n_mine; ++i, ++issued) issue(issued, (stage + i) % STAGES);
+
+        // ---- queries: fragments of the second operand, lane (row g8 of each block of eight, t4) ------------------------------
+        // fp16 products take them times a power of two that brings a row's largest to 2^14 .. 2^15
+        uint32_t qr[T::Q_SMEM ? 1 : NT][T::Q_SMEM ? 1 : NB][KS][2];
+        float cs[NB][2];                           // factor of the scores of rows 2 t4, 2 t4 + 1
+        float bias[T::Q4 ? NB : 1][T::Q4 ? NBLK : 1][2];
+        int pos[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = 8 * nb + g8;
+            const bool real = r < g.rows;
+            const int t = (g.row0 + r) / p.group;
+            const IO *q = static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + r) % p.group) * D;
+            float x[KS][4];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // 16-bit caches: dims 16 k + 2 t, + 1, + 8, + 9.  Q4_0: of block k / 2, its lower (k even) or upper 16: 4 t, + 2, + 1, + 3
+                    const int d = T::Q4 ? 16 * k + 4 * t4 + ((i & 1) << 1) + (i >> 1) : 16 * k + 2 * t4 + (i & 1) + 8 * (i >> 1);
+                    x[k][i] = 0.f;
+                    if constexpr (EX) {
+                        if (real) x[k][i] = q[d];
+                    } else {
+                        if (real) x[k][i] = __bfloat162float(q[d]);
+                    }
+                }
+            }
+            float f = 1.f;
+            if constexpr (!T::BF) {
+                float top = 0.f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[k][i]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                int e = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
+                e = top > 0.f && top < INFINITY ? max(-120, min(120, e)) : 0;
+                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                f = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[k][i] *= up;
+            }
+            float bs[T::Q4 ? NBLK : 1];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                if constexpr (T::Q4) {
+                    const float sum = (x[k][0] + x[k][1]) + (x[k][2] + x[k][3]);
+                    if (k & 1) bs[k >> 1] += sum; else bs[k >> 1] = sum;
+                    if (k & 1) {                    // the upper nibble stands 16 times higher
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[k][i] *= 0.0625f;
+                    }
+                }
+                uint32_t a[NT], b[NT];
+                terms_of<CT, NT>(x[k][0], x[k][1], a);
+                terms_of<CT, NT>(x[k][2], x[k][3], b);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (T::Q_SMEM) {
+                        if (warp == 0) qf[((n * NB + nb) * KS + k) * 32 + lane] = make_uint2(a[n], b[n]);
+                    } else {
+                        qr[n][nb][k][0] = a[n];
+                        qr[n][nb][k][1] = b[n];
+                    }
+                }
+            }
+            f *= p.scale;
+            if constexpr (T::Q4) f *= 16777216.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int src = 4 * (2 * t4 + c);
+                cs[nb][c] = __shfl_sync(0xffffffffu, f, src);
+                const int rc = 8 * nb + 2 * t4 + c;
+                pos[nb][c] = rc < g.rows ? g.len - g.n + (g.row0 + rc) / p.group : -1;
+                if constexpr (T::Q4) {
+#pragma unroll
+                    for (int b = 0; b < NBLK; ++b) {
+                        float s = bs[b];
+                        s += __shfl_xor_sync(0xffffffffu, s, 1);
+                        s += __shfl_xor_sync(0xffffffffu, s, 2);
+                        bias[nb][b][c] = __shfl_sync(0xffffffffu, s, src) * (-8.f / 16777216.f);
+                    }
+                }
+            }
+        }
+        if constexpr (T::Q_SMEM) __syncthreads();
+
+        // ---- the units ------------------------------------------------------------------------------------------------------
+        float o[D / 16][NB][4], m[NB][2], l[NB][2];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[i][nb][c] = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                m[nb][c] = PA_NONE;
+                l[nb][c] = 0.f;
+            }
+        float ve = 1.f;                            // Q4_0: 2^-E
+        float ve_inv = 1.f;
+        __half2 vlim = __floats2half2_rn(0.f, 0.f); // and the largest |d| that it takes
+        for (int j = 0; j < n_mine && !dead; ++j) {
+            const int kbase = key_of(j);
+            bool gone = false;
+            {
+                uint64_t *bar = &full[warp * STAGES + stage];
+                if (!tc_wait_warp(bar, parity, lane)) gone = true;
+            }
+            if (gone) {
+                if (lane == 0) {
+                    *st.status = SKN_ERR_TIMEOUT;
+                    flags[1] = 1;
+                }
+                for (; j < issued; ++j) {          // what is on its way lands before its place is used again
+                    tc_wait_warp(&full[warp * STAGES + stage], parity, lane);
+                    if (++stage == STAGES) {
+                        stage = 0;
+                        parity ^= 1;
+                    }
+                }
+                break;
+            }
+            const bool has0 = there >> (2 * stage) & 1, has1 = !T::Q4 || (there >> (2 * stage + 1) & 1);
+            uint8_t *kt = mine + stage * T::STAGE, *vt = kt + T::TILE;
+            const bool whole = kbase + UNIT - 1 <= pmin && has0 && has1 && (!p.window || kbase > pmax - p.window || kbase + UNIT <= p.sinks);
+            if constexpr (!T::Q4) {
+                if (!whole) {                      // rows of V that are not finite: cleared if nobody sees them
+                    const int r = lane & 15, key = kbase + r;
+                    const uint32_t base = skn_smem_u32(vt) + r * 128;
+                    bool odd = false, some = false;
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        const int cc = (lane >> 4) * (D / 16) + c;
+                        const uint4 v = tc_lds128(base + (cc >> 3) * 2048 + (((cc & 7) ^ (r & 7)) << 4));
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                        constexpr uint32_t EXP = T::BF ? 0x7F80u : 0x7C00u;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) odd |= (w[i] & EXP) == EXP || (w[i] & (EXP << 16)) == (EXP << 16);
+                    }
+                    odd |= __shfl_xor_sync(0xffffffffu, (int)odd, 16) != 0;      // (every lane takes part)
+                    for (int t = g.row0 / p.group; t <= (g.row0 + g.rows - 1) / p.group; ++t) some |= has0 && paged_sees(p, key, g.len - g.n + t);
+                    if (odd && !some) {
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            const int cc = (lane >> 4) * (D / 16) + c;
+                            *reinterpret_cast<uint4 *>(vt + r * 128 + (cc >> 3) * 2048 + (((cc & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                        }
+                        skn_fence_proxy_async();
+                    }
+                    __syncwarp();
+                }
+            }
+#pragma unroll
+            for (int sub = 0; sub < UNIT / 16; ++sub) {
+                const int key0 = kbase + 16 * sub;
+                const bool hidden_page = !(sub ? has1 : has0);
+                float s[NB][4];
+                // ---- scores ------------------------------------------------------------------------------------------------
+                const uint8_t *vq = nullptr;       // Q4_0: this half's rows of V, and between blocks
+                int bstep = 0;
+                float dv[2][T::Q4 ? NBLK : 1];
+                __half2 dtop = vlim;
+                if constexpr (T::Q4) {
+                    const bool two = st.page_shift == 4;
+                    bstep = two ? 256 : 512;
+                    const int off = two ? sub * T::HALF : sub * 256;
+                    const uint8_t *kq = kt + off;
+                    const uint8_t *kd = kt + (two ? sub * T::HALF + 16 * (D / 2) : 32 * (D / 2) + sub * 16 * (D / 16));
+                    vq = vt + off;
+                    const uint8_t *vd = vt + (kd - kt);
+                    float dk[2][NBLK];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t wk[NBLK / 2], wv[NBLK / 2];
+                        if constexpr (D == 128) {
+                            const uint2 a = *reinterpret_cast<const uint2 *>(kd + (g8 + 8 * h) * 8), b = *reinterpret_cast<const uint2 *>(vd + (g8 + 8 * h) * 8);
+                            wk[0] = a.x; wk[1] = a.y; wv[0] = b.x; wv[1] = b.y;
+                        } else {
+                            wk[0] = *reinterpret_cast<const uint32_t *>(kd + (g8 + 8 * h) * 4);
+                            wv[0] = *reinterpret_cast<const uint32_t *>(vd + (g8 + 8 * h) * 4);
+                        }
+#pragma unroll
+                        for (int b = 0; b < NBLK / 2; ++b) {
+                            const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&wk[b]));
+                            const __half2 hv = *reinterpret_cast<const __half2 *>(&wv[b]);
+                            const float2 c = __half22float2(hv);
+                            dk[h][2 * b] = a.x; dk[h][2 * b + 1] = a.y;
+                            dv[h][2 * b] = c.x; dv[h][2 * b + 1] = c.y;
+                            dtop = __hmax2_nan(dtop, __habs2(hv));
+                        }
+                    }
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) s[nb][c] = 0.f;
+#pragma unroll
+                    for (int b = 0; b < NBLK; ++b) {
+                        const uint32_t w0 = *reinterpret_cast<const uint32_t *>(kq + b * bstep + g8 * 16 + t4 * 4);
+                        const uint32_t w1 = *reinterpret_cast<const uint32_t *>(kq + b * bstep + (g8 + 8) * 16 + t4 * 4);
+                        const uint32_t lo[4] = {w0 & 0x000F000Fu, w1 & 0x000F000Fu, (w0 >> 8) & 0x000F000Fu, (w1 >> 8) & 0x000F000Fu};
+                        const uint32_t hi[4] = {w0 & 0x00F000F0u, w1 & 0x00F000F0u, (w0 >> 8) & 0x00F000F0u, (w1 >> 8) & 0x00F000F0u};
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            float acc[4] = {bias[nb][b][0], bias[nb][b][1], bias[nb][b][0], bias[nb][b][1]};
+#pragma unroll
+                            for (int n = NT - 1; n >= 0; --n) {
+                                uint2 f0, f1;
+                                if constexpr (T::Q_SMEM) {
+                                    f0 = qf[((n * NB + nb) * KS + 2 * b) * 32 + lane];
+                                    f1 = qf[((n * NB + nb) * KS + 2 * b + 1) * 32 + lane];
+                                } else {
+                                    f0 = make_uint2(qr[n][nb][2 * b][0], qr[n][nb][2 * b][1]);
+                                    f1 = make_uint2(qr[n][nb][2 * b + 1][0], qr[n][nb][2 * b + 1][1]);
+                                }
+                                mma_f16(acc, lo, f0.x, f0.y);
+                                mma_f16(acc, hi, f1.x, f1.y);
+                            }
+                            s[nb][0] = fmaf(acc[0], dk[0][b], s[nb][0]);
+                            s[nb][1] = fmaf(acc[1], dk[0][b], s[nb][1]);
+                            s[nb][2] = fmaf(acc[2], dk[1][b], s[nb][2]);
+                            s[nb][3] = fmaf(acc[3], dk[1][b], s[nb][3]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) s[nb][c] = 0.f;
+                    const int row = (lane & 7) + (lane & 8);
+                    const uint32_t base = skn_smem_u32(kt) + row * 128;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const int c = 2 * k + (lane >> 4);
+                        uint32_t a[4];
+                        ldsm4(a, base + (c >> 3) * 2048 + (((c & 7) ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int n = NT - 1; n >= 0; --n) {
+                                uint2 f;
+                                if constexpr (T::Q_SMEM) f = qf[((n * NB + nb) * KS + k) * 32 + lane];
+                                else f = make_uint2(qr[n][nb][k][0], qr[n][nb][k][1]);
+                                mma_as<CT>(s[nb], a, f.x, f.y);
+                            }
+                    }
+                }
+                // ---- weights -----------------------------------------------------------------------------------------------
+                bool move = false;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        s[nb][c] *= cs[nb][c & 1];
+                        if (!whole && (hidden_page || !paged_sees(p, key0 + g8 + 8 * (c >> 1), pos[nb][c & 1]))) s[nb][c] = -INFINITY;
+                        move |= s[nb][c] > m[nb][c & 1] + (float)T::SLACK;
+                    }
+                if constexpr (T::Q4) move |= !__hble2(dtop, vlim);
+                if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float top = fmaxf(s[nb][c], s[nb][c + 2]);
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                            top = fmaxf(top, m[nb][c]);
+                            const float fix = exp2f(m[nb][c] - top);
+                            m[nb][c] = top;
+                            l[nb][c] *= fix;
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i) {
+                                o[i][nb][c] *= fix;
+                                o[i][nb][c + 2] *= fix;
+                            }
+                        }
+                    if constexpr (T::Q4) {
+                        // scales of V: those of keys that nobody sees count for nothing; the largest of the others decides E
+                        float top = 0.f;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int key = key0 + g8 + 8 * h;
+                            bool some = false;
+                            for (int t = g.row0 / p.group; t <= (g.row0 + g.rows - 1) / p.group; ++t) some |= !hidden_page && paged_sees(p, key, g.len - g.n + t);
+#pragma unroll
+                            for (int b = 0; b < NBLK; ++b) {
+                                if (!some) dv[h][b] = 0.f;
+                                if (fabsf(dv[h][b]) < INFINITY) top = fmaxf(top, fabsf(dv[h][b]));
+                            }
+                        }
+#pragma unroll
+                        for (int o2 = 1; o2 < 32; o2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
+                        if (top > __half2float(__low2half(vlim))) {
+                            // up to LIFT: weights stay within 2^15
+                            const int e = (int)(__float_as_uint(top) >> 23) - 127 - T::V_UP;
+                            const float fresh = __uint_as_float((uint32_t)(127 - e) << 23), fix = fresh * ve_inv;
+                            ve = fresh;
+                            ve_inv = __uint_as_float((uint32_t)(127 + e) << 23);
+                            vlim = __float2half2_rn(fminf(ve_inv * T::LIFT, 65504.f));
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                                    for (int c = 0; c < 4; ++c) o[i][nb][c] *= fix;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        s[nb][c] = exp2f(s[nb][c] - m[nb][c & 1]);
+                        l[nb][c & 1] += s[nb][c];
+                    }
+                // ---- values ------------------------------------------------------------------------------------------------
+                if constexpr (T::Q4) {
+                    // 1024 + q or 1024 + 16 q in fp16, then q - 8: exact, so that a value of zero adds nothing
+                    const uint32_t mask = g8 & 4 ? 0x00F000F0u : 0x000F000Fu;
+                    const __half2 vmul = __float2half2_rn(g8 & 4 ? 0.0625f : 1.f), vadd = __float2half2_rn(g8 & 4 ? -72.f : -1032.f);
+                    auto less8 = [&](uint32_t x) {
+                        const uint32_t y = (x & mask) | 0x64006400u;
+                        const __half2 z = __hfma2(*reinterpret_cast<const __half2 *>(&y), vmul, vadd);
+                        return *reinterpret_cast<const uint32_t *>(&z);
+                    };
+#pragma unroll
+                    for (int b = 0; b < NBLK; ++b) {
+                        uint32_t pb[NB][NT][2];
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const float d0 = dv[0][b] * ve, d1 = dv[1][b] * ve;
+                            const float w0 = s[nb][0] * d0, w1 = s[nb][1] * d0, w2 = s[nb][2] * d1, w3 = s[nb][3] * d1;
+                            uint32_t a[NT], c[NT];
+                            terms_of<CT, NT>(w0, w1, a);
+                            terms_of<CT, NT>(w2, w3, c);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                pb[nb][n][0] = movm(a[n]);
+                                pb[nb][n][1] = movm(c[n]);
+                            }
+                        }
+                        const uint8_t *at = vq + b * bstep + 2 * t4 * 16 + (g8 & 3) * 4;
+                        const uint32_t x0 = *reinterpret_cast<const uint32_t *>(at), x1 = *reinterpret_cast<const uint32_t *>(at + 16);
+                        const uint32_t x2 = *reinterpret_cast<const uint32_t *>(at + 128), x3 = *reinterpret_cast<const uint32_t *>(at + 144);
+                        const uint32_t lo = __byte_perm(x0, x1, 0x5410), lo2 = __byte_perm(x2, x3, 0x5410), hi = __byte_perm(x0, x1, 0x7632), hi2 = __byte_perm(x2, x3, 0x7632);
+                        const uint32_t a0[4] = {less8(lo), less8(lo >> 8), less8(lo2), less8(lo2 >> 8)};
+                        const uint32_t a1[4] = {less8(hi), less8(hi >> 8), less8(hi2), less8(hi2 >> 8)};
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int n = NT - 1; n >= 0; --n) {
+                                mma_f16(o[2 * b][nb], a0, pb[nb][n][0], pb[nb][n][1]);
+                                mma_f16(o[2 * b + 1][nb], a1, pb[nb][n][0], pb[nb][n][1]);
+                            }
+                    }
+                } else {
+                    uint32_t pb[NB][NT][2];
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        uint32_t a[NT], c[NT];
+                        terms_of<CT, NT>(s[nb][0] * T::LIFT, s[nb][1] * T::LIFT, a);
+                        terms_of<CT, NT>(s[nb][2] * T::LIFT, s[nb][3] * T::LIFT, c);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            pb[nb][n][0] = movm(a[n]);
+                            pb[nb][n][1] = movm(c[n]);
+                        }
+                    }
+                    const int row = (lane & 7) + ((lane & 16) >> 1);
+                    const uint32_t base = skn_smem_u32(vt) + row * 128;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const int c = 2 * i + ((lane >> 3) & 1);
+                        uint32_t a[4];
+                        ldsm4t(a, base + (c >> 3) * 2048 + (((c & 7) ^ (row & 7)) << 4));
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int n = NT - 1; n >= 0; --n) mma_as<CT>(o[i][nb], a, pb[nb][n][0], pb[nb][n][1]);
+                    }
+                }
+            }
+            __syncwarp();                          // the stage is read
+            if (issued < n_mine) {
+                if ((issued & 31) == 0) look_up(issued);
+                issue(issued, stage);
+                ++issued;
+            }
+            if (++stage == STAGES) {
+                stage = 0;
+                parity ^= 1;
+            }
+        }
+        // ---- the warps' results -----------------------------------------------------------------------------------------------
+        __syncthreads();                           // every ring is empty: the results lie over them
+        float *comb = reinterpret_cast<float *>(ring);
+        {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float x = l[nb][c];
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    const int r = 8 * nb + 2 * t4 + c;
+                    if (g8 == 0) {
+                        wml[warp][2 * r] = m[nb][c];
+                        wml[warp][2 * r + 1] = x;
+                    }
+                    float *to = comb + (warp * ROWS + r) * (D + 4);
+                    if constexpr (T::Q4) {
+#pragma unroll
+                        for (int b = 0; b < NBLK; ++b) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) {
+                                const int d = 32 * b + 4 * (g8 & 3) + 16 * (g8 >> 2) + 2 * i;
+                                *reinterpret_cast<float2 *>(to + d) = make_float2(o[2 * b + i][nb][c] * ve_inv, o[2 * b + i][nb][c + 2] * ve_inv);
+                            }
+                        }
+                    } else {
+                        constexpr float DOWN = 1.f / T::LIFT;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            to[16 * i + g8] = o[i][nb][c] * DOWN;
+                            to[16 * i + g8 + 8] = o[i][nb][c + 2] * DOWN;
+                        }
+                    }
+                }
+            __syncthreads();
+            // maximum, sum and output of all warps
+            if (tid < ROWS) {
+                float top = PA_NONE;
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, wml[w][2 * tid]);
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) {
+                    const float f = exp2f(wml[w][2 * tid] - top);
+                    sum += wml[w][2 * tid + 1] * f;
+                    wml[w][2 * tid] = f;
+                }
+                rml[2 * tid] = top;
+                rml[2 * tid + 1] = sum;
+            }
+            __syncthreads();
+            for (int i = tid; i < ROWS * (D / 4); i += PA_THREADS) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) {
+                    const float f = wml[w][2 * r];
+                    const float4 y = *reinterpret_cast<const float4 *>(comb + (w * ROWS + r) * (D + 4) + d);
+                    if (f != 0.f) { x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w); }
+                }
+                *reinterpret_cast<float4 *>(comb + r * (D + 4) + d) = x;        // (warp 0's place: read by this thread alone)
+                const float sum = (x.x + x.y) + (x.z + x.w) + rml[2 * r + 1];
+                if (!(fabsf(sum) < INFINITY) && r < g.rows) flags[0] = 1;       // (a sum of finite values that overflows is computed again for nothing)
+            }
+            __syncthreads();
+            if (flags[0]) {
+                paged_redo<CT, D, IO>(p, g, UNIT, comb, rml, scratch);
+                if (tid == 0) flags[0] = 0;
+            }
+        }
+        // ---- out, or to the other CTAs of the segment ---------------------------------------------------------------------------
+        bool last = true;
+        if (g.n_parts > 1) {
+            float *part = p.parts + (int64_t)g.slot * SKN_PAGED_PART_ROWS * (D + 4);
+            for (int i = tid; i < g.rows * (D / 4); i += PA_THREADS) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                const float4 x = *reinterpret_cast<const float4 *>(comb + r * (D + 4) + d);
+                *reinterpret_cast<float4 *>(part + r * (D + 4) + d) = x;
+            }
+            if (tid < g.rows) {
+                part[tid * (D + 4) + D] = rml[2 * tid];
+                part[tid * (D + 4) + D + 1] = rml[2 * tid + 1];
+            }
+            __threadfence();
+            __syncthreads();
+            // the first CTA's slot: 0 where the segment is the first of its share
+            const long long a = u - (g.u1 - g.u0) - g.u0;
+            auto slot_of = [&](int c) { return 2 * c + (c == g.c0 && total * c / n_cta < a); };
+            if (tid == 0) ticket = atomicInc(&p.tickets[slot_of(g.c0)], (unsigned)g.n_parts - 1);
+            __syncthreads();
+            last = ticket == (unsigned)g.n_parts - 1;
+            if (last) {
+                __threadfence();
+                for (int i = tid; i < g.rows * (D / 4); i += PA_THREADS) {
+                    const int r = i / (D / 4), d = i % (D / 4) * 4;
+                    float top = PA_NONE;
+                    for (int k = 0; k < g.n_parts; ++k)
+                        top = fmaxf(top, __ldcg(p.parts + ((int64_t)slot_of(g.c0 + k) * SKN_PAGED_PART_ROWS + r) * (D + 4) + D));
+                    float sum = 0.f;
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int k = 0; k < g.n_parts; ++k) {
+                        const float *from = p.parts + ((int64_t)slot_of(g.c0 + k) * SKN_PAGED_PART_ROWS + r) * (D + 4);
+                        const float f = exp2f(__ldcg(from + D) - top);
+                        if (f == 0.f) continue;
+                        sum = fmaf(__ldcg(from + D + 1), f, sum);
+                        const float4 y = __ldcg(reinterpret_cast<const float4 *>(from + d));
+                        x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+                    }
+                    *reinterpret_cast<float4 *>(comb + r * (D + 4) + d) = x;
+                    if (d == 0) rml[2 * r + 1] = sum;
+                }
+                __syncthreads();
+            }
+        }
+        if (last) {
+            for (int i = tid; i < g.rows * (D / 8); i += PA_THREADS) {
+                const int r = i / (D / 8), d = i % (D / 8) * 8, t = (g.row0 + r) / p.group;
+                const float sum = rml[2 * r + 1];
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = sum == 0.f ? 0.f : comb[r * (D + 4) + d + k] / sum;
+                io_store8(static_cast<IO *>(p.out) + (int64_t)(g.first + t) * p.out_stride + (g.head * p.group + (g.row0 + r) % p.group) * D + d, x);
+            }
+        }
+        skn_fence_proxy_async();                   // the rings were written to as results
+        __syncthreads();
+    }
+}
+
+// ---- launches ---------------------------------------------------------------------------------------------------------------
+template <class CT, int D, int NB, bool EX> static cudaError_t attn_launch(const skn_paged *pc, const PagedAttn &p) {
+    using T = PaTraits<CT, D, NB, EX>;
+    auto *kern = skn_paged_attn_kernel<CT, D, NB, EX>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t rows = (int64_t)p.st.max_new * p.group;
+    const dim3 grid = p.direct ? dim3((unsigned)((rows + T::ROWS - 1) / T::ROWS), (unsigned)p.st.heads, (unsigned)p.st.n_seqs) : dim3((unsigned)(T::PER_SM * pc->ctx->sm_count));
+    kern<<<grid, PA_THREADS, T::SMEM, pc->ctx->stream>>>(p, pc->map[0], pc->map[1], pc->map[2], pc->map[3]);
+    return cudaGetLastError();
+}
+template <class CT, int D, bool EX> static cudaError_t attn_by_rows(const skn_paged *pc, PagedAttn &p) {
+    const int64_t rows = (int64_t)p.st.max_new * p.group;
+    p.direct = rows > SKN_PAGED_PART_ROWS || p.st.n_seqs > PA_MAX_SEQS;
+    return rows <= 8 ? attn_launch<CT, D, 1, EX>(pc, p) : rows <= 16 ? attn_launch<CT, D, 2, EX>(pc, p) : attn_launch<CT, D, 4, EX>(pc, p);
+}
+template <class CT> static cudaError_t attn_by_type(const skn_paged *pc, int32_t io, PagedAttn &p) {
+    if (pc->spec.head_dim == 64) return io == SKN_KV_F32 ? attn_by_rows<CT, 64, true>(pc, p) : attn_by_rows<CT, 64, false>(pc, p);
+    return io == SKN_KV_F32 ? attn_by_rows<CT, 128, true>(pc, p) : attn_by_rows<CT, 128, false>(pc, p);
+}
+
+cudaError_t skn_paged_attn_f16(const skn_paged *pc, int32_t io, PagedAttn &p);
+cudaError_t skn_paged_attn_bf16(const skn_paged *pc, int32_t io, PagedAttn &p);
+cudaError_t skn_paged_attn_q4(const skn_paged *pc, int32_t io, PagedAttn &p);

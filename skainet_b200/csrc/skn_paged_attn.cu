@@ -1,5 +1,5 @@
 // Attention over the paged KV cache: tensor maps, workspace and the choice of the kernel.
-#include "skn_paged_attn.cuh"
+#include "skn_paged_prompt.cuh"
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 static cudaError_t encode(CUtensorMap *map, CUtensorMapDataType type, int rank, void *base, const cuuint64_t *dim, const cuuint64_t *stride, const cuuint32_t *box,
@@ -25,19 +25,23 @@ cudaError_t skn_paged_attn_prepare(skn_paged *pc) {
             const cuuint64_t dim[3] = {64, heads * P, (cuuint64_t)D / 64}, stride[2] = {(cuuint64_t)D * 2, 128};
             const cuuint32_t box[3] = {64, 16, (cuuint32_t)D / 64};
             e = encode(&pc->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, pool, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_128B);
+            const cuuint32_t whole[3] = {64, (cuuint32_t)P, 1};
+            if (e == cudaSuccess) e = encode(&pc->wide[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, pool, dim, stride, whole, CU_TENSOR_MAP_SWIZZLE_128B);
         } else {
             const cuuint32_t rows = P < 32 ? P : 32;
             // quants of 16 or 32 rows, in words: [D / 32][rows][4]; scales [rows][D / 32], two to a word
             const cuuint64_t dim[3] = {(cuuint64_t)P * 4, (cuuint64_t)D / 32, heads}, stride[2] = {(cuuint64_t)P * 16, (cuuint64_t)pc->head_bytes};
             const cuuint32_t box[3] = {rows * 4, (cuuint32_t)D / 32, 1};
             e = encode(&pc->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, pool, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+            pc->wide[i] = pc->map[i];
             const cuuint64_t sdim[2] = {(cuuint64_t)P * D / 64, heads}, sstride[1] = {(cuuint64_t)pc->head_bytes};
             const cuuint32_t sbox[2] = {rows * (cuuint32_t)D / 64, 1};
             if (e == cudaSuccess) e = encode(&pc->map[2 + i], CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, pool + (size_t)P * D / 2, sdim, sstride, sbox, CU_TENSOR_MAP_SWIZZLE_NONE);
         }
     }
     pc->n_parts = 2 * pc->ctx->sm_count;
-    const size_t parts = (size_t)2 * pc->n_parts * SKN_PAGED_PART_ROWS * (D + 4) * sizeof(float);
+    const size_t decode_rows = (size_t)2 * pc->n_parts * SKN_PAGED_PART_ROWS, prompt_rows = (size_t)2 * pc->ctx->sm_count * PP_ROWS;
+    const size_t parts = (decode_rows > prompt_rows ? decode_rows : prompt_rows) * (D + 4) * sizeof(float);
     if (e == cudaSuccess) e = cudaMalloc((void **)&pc->d_parts, parts);
     if (e == cudaSuccess) e = cudaMalloc((void **)&pc->d_tickets, (size_t)2 * pc->n_parts * sizeof(unsigned));
     if (e == cudaSuccess) e = cudaMemsetAsync(pc->d_tickets, 0, (size_t)2 * pc->n_parts * sizeof(unsigned), pc->ctx->stream);

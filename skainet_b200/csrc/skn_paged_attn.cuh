@@ -110,23 +110,23 @@ struct PagedSegment {
     int c0, n_parts, slot;                // CTAs that have some of it: c0 .. c0 + n_parts - 1
 };
 
-// A segment from the definition: for rows in turn, a thread per key and then a thread per dimension.  Results as the warps' are: maximum (base 2), sum and
-// unnormalised output in `comb`.
-template <class CT, int D, class IO>
-__device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &g, int unit, float *comb, float *ml, float *scratch) {
+// A segment from the definition: for rows in turn, a thread per key and then a thread per dimension (PA_THREADS of them, which `bar` brings together).
+// put(row, maximum (base 2), sum, this thread's dimension of the unnormalised output)
+template <class CT, int D, class IO, class Bar, class Put>
+__device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &g, int unit, float *scratch, Bar bar, Put put) {
     float *qs = scratch, *ps = scratch + D, *red = ps + PA_THREADS;
     const int tid = threadIdx.x;
     for (int r = 0; r < g.rows; ++r) {
         const int t = (g.row0 + r) / p.group, pos = g.len - g.n + t;
         const IO *q = static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + r) % p.group) * D;
-        __syncthreads();
+        bar();
         if (tid < D / 8) {
             float x[8];
             io_load8(q + 8 * tid, x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) qs[8 * tid + i] = x[i];
         }
-        __syncthreads();
+        bar();
         float m = PA_NONE, l = 0.f, acc = 0.f;
         for (int b = g.u0 * unit; b < g.u1 * unit; b += PA_THREADS) {
             auto key_of = [&](int i) { const int u = i / unit; return (u < g.span.a ? u : u + g.span.gap) * unit + i % unit; };
@@ -152,7 +152,7 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
 #pragma unroll
             for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             if ((tid & 31) == 0) red[tid >> 5] = top;
-            __syncthreads();
+            bar();
             top = m;
 #pragma unroll
             for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, red[w]);
@@ -161,9 +161,9 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
             float sum = w;
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            __syncthreads();
+            bar();
             if ((tid & 31) == 0) red[tid >> 5] = sum;
-            __syncthreads();
+            bar();
             l *= fix;
 #pragma unroll
             for (int k = 0; k < PA_WARPS; ++k) l += red[k];
@@ -181,15 +181,11 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
                     for (int e = 1; e < 8; ++e) v = (tid & 7) == e ? x[e] : v;
                     acc = fmaf(ps[j], v, acc);
                 }
-            __syncthreads();
+            bar();
         }
-        if (tid < D) comb[r * (D + 4) + tid] = acc;
-        if (tid == 0) {
-            ml[2 * r] = m;
-            ml[2 * r + 1] = l;
-        }
+        put(r, m, l, acc);
     }
-    __syncthreads();
+    bar();
 }
 
 template <class CT, int D, int NB, bool EX> struct PaTraits {
@@ -856,7 +852,13 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             }
             __syncthreads();
             if (flags[0]) {
-                paged_redo<CT, D, IO>(p, g, UNIT, comb, rml, scratch);
+                paged_redo<CT, D, IO>(p, g, UNIT, scratch, [] { __syncthreads(); }, [&](int r, float rm, float rl, float acc) {
+                    if (tid < D) comb[r * (D + 4) + tid] = acc;
+                    if (tid == 0) {
+                        rml[2 * r] = rm;
+                        rml[2 * r + 1] = rl;
+                    }
+                });
                 if (tid == 0) flags[0] = 0;
             }
         }
@@ -930,8 +932,14 @@ template <class CT, int D, int NB, bool EX> static cudaError_t attn_launch(const
     kern<<<grid, PA_THREADS, T::SMEM, pc->ctx->stream>>>(p, pc->map[0], pc->map[1], pc->map[2], pc->map[3]);
     return cudaGetLastError();
 }
+// bf16 rows of prompts (skn_paged_prompt.cuh); the first argument names the cache type
+cudaError_t skn_paged_prompt(__half, const skn_paged *pc, const PagedAttn &p);
+cudaError_t skn_paged_prompt(__nv_bfloat16, const skn_paged *pc, const PagedAttn &p);
+cudaError_t skn_paged_prompt(skn_q4, const skn_paged *pc, const PagedAttn &p);
+
 template <class CT, int D, bool EX> static cudaError_t attn_by_rows(const skn_paged *pc, PagedAttn &p) {
     const int64_t rows = (int64_t)p.st.max_new * p.group;
+    if (!EX && rows > SKN_PAGED_PART_ROWS) return skn_paged_prompt(CT(), pc, p);
     p.direct = rows > SKN_PAGED_PART_ROWS || p.st.n_seqs > PA_MAX_SEQS;
     return rows <= 8 ? attn_launch<CT, D, 1, EX>(pc, p) : rows <= 16 ? attn_launch<CT, D, 2, EX>(pc, p) : attn_launch<CT, D, 4, EX>(pc, p);
 }

@@ -1,0 +1,696 @@
+// Attention of prompts over the paged KV cache: bf16 rows, more than the 32 rows per kv head that the kernel of skn_paged_attn.cuh takes at a time.
+//
+// 256 rows (tokens x query heads of one kv head) in two tiles of 128 against 128 keys at a time, on tcgen05: S = Q K^T and O += P V with S, O and P in tensor
+// memory (P in fp16, bf16 for bf16 caches, over its own S: the first operand of the second product), Q, K and V in shared memory with 128-byte swizzle, V
+// as the transposed second operand.  A thread of the two softmax warpgroups owns a row: its maximum and sum need no exchange.  The maximum moves only
+// when a weight would exceed 2^SLACK; O is then scaled where it is, by the same threads.  While one tile's softmax runs, the tensor cores work
+// on the other tile.  One warp issues the MMAs, one the TMA loads (a box per page, or 128 rows of larger ones).  Q4_0: a warpgroup turns quants into
+// fp16 (q - 8) d between the two.
+//
+// Work is shared out as in skn_paged_attn.cuh: the units (128 keys of a block of rows) of all blocks form one line, one contiguous share for each CTA;
+// blocks that lie in several shares are joined by the last of their CTAs to finish.
+//
+// Hidden rows of V (behind the last key that the block sees, before its window, on pages that were given back) are cleared in shared memory before the
+// product: a warp does it in the few units that have some.  A result that is not finite is computed again from the definition.
+#pragma once
+#include "skn_paged_attn.cuh"
+
+constexpr int PP_ROWS = 256, PP_KEYS = 128;
+
+template <class CT, int D> struct PpTraits {
+    static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
+    static constexpr int THREADS = Q4 ? 512 : 384;                // two softmax warpgroups, one of MMA / TMA / clearing, one of unpacking
+    static constexpr int TILE = PP_KEYS * D * 2;                  // K or V of a unit in 16 bits; also one tile of Q
+    static constexpr int SLOTS = Q4 ? 3 : D == 64 ? 6 : 4;        // K and V in turn
+    static_assert(Q4 || SLOTS % 2 == 0, "V always in the same slots");
+    static constexpr int HALF = (16 * (D / 2 + D / 16) + 127) / 128 * 128;
+    static constexpr int RAW = Q4 ? 8 * HALF : 0, RAW_SLOTS = Q4 ? 4 : 0;
+    static constexpr size_t SMEM = 1024 + 2 * TILE + (size_t)SLOTS * TILE + (size_t)RAW_SLOTS * RAW;
+    static constexpr int SLACK = 4;
+    static constexpr float LIFT = BF ? 0.f : 11.f;                // exponent: fp16 weights up to 2^15 (see skn_paged_attn.cuh)
+};
+
+__device__ __forceinline__ void pp_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ bool pp_any(bool x) {
+    uint32_t y;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(y) : "r"((uint32_t)x) : "memory");
+    return y != 0;
+}
+// B operand that lies [k][64 n] (n contiguous, 128-byte swizzle): 64-wide pieces of n `lead` bytes apart, groups of eight k 1024
+__device__ __forceinline__ uint64_t pp_desc_n(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// 32 columns into registers; the caller waits for all of its loads at once
+__device__ __forceinline__ void pp_ld32(uint32_t taddr, float *r) {
+    uint32_t *u = reinterpret_cast<uint32_t *>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]),
+          "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]),
+          "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(taddr));
+}
+// ... after which they may be used (and not before: the empty statements keep the compiler from moving a use up)
+template <int N> __device__ __forceinline__ void pp_wait_ld(float *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(r[i]));
+}
+__device__ __forceinline__ void pp_st32(uint32_t taddr, const uint32_t *u) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]),
+          "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]),
+          "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ float pp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A CTA's share of the line, segment by segment; every role walks it for itself
+struct PpWalk {
+    long long u, u_begin, u_end, total, a;      // a: where the present block and head begin
+    int n_cta, seq, rb, head;
+    PagedSeq sq;
+};
+__device__ __forceinline__ int pp_blocks(const PagedAttn &p, const PagedSeq &q) { return (int)(((long long)q.n * p.group + PP_ROWS - 1) / PP_ROWS); }
+__device__ __forceinline__ PagedSpan pp_span(const PagedAttn &p, const PagedSeq &q, int rb) {
+    const long long r0 = (long long)rb * PP_ROWS, r1 = min(r0 + PP_ROWS, (long long)q.n * p.group) - 1;
+    return paged_span(p, q.len - q.n + (int)(r0 / p.group), q.len - q.n + (int)(r1 / p.group), PP_KEYS);
+}
+__device__ __forceinline__ bool pp_next(const PagedAttn &p, PpWalk &w, PagedSegment &g) {
+    if (w.u >= w.u_end) return false;
+    for (;;) {                                   // the block that holds u
+        const int nb = w.seq < p.st.n_seqs ? pp_blocks(p, w.sq) : 0;
+        if (w.seq >= p.st.n_seqs) return false;
+        if (w.rb < nb) {
+            g.span = pp_span(p, w.sq, w.rb);
+            if (w.u < w.a + g.span.units) break;
+            w.a += g.span.units;
+            if (++w.head == p.st.heads) {
+                w.head = 0;
+                ++w.rb;
+            }
+            continue;
+        }
+        w.rb = w.head = 0;
+        if (++w.seq < p.st.n_seqs) w.sq = paged_seq(p.st, w.seq);
+    }
+    g.seq = w.seq; g.head = w.head; g.first = w.sq.first; g.n = w.sq.n; g.len = w.sq.len;
+    g.row0 = w.rb * PP_ROWS;
+    g.rows = min(PP_ROWS, w.sq.n * p.group - g.row0);
+    g.u0 = (int)(w.u - w.a);
+    g.u1 = (int)min((long long)g.span.units, w.u_end - w.a);
+    g.c0 = (int)(((w.a + 1) * w.n_cta - 1) / w.total);
+    g.n_parts = (int)(((w.a + g.span.units) * w.n_cta - 1) / w.total) - g.c0 + 1;
+    g.slot = 2 * (int)blockIdx.x + (w.u == w.u_begin ? 0 : 1);
+    w.u += g.u1 - g.u0;
+    return true;
+}
+
+// Whether some key of the segment's unit j is seen by nobody (or may be: the first tokens' last unit and the window's first one count as such)
+__device__ __forceinline__ bool pp_hides(const PagedAttn &p, const PagedSegment &g, int j) {
+    const int i = g.u0 + j, k0 = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS;
+    const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
+    const int from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
+    return k0 + PP_KEYS - 1 > pmax || (k0 < from && k0 + PP_KEYS > p.sinks);
+}
+
+template <class CT, int D>
+__global__ void __launch_bounds__(PpTraits<CT, D>::THREADS, 1)
+skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                        const __grid_constant__ CUtensorMap mks, const __grid_constant__ CUtensorMap mvs) {
+    using T = PpTraits<CT, D>;
+    using IO = __nv_bfloat16;
+    constexpr int THREADS = T::THREADS, SLOTS = T::SLOTS, TILE = T::TILE, NBLK = D / 32;
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t *const base = reinterpret_cast<uint8_t *>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
+    uint8_t *const q_tile = base, *const ring = base + 2 * TILE, *const raw_ring = ring + SLOTS * TILE;
+    __shared__ uint64_t full[SLOTS], empty[SLOTS], raw_full[4], raw_empty[4];
+    __shared__ uint64_t s_full[2], p_full[2], pv_done[2], q_full[2], o_free[2], clean[SLOTS];
+    __shared__ long long warp_sum[THREADS / 32];
+    __shared__ long long found_at;
+    __shared__ int found[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ unsigned ticket;
+    __shared__ float scratch[D + PA_THREADS + PA_WARPS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const PagedStep &st = p.st;
+
+    if (tid == 0) {
+        for (int i = 0; i < SLOTS; ++i) {
+            skn_mbar_init(&full[i], T::Q4 ? 4 : 1);
+            skn_mbar_init(&empty[i], 1);
+            skn_mbar_init(&clean[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            skn_mbar_init(&raw_full[i], 1);
+            skn_mbar_init(&raw_empty[i], 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            skn_mbar_init(&s_full[i], 1);
+            skn_mbar_init(&p_full[i], 4);
+            skn_mbar_init(&pv_done[i], 1);
+            skn_mbar_init(&q_full[i], 4);
+            skn_mbar_init(&o_free[i], 4);
+        }
+        skn_fence_mbar_init();
+        found[0] = -1;
+    }
+
+    // ---- the line: items are the blocks of all sequences, each of them units x heads long ----------------------------------
+    PpWalk w;
+    {
+        // total first, then the block in which this CTA's share begins
+        long long share = -1;
+        for (int pass = 0; pass < 2; ++pass) {
+            long long run = 0;
+            int seq = 0, skip = tid;                 // this thread's item: block `skip` counted from sequence `seq`
+            PagedSeq sq = paged_seq(st, 0);
+            for (;;) {
+                while (seq < st.n_seqs && skip >= pp_blocks(p, sq)) {
+                    skip -= pp_blocks(p, sq);
+                    if (++seq < st.n_seqs) sq = paged_seq(st, seq);
+                }
+                const bool have = seq < st.n_seqs;
+                const long long x = have ? (long long)pp_span(p, sq, skip).units * st.heads : 0;
+                long long inc = x;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += y;
+                }
+                __syncthreads();
+                if (lane == 31) warp_sum[warp] = inc;
+                __syncthreads();
+                long long at = run + inc - x;
+                for (int i = 0; i < THREADS / 32; ++i) {
+                    if (i < warp) at += warp_sum[i];
+                    run += warp_sum[i];
+                }
+                if (pass && have && at <= share && share < at + x) {
+                    found[0] = seq;
+                    found[1] = skip;
+                    found_at = at;
+                }
+                skip += THREADS;
+                if (!__syncthreads_or(have)) break;
+            }
+            if (pass == 0) {
+                w.total = run;
+                if (run == 0) return;
+                const long long want = (run + 3) / 4;            // four units a CTA at least
+                w.n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
+                if ((int)blockIdx.x >= w.n_cta) return;
+                share = w.u = w.u_begin = run * blockIdx.x / w.n_cta;
+                w.u_end = run * (blockIdx.x + 1) / w.n_cta;
+            }
+        }
+        __syncthreads();
+        w.seq = found[0];
+        w.rb = found[1];
+        w.head = 0;
+        w.a = found_at;
+        w.sq = paged_seq(st, w.seq);
+    }
+    if (warp == 8) tc_alloc(&tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    PagedSegment g;
+
+    // ---- softmax: warps 0 .. 3 rows 0 .. 127 of a block, warps 4 .. 7 the others ---------------------------------------------
+    if (warp < 8) {
+        const int tile = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const uint32_t ts = tmem + tile * 128 + lanes, to = tmem + 256 + tile * D + lanes;
+        uint32_t n_units = 0;                        // of this tile so far
+        bool ok = true;                              // once a wait has run out the share is only walked: the barriers below want every warp
+        while (pp_next(p, w, g)) {
+            const int R = tile * 128 + r;
+            const bool real = R < g.rows, used = tile * 128 < g.rows;
+            const int t = (g.row0 + R) / p.group, pos = real ? g.len - g.n + t : -1;
+            float m = PA_NONE, l = 0.f, cs = 0.f;
+            if (used && ok) {
+                // the tile's queries, for fp16 products times a power of two that brings a row's largest to 2^14 .. 2^15
+                const IO *q = static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + R) % p.group) * D;
+                uint8_t *const qt = q_tile + tile * TILE;
+                float f = 1.f, up = p.scale < 0.f ? -1.f : 1.f;
+                if constexpr (!T::BF) {
+                    float top = 0.f;
+                    if (real)
+#pragma unroll 4
+                        for (int c = 0; c < D / 8; ++c) {
+                            float x[8];
+                            io_load8(q + 8 * c, x);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+                        }
+                    int e = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
+                    e = top > 0.f && top < INFINITY ? max(-120, min(120, e)) : 0;
+                    up *= __uint_as_float((uint32_t)(127 + e) << 23);
+                    f = __uint_as_float((uint32_t)(127 - e) << 23);
+                }
+                // (a scale of zero moves into the queries: hidden scores of minus infinity stay what they are)
+                if (p.scale == 0.f) up = 0.f;
+                cs = (p.scale == 0.f ? 1.f : fabsf(p.scale)) * f;
+#pragma unroll 4
+                for (int c = 0; c < D / 8; ++c) {
+                    float x[8] = {};
+                    if (real) io_load8(q + 8 * c, x);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] *= up;
+                    uint4 v;
+                    if constexpr (T::BF) v = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+                    else v = make_uint4(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+                    *reinterpret_cast<uint4 *>(qt + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+                }
+                skn_fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) skn_mbar_arrive(&q_full[tile]);
+                const int ta = (g.row0 + tile * 128) / p.group, tb = (g.row0 + min(tile * 128 + 127, g.rows - 1)) / p.group;
+                const int pmin = g.len - g.n + ta, pmax = g.len - g.n + tb;
+
+                for (int j = 0; j < g.u1 - g.u0; ++j, ++n_units) {
+                    const int i = g.u0 + j, k0 = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS;
+                    if (!tc_wait_warp(&s_full[tile], n_units & 1, lane)) { ok = false; break; }
+                    tc_fence_after();
+                    float v[PP_KEYS];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) pp_ld32(ts + 32 * c, v + 32 * c);
+                    pp_wait_ld<PP_KEYS>(v);
+                    const bool whole = k0 + PP_KEYS - 1 <= pmin && (!p.window || k0 > pmax - p.window || k0 + PP_KEYS <= p.sinks);
+                    if (!whole) {
+                        const int hi = pos - k0, lo = p.window ? pos - p.window + 1 - k0 : -1, sk = p.sinks - k0;
+#pragma unroll
+                        for (int c = 0; c < PP_KEYS; ++c)
+                            if (c > hi || (c < lo && c >= sk)) v[c] = -INFINITY;
+                    }
+                    float top = fmaxf(v[0], v[1]);
+#pragma unroll
+                    for (int c = 2; c < PP_KEYS; c += 2) top = fmaxf(top, fmaxf(v[c], v[c + 1]));
+                    top *= cs;
+                    if (__any_sync(0xffffffffu, top > m + (float)T::SLACK)) {
+                        const float fresh = fmaxf(m, top), fix = pp_ex2(m - fresh);
+                        m = fresh;
+                        l *= fix;
+                        if (j > 0) {
+                            if (!tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane)) { ok = false; break; }
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                float o[32];
+                                pp_ld32(to + c, o);
+                                pp_wait_ld<32>(o);
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) o[k] *= fix;
+                                pp_st32(to + c, reinterpret_cast<uint32_t *>(o));
+                            }
+                            tc_wait_st();
+                        }
+                    }
+                    const float off = T::LIFT - m;
+                    float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            const float a = pp_ex2(fmaf(v[64 * h + 2 * c], cs, off)), b = pp_ex2(fmaf(v[64 * h + 2 * c + 1], cs, off));
+                            sum0 += a;
+                            sum1 += b;
+                            pk[c] = T::BF ? pack_bf16(a, b) : pack_f16(a, b);
+                        }
+                        pp_st32(ts + 32 * h, pk);
+                    }
+                    l += sum0 + sum1;
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) skn_mbar_arrive(&p_full[tile]);
+                }
+                if (ok && g.u1 > g.u0) ok = tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane);
+                if (!ok) {
+                    if (lane == 0) *st.status = SKN_ERR_TIMEOUT;
+                }
+            }
+            // ---- out, or to the other CTAs of the block -------------------------------------------------------------------------
+            const bool shared = g.n_parts > 1;
+            float *part = p.parts + (int64_t)g.slot * PP_ROWS * (D + 4);          // [D / 4][256] float4, then [256] maximum, [256] sum
+            IO *const out = static_cast<IO *>(p.out) + (int64_t)(g.first + t) * p.out_stride + (g.head * p.group + (g.row0 + R) % p.group) * D;
+            bool odd = false;
+            if (used && ok) {
+                tc_fence_after();
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float o[32];
+                    pp_ld32(to + c, o);
+                    pp_wait_ld<32>(o);
+                    float s = 0.f;
+                    if (shared) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            s += (o[k] + o[k + 1]) + (o[k + 2] + o[k + 3]);
+                            reinterpret_cast<float4 *>(part)[((c + k) / 4) * PP_ROWS + R] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            float x[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                x[e] = l == 0.f ? 0.f : o[k + e] * inv;
+                                s += x[e];
+                            }
+                            if (real) io_store8(out + c + k, x);
+                        }
+                    }
+                    odd |= !(fabsf(s) < INFINITY);
+                }
+                odd = real && (odd || !(fabsf(l) < INFINITY));
+                if (shared) {
+                    part[D * PP_ROWS + R] = m;
+                    part[(D + 1) * PP_ROWS + R] = l;
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) skn_mbar_arrive(&o_free[tile]);
+            }
+            if (pp_any(odd))
+                paged_redo<CT, D, IO>(p, g, PP_KEYS, scratch, [] { pp_bar(); }, [&](int row, float rm, float rl, float acc) {
+                    const int tr = (g.row0 + row) / p.group;
+                    if (shared) {
+                        if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;
+                        if (tid == 0) {
+                            part[D * PP_ROWS + row] = rm + T::LIFT;      // (its weights are not lifted)
+                            part[(D + 1) * PP_ROWS + row] = rl;
+                        }
+                    } else if (tid < D)
+                        static_cast<IO *>(p.out)[(int64_t)(g.first + tr) * p.out_stride + (g.head * p.group + (g.row0 + row) % p.group) * D + tid] =
+                            __float2bfloat16_rn(rl == 0.f ? 0.f : acc / rl);
+                });
+            if (shared) {
+                __threadfence();
+                pp_bar();
+                const long long a = w.u - g.u1;                    // where the block begins
+                auto slot_of = [&](int c) { return 2 * c + (c == g.c0 && w.total * c / w.n_cta < a); };
+                if (tid == 0) ticket = atomicInc(&p.tickets[slot_of(g.c0)], (unsigned)g.n_parts - 1);
+                pp_bar();
+                if (ticket == (unsigned)g.n_parts - 1 && real) {
+                    __threadfence();
+                    float top = PA_NONE, sum = 0.f;
+                    for (int k = 0; k < g.n_parts; ++k) top = fmaxf(top, __ldcg(p.parts + (int64_t)slot_of(g.c0 + k) * PP_ROWS * (D + 4) + D * PP_ROWS + R));
+                    for (int k = 0; k < g.n_parts; ++k) {
+                        const float *from = p.parts + (int64_t)slot_of(g.c0 + k) * PP_ROWS * (D + 4);
+                        sum = fmaf(__ldcg(from + (D + 1) * PP_ROWS + R), exp2f(__ldcg(from + D * PP_ROWS + R) - top), sum);
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        float4 o[8] = {};
+                        for (int k = 0; k < g.n_parts; ++k) {
+                            const float *from = p.parts + (int64_t)slot_of(g.c0 + k) * PP_ROWS * (D + 4);
+                            const float f = exp2f(__ldcg(from + D * PP_ROWS + R) - top);
+                            if (f == 0.f) continue;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float4 y = __ldcg(reinterpret_cast<const float4 *>(from) + (c / 4 + e) * PP_ROWS + R);
+                                o[e].x = fmaf(y.x, f, o[e].x); o[e].y = fmaf(y.y, f, o[e].y); o[e].z = fmaf(y.z, f, o[e].z); o[e].w = fmaf(y.w, f, o[e].w);
+                            }
+                        }
+                        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const float x[8] = {o[e].x * inv, o[e].y * inv, o[e].z * inv, o[e].w * inv, o[e + 1].x * inv, o[e + 1].y * inv, o[e + 1].z * inv, o[e + 1].w * inv};
+                            io_store8(out + c + 4 * e, x);
+                        }
+                    }
+                }
+                pp_bar();                            // (the ticket is read)
+            }
+        }
+    }
+    // ---- MMAs: warp 8 --------------------------------------------------------------------------------------------------------
+    else if (warp == 8) {
+        constexpr uint32_t FMT = T::BF ? 1u << 7 | 1u << 10 : 0u;
+        constexpr uint32_t ID_S = 1u << 4 | FMT | (PP_KEYS >> 3) << 17 | 8u << 24, ID_O = 1u << 4 | FMT | 1u << 16 | (D >> 3) << 17 | 8u << 24;
+        int slot = 0, parity = 0;                    // of the next K or V
+        uint32_t units[2] = {0, 0}, segs[2] = {0, 0};
+        bool ok = true;
+        auto step = [&] {
+            if (++slot == SLOTS) {
+                slot = 0;
+                parity ^= 1;
+            }
+        };
+        auto scores = [&](int tile, int at) {        // S of a tile from the keys in slot `at`
+            const uint32_t qa = skn_smem_u32(q_tile + tile * TILE), ka = skn_smem_u32(ring + at * TILE);
+            if (tc_elect()) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+                    tc_mma_bf16(tmem + tile * 128, tc_smem_desc(qa + off), tc_smem_desc(ka + off), ID_S, k > 0);
+                }
+                tc_commit(&s_full[tile]);
+            }
+            __syncwarp();
+        };
+        while (ok && pp_next(p, w, g)) {
+            const int n = g.u1 - g.u0, tiles = g.rows > 128 ? 2 : 1;
+            int k_slot = slot;
+            for (int x = 0; x < tiles && ok; ++x) ok = tc_wait_warp(&q_full[x], segs[x] & 1, lane);
+            ok = ok && tc_wait_warp(&full[slot], parity, lane);
+            if (!ok) break;
+            tc_fence_after();
+            for (int x = 0; x < tiles; ++x) scores(x, slot);
+            if (tc_elect()) tc_commit(&empty[k_slot]);
+            __syncwarp();
+            step();
+            for (int j = 0; j < n && ok; ++j) {
+                const int v_slot = slot;
+                ok = tc_wait_warp(T::Q4 ? &full[slot] : &clean[slot], parity, lane);
+                step();
+                const bool more = j + 1 < n;
+                k_slot = slot;
+                const uint32_t va = skn_smem_u32(ring + v_slot * TILE);
+                for (int x = 0; x < tiles && ok; ++x) {
+                    ok = tc_wait_warp(&p_full[x], units[x] & 1, lane);
+                    if (ok && j == 0 && segs[x] > 0) ok = tc_wait_warp(&o_free[x], (segs[x] - 1) & 1, lane);
+                    if (!ok) break;
+                    ++units[x];
+                    tc_fence_after();
+                    if (tc_elect()) {
+#pragma unroll
+                        for (int k = 0; k < PP_KEYS / 16; ++k)
+                            tc_mma_ts(tmem + 256 + x * D, tmem + x * 128 + 8 * k, pp_desc_n(va + k * 2048, PP_KEYS * 128), ID_O, j > 0 || k > 0);
+                        tc_commit(&pv_done[x]);
+                        if (x == tiles - 1) tc_commit(&empty[v_slot]);
+                    }
+                    __syncwarp();
+                    if (more) {
+                        if (x == 0) ok = tc_wait_warp(&full[k_slot], parity, lane);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(x, k_slot);
+                        if (x == tiles - 1) {
+                            if (tc_elect()) tc_commit(&empty[k_slot]);
+                            __syncwarp();
+                        }
+                    }
+                }
+                if (more) step();
+            }
+            for (int x = 0; x < tiles; ++x) ++segs[x];
+        }
+        if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+    }
+    // ---- loads: warp 9 -----------------------------------------------------------------------------------------------------------
+    else if (warp == 9) {
+        int slot = 0, parity = 0;
+        bool ok = true;
+        uint32_t loads = 0;
+        while (ok && pp_next(p, w, g)) {
+            const int n = g.u1 - g.u0;
+            const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
+            const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
+            // a box is a page's rows, up to 128 (Q4_0: 32); a lane per box of K (16-bit types: and half of the dims)
+            const int box_shift = T::Q4 ? min(st.page_shift, 5) : min(st.page_shift, 7), boxes = PP_KEYS >> box_shift;
+            for (int j = 0; j < n && ok; ++j) {
+                const int i = g.u0 + j, k0 = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS;
+                int page = -1;
+                const int b = lane & (boxes - 1), kb = k0 + (b << box_shift);
+                if (lane < boxes * (T::Q4 ? 1 : D / 64)) {
+                    bool need = false;               // some row sees some of the box
+                    for (int k = kb; k < kb + (1 << box_shift); k += 16) need |= k <= pmax && (k + 15 >= seen_from || k < p.sinks);
+                    if (need) page = paged_page(st, g.seq, kb);
+                }
+                const int count = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                const int row = kb & ((1 << st.page_shift) - 1);
+                for (int kv = 0; kv < 2 && ok; ++kv) {
+                    const CUtensorMap *map = kv ? &mv : &mk;
+                    if constexpr (!T::Q4) {
+                        if (loads >= (uint32_t)SLOTS) ok = tc_wait_warp(&empty[slot], parity ^ 1, lane);
+                        if (!ok) break;
+                        uint8_t *dst = ring + slot * TILE;
+                        if (lane == 0) {
+                            if (count) skn_mbar_expect_tx(&full[slot], (uint32_t)count << box_shift << 7);
+                            else skn_mbar_arrive(&full[slot]);
+                        }
+                        __syncwarp();
+                        if (page >= 0) {
+                            const int h = lane / boxes;
+                            tma_3d(dst + h * 16384 + (b << box_shift) * 128, map, 0, ((page * st.heads + g.head) << st.page_shift) + row, h, &full[slot]);
+                        }
+                        ++loads;
+                        if (++slot == SLOTS) {
+                            slot = 0;
+                            parity ^= 1;
+                        }
+                    } else {
+                        if (loads >= 4) ok = tc_wait_warp(&raw_empty[slot], parity ^ 1, lane);
+                        if (!ok) break;
+                        uint8_t *dst = raw_ring + slot * T::RAW + ((b << box_shift) >> 4) * T::HALF;
+                        if (lane == 0) {
+                            if (count) skn_mbar_expect_tx(&raw_full[slot], ((uint32_t)count << box_shift) * (D / 2 + D / 16));
+                            else skn_mbar_arrive(&raw_full[slot]);
+                        }
+                        __syncwarp();
+                        if (page >= 0) {
+                            tma_3d(dst, map, row * 4, 0, page * st.heads + g.head, &raw_full[slot]);
+                            tc_tma_load_2d(dst + (D / 2 << box_shift), kv ? &mvs : &mks, row * (D / 64), page * st.heads + g.head, &raw_full[slot]);
+                        }
+                        ++loads;
+                        if (++slot == 4) {
+                            slot = 0;
+                            parity ^= 1;
+                        }
+                    }
+                }
+            }
+        }
+        if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+        // nothing is on its way when the CTA ends: every load is waited for by who reads it, unless a wait ran out
+        if (!ok)
+            for (int i = 0; i < (T::Q4 ? 4 : SLOTS); ++i) {
+                uint64_t *bar = T::Q4 ? &raw_full[i] : &full[i];
+                tc_wait_warp(bar, i < slot ? parity : parity ^ 1, lane);
+            }
+    }
+    // ---- 16-bit types: rows of V that nobody sees are cleared, warp 10 -------------------------------------------------------------
+    else if (!T::Q4 && warp == 10) {
+        int slot = 0, parity = 0;
+        bool ok = true;
+        auto step = [&] {
+            if (++slot == SLOTS) {
+                slot = 0;
+                parity ^= 1;
+            }
+        };
+        while (ok && pp_next(p, w, g)) {
+            const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
+            const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
+            for (int j = 0; j < g.u1 - g.u0 && ok; ++j) {
+                step();                              // K
+                ok = tc_wait_warp(&full[slot], parity, lane);
+                if (!ok) break;
+                if (pp_hides(p, g, j)) {
+                    const int i = g.u0 + j, k0 = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS;
+                    uint8_t *v = ring + slot * TILE;
+                    for (int x = lane; x < PP_KEYS * (D / 8); x += 32) {
+                        const int row = x / (D / 8), c = x % (D / 8), key = k0 + row;
+                        if (!(key <= pmax && (key >= seen_from || key < p.sinks))) *reinterpret_cast<uint4 *>(v + (c >> 3) * 16384 + row * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    skn_fence_proxy_async();
+                    __syncwarp();
+                }
+                if (lane == 0) skn_mbar_arrive(&clean[slot]);      // V lies in every second slot: once a round
+                step();
+            }
+        }
+        if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+    }
+    // ---- Q4_0: quants to fp16, warps 12 .. 15, a key per thread -----------------------------------------------------------------------
+    else if (T::Q4 && warp >= 12) {
+        int slot = 0, parity = 0, raw = 0, raw_parity = 0;
+        uint32_t tiles = 0;
+        bool ok = true;
+        const int row = tid & 127;
+        while (ok && pp_next(p, w, g)) {
+            const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
+            const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
+            for (int j = 0; j < g.u1 - g.u0 && ok; ++j) {
+                const int i = g.u0 + j, key = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS + row;
+                const bool need = key <= pmax && (key >= seen_from || key < p.sinks);
+                for (int kv = 0; kv < 2; ++kv) {
+                    ok = tc_wait_warp(&raw_full[raw], raw_parity, lane);
+                    if (ok && tiles >= (uint32_t)SLOTS) ok = tc_wait_warp(&empty[slot], parity ^ 1, lane);
+                    if (!ok) break;
+                    const int box_shift = min(st.page_shift, 5), in = row & ((1 << box_shift) - 1);
+                    const uint8_t *src = raw_ring + raw * T::RAW + ((row - in) >> 4) * T::HALF;
+                    uint8_t *dst = ring + slot * TILE + row * 128;
+#pragma unroll
+                    for (int b = 0; b < NBLK; ++b) {
+                        uint4 u = need ? *reinterpret_cast<const uint4 *>(src + (((b << box_shift) + in) << 4)) : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+                        const __half d = need ? *reinterpret_cast<const __half *>(src + (D / 2 << box_shift) + (in * NBLK + b) * 2) : __float2half_rn(0.f);
+                        const __half2 d2 = __half2half2(d), off = __float2half2_rn(-1032.f);
+                        const uint32_t ws[4] = {u.x, u.y, u.z, u.w};
+                        uint32_t h[16];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+#pragma unroll
+                            for (int hi = 0; hi < 2; ++hi) {
+                                const uint32_t n = (hi ? ws[x] >> 4 : ws[x]) & 0x0F0F0F0Fu;
+#pragma unroll
+                                for (int y = 0; y < 2; ++y) {
+                                    const uint32_t z = __byte_perm(n, 0x64646464u, y ? 0x4342 : 0x4140);
+                                    const __half2 v = __hmul2(__hadd2(*reinterpret_cast<const __half2 *>(&z), off), d2);
+                                    h[8 * hi + 2 * x + y] = *reinterpret_cast<const uint32_t *>(&v);
+                                }
+                            }
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const int c = 4 * b + x;
+                            *reinterpret_cast<uint4 *>(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(h[4 * x], h[4 * x + 1], h[4 * x + 2], h[4 * x + 3]);
+                        }
+                    }
+                    skn_fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        skn_mbar_arrive(&raw_empty[raw]);
+                        skn_mbar_arrive(&full[slot]);
+                    }
+                    ++tiles;
+                    if (++raw == 4) {
+                        raw = 0;
+                        raw_parity ^= 1;
+                    }
+                    if (++slot == SLOTS) {
+                        slot = 0;
+                        parity ^= 1;
+                    }
+                }
+            }
+        }
+        if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tc_dealloc(tmem, 512);
+}
+
+template <class CT, int D> static cudaError_t prompt_launch(const skn_paged *pc, const PagedAttn &p) {
+    using T = PpTraits<CT, D>;
+    auto *kern = skn_paged_prompt_kernel<CT, D>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM);
+    if (e != cudaSuccess) return e;
+    kern<<<pc->ctx->sm_count, T::THREADS, T::SMEM, pc->ctx->stream>>>(p, pc->wide[0], pc->wide[1], pc->map[2], pc->map[3]);
+    return cudaGetLastError();
+}

@@ -110,6 +110,9 @@ struct PagedSegment {
     int c0, n_parts, slot;                // CTAs that have some of it: c0 .. c0 + n_parts - 1
 };
 
+// Where a CTA leaves its part of a segment that others share: a CTA ends in at most one such segment and begins in at most one
+__device__ __forceinline__ int paged_slot(const PagedSegment &g, int cta) { return 2 * cta + (cta == g.c0); }
+
 // A segment from the definition: for rows in turn, a thread per key and then a thread per dimension (PA_THREADS of them, which `bar` brings together).
 // put(row, maximum (base 2), sum, this thread's dimension of the unnormalised output)
 template <class CT, int D, class IO, class Bar, class Put>
@@ -278,7 +281,6 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
     } else __syncthreads();
 
     int stage = 0, parity = 0;                 // of the warp's next unit
-    const long long u_begin = u;
     int s_at = 0;
     while (u < u_end) {
         // ---- which segment ------------------------------------------------------------------------------------------------
@@ -316,7 +318,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             const long long a = u - g.u0;
             g.c0 = (int)(((a + 1) * n_cta - 1) / total);
             g.n_parts = (int)(((a + g.span.units) * n_cta - 1) / total) - g.c0 + 1;
-            g.slot = 2 * (int)blockIdx.x + (u == u_begin ? 0 : 1);
+            g.slot = paged_slot(g, (int)blockIdx.x);
             u += g.u1 - g.u0;
         }
         const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
@@ -877,10 +879,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             }
             __threadfence();
             __syncthreads();
-            // the first CTA's slot: 0 where the segment is the first of its share
-            const long long a = u - (g.u1 - g.u0) - g.u0;
-            auto slot_of = [&](int c) { return 2 * c + (c == g.c0 && total * c / n_cta < a); };
-            if (tid == 0) ticket = atomicInc(&p.tickets[slot_of(g.c0)], (unsigned)g.n_parts - 1);
+            if (tid == 0) ticket = atomicInc(&p.tickets[paged_slot(g, g.c0)], (unsigned)g.n_parts - 1);
             __syncthreads();
             last = ticket == (unsigned)g.n_parts - 1;
             if (last) {
@@ -889,11 +888,11 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                     const int r = i / (D / 4), d = i % (D / 4) * 4;
                     float top = PA_NONE;
                     for (int k = 0; k < g.n_parts; ++k)
-                        top = fmaxf(top, __ldcg(p.parts + ((int64_t)slot_of(g.c0 + k) * SKN_PAGED_PART_ROWS + r) * (D + 4) + D));
+                        top = fmaxf(top, __ldcg(p.parts + ((int64_t)paged_slot(g, g.c0 + k) * SKN_PAGED_PART_ROWS + r) * (D + 4) + D));
                     float sum = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                     for (int k = 0; k < g.n_parts; ++k) {
-                        const float *from = p.parts + ((int64_t)slot_of(g.c0 + k) * SKN_PAGED_PART_ROWS + r) * (D + 4);
+                        const float *from = p.parts + ((int64_t)paged_slot(g, g.c0 + k) * SKN_PAGED_PART_ROWS + r) * (D + 4);
                         const float f = exp2f(__ldcg(from + D) - top);
                         if (f == 0.f) continue;
                         sum = fmaf(__ldcg(from + D + 1), f, sum);

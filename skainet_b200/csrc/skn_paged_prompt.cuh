@@ -16,6 +16,7 @@
 #include "skn_paged_attn.cuh"
 
 constexpr int PP_ROWS = 256, PP_KEYS = 128;
+constexpr int PP_COST = 3;        // units that a block's start and end are worth on the line
 
 template <class CT, int D> struct PpTraits {
     static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
@@ -28,6 +29,9 @@ template <class CT, int D> struct PpTraits {
     static constexpr size_t SMEM = 1024 + 2 * TILE + (size_t)SLOTS * TILE + (size_t)RAW_SLOTS * RAW;
     static constexpr int SLACK = 4;
     static constexpr float LIFT = BF ? 0.f : 11.f;                // exponent: fp16 weights up to 2^15 (see skn_paged_attn.cuh)
+    // registers a thread of the softmax warpgroups, of the MMA / TMA / clearing warpgroup and of the unpacking one: at most the launch's, 384 x 168 or 512 x 128
+    static constexpr int REGS_SOFT = Q4 ? 176 : 208, REGS_MMA = Q4 ? 64 : 80, REGS_UNPACK = 96;
+    static_assert(128 * (2 * REGS_SOFT + REGS_MMA + (Q4 ? REGS_UNPACK : 0)) <= THREADS * (Q4 ? 128 : 168), "more than the launch has");
 };
 
 __device__ __forceinline__ void pp_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -74,9 +78,37 @@ __device__ __forceinline__ float pp_ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ float pp_max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of two values: on the special-function units, which at 16 a clock and SM would take as long as the products, and with FMAs.
+// The latter: x = n + f with f in -1/2 .. 1/2 (n from the sum with 1.5 2^23), a cubic of least relative error 7.5e-5 there (fp16 weights
+// are off by 2.4e-4, bf16 by more), n added to the exponent; from 2^-126 on.
+__device__ __forceinline__ uint64_t pp_ex2_unit(uint64_t x) {
+    float a, b;
+    skn_unpack2(x, a, b);
+    return skn_pack2(pp_ex2(a), pp_ex2(b));
+}
+__device__ __forceinline__ uint64_t pp_ex2_fma(uint64_t x) {
+    float a, b;
+    skn_unpack2(x, a, b);
+    x = skn_pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const uint64_t big = skn_pack2(12582912.f, 12582912.f), n = skn_add2(x, big);
+    const uint64_t f = skn_fma2(skn_add2(n, skn_pack2(-12582912.f, -12582912.f)), skn_pack2(-1.f, -1.f), x);
+    uint64_t y = skn_fma2(f, skn_pack2(0.05517166905792616f, 0.05517166905792616f), skn_pack2(0.2426111221932161f, 0.2426111221932161f));
+    y = skn_fma2(y, f, skn_pack2(0.6932609854606553f, 0.6932609854606553f));
+    y = skn_fma2(y, f, skn_pack2(0.9999280735394012f, 0.9999280735394012f));
+    float ya, yb, na, nb;
+    skn_unpack2(y, ya, yb);
+    skn_unpack2(n, na, nb);
+    return skn_pack2u(__float_as_uint(ya) + (__float_as_uint(na) << 23), __float_as_uint(yb) + (__float_as_uint(nb) << 23));
+}
+
 // A CTA's share of the line, segment by segment; every role walks it for itself
 struct PpWalk {
-    long long u, u_begin, u_end, total, a;      // a: where the present block and head begin
+    long long u, u_end, total, a;               // a: where the present block and head begin
     int n_cta, seq, rb, head;
     PagedSeq sq;
 };
@@ -86,14 +118,19 @@ __device__ __forceinline__ PagedSpan pp_span(const PagedAttn &p, const PagedSeq 
     return paged_span(p, q.len - q.n + (int)(r0 / p.group), q.len - q.n + (int)(r1 / p.group), PP_KEYS);
 }
 __device__ __forceinline__ bool pp_next(const PagedAttn &p, PpWalk &w, PagedSegment &g) {
-    if (w.u >= w.u_end) return false;
-    for (;;) {                                   // the block that holds u
-        const int nb = w.seq < p.st.n_seqs ? pp_blocks(p, w.sq) : 0;
-        if (w.seq >= p.st.n_seqs) return false;
-        if (w.rb < nb) {
+    for (;;) {                                   // the next block of which this share has units
+        if (w.u >= w.u_end || w.seq >= p.st.n_seqs) return false;
+        if (w.rb < pp_blocks(p, w.sq)) {
             g.span = pp_span(p, w.sq, w.rb);
-            if (w.u < w.a + g.span.units) break;
-            w.a += g.span.units;
+            const int length = g.span.units + PP_COST;
+            if (w.u < w.a + length) {
+                g.u0 = (int)max(0LL, w.u - w.a - PP_COST);
+                g.u1 = (int)min((long long)g.span.units, w.u_end - w.a - PP_COST);
+                w.u = min(w.u_end, w.a + length);
+                if (g.u1 > g.u0) break;
+                continue;
+            }
+            w.a += length;
             if (++w.head == p.st.heads) {
                 w.head = 0;
                 ++w.rb;
@@ -106,12 +143,10 @@ __device__ __forceinline__ bool pp_next(const PagedAttn &p, PpWalk &w, PagedSegm
     g.seq = w.seq; g.head = w.head; g.first = w.sq.first; g.n = w.sq.n; g.len = w.sq.len;
     g.row0 = w.rb * PP_ROWS;
     g.rows = min(PP_ROWS, w.sq.n * p.group - g.row0);
-    g.u0 = (int)(w.u - w.a);
-    g.u1 = (int)min((long long)g.span.units, w.u_end - w.a);
-    g.c0 = (int)(((w.a + 1) * w.n_cta - 1) / w.total);
-    g.n_parts = (int)(((w.a + g.span.units) * w.n_cta - 1) / w.total) - g.c0 + 1;
-    g.slot = 2 * (int)blockIdx.x + (w.u == w.u_begin ? 0 : 1);
-    w.u += g.u1 - g.u0;
+    const long long a = w.a + PP_COST;
+    g.c0 = (int)(((a + 1) * w.n_cta - 1) / w.total);
+    g.n_parts = (int)(((a + g.span.units) * w.n_cta - 1) / w.total) - g.c0 + 1;
+    g.slot = paged_slot(g, (int)blockIdx.x);
     return true;
 }
 
@@ -134,7 +169,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     uint8_t *const base = reinterpret_cast<uint8_t *>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
     uint8_t *const q_tile = base, *const ring = base + 2 * TILE, *const raw_ring = ring + SLOTS * TILE;
     __shared__ uint64_t full[SLOTS], empty[SLOTS], raw_full[4], raw_empty[4];
-    __shared__ uint64_t s_full[2], p_full[2], pv_done[2], q_full[2], o_free[2], clean[SLOTS];
+    __shared__ uint64_t s_full[2], p_full[4], pv_done[2], q_full[2], o_free[2], clean[SLOTS];
     __shared__ long long warp_sum[THREADS / 32];
     __shared__ long long found_at;
     __shared__ int found[2];
@@ -156,7 +191,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         }
         for (int i = 0; i < 2; ++i) {
             skn_mbar_init(&s_full[i], 1);
-            skn_mbar_init(&p_full[i], 4);
+            skn_mbar_init(&p_full[2 * i], 4);
+            skn_mbar_init(&p_full[2 * i + 1], 4);
             skn_mbar_init(&pv_done[i], 1);
             skn_mbar_init(&q_full[i], 4);
             skn_mbar_init(&o_free[i], 4);
@@ -180,7 +216,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     if (++seq < st.n_seqs) sq = paged_seq(st, seq);
                 }
                 const bool have = seq < st.n_seqs;
-                const long long x = have ? (long long)pp_span(p, sq, skip).units * st.heads : 0;
+                const long long x = have ? (long long)(pp_span(p, sq, skip).units + PP_COST) * st.heads : 0;
                 long long inc = x;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -206,10 +242,10 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             if (pass == 0) {
                 w.total = run;
                 if (run == 0) return;
-                const long long want = (run + 3) / 4;            // four units a CTA at least
+                const long long want = (run + PP_COST + 3) / (PP_COST + 4);        // four units a CTA at least
                 w.n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
                 if ((int)blockIdx.x >= w.n_cta) return;
-                share = w.u = w.u_begin = run * blockIdx.x / w.n_cta;
+                share = w.u = run * blockIdx.x / w.n_cta;
                 w.u_end = run * (blockIdx.x + 1) / w.n_cta;
             }
         }
@@ -229,6 +265,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
 
     // ---- softmax: warps 0 .. 3 rows 0 .. 127 of a block, warps 4 .. 7 the others ---------------------------------------------
     if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::REGS_SOFT));
         const int tile = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const uint32_t ts = tmem + tile * 128 + lanes, to = tmem + 256 + tile * D + lanes;
@@ -241,38 +278,40 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             float m = PA_NONE, l = 0.f, cs = 0.f;
             if (used && ok) {
                 // the tile's queries, for fp16 products times a power of two that brings a row's largest to 2^14 .. 2^15
-                const IO *q = static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + R) % p.group) * D;
-                uint8_t *const qt = q_tile + tile * TILE;
-                float f = 1.f, up = p.scale < 0.f ? -1.f : 1.f;
-                if constexpr (!T::BF) {
-                    float top = 0.f;
-                    if (real)
-#pragma unroll 4
-                        for (int c = 0; c < D / 8; ++c) {
-                            float x[8];
-                            io_load8(q + 8 * c, x);
+                const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + R) % p.group) * D);
+                uint8_t *const qt = q_tile + tile * TILE + r * 128;
+                uint4 x[D / 8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-                        }
-                    int e = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
-                    e = top > 0.f && top < INFINITY ? max(-120, min(120, e)) : 0;
-                    up *= __uint_as_float((uint32_t)(127 + e) << 23);
+                for (int c = 0; c < D / 8; ++c) x[c] = real ? q[c] : make_uint4(0, 0, 0, 0);
+                float f = 1.f;
+                if constexpr (T::BF) {
+                    const uint32_t keep = p.scale == 0.f ? 0u : 0xFFFFFFFFu, flip = p.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+                    for (int c = 0; c < D / 8; ++c) x[c] = make_uint4((x[c].x ^ flip) & keep, (x[c].y ^ flip) & keep, (x[c].z ^ flip) & keep, (x[c].w ^ flip) & keep);
+                } else {
+                    uint32_t top = 0;                // largest size, as the bits of a bf16
+#pragma unroll
+                    for (int c = 0; c < D / 8; ++c) {
+                        const uint32_t a = __vmaxu2(x[c].x & 0x7FFF7FFFu, x[c].y & 0x7FFF7FFFu), b = __vmaxu2(x[c].z & 0x7FFF7FFFu, x[c].w & 0x7FFF7FFFu);
+                        top = __vmaxu2(top, __vmaxu2(a, b));
+                    }
+                    top = max(top & 0xFFFFu, top >> 16);
+                    int e = 14 - ((int)(top >> 7) - 127);
+                    e = top > 0 && top < 0x7F80u ? max(-120, min(120, e)) : 0;
+                    const float up = p.scale == 0.f ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale < 0.f ? -1.f : 1.f);
                     f = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+                    for (int c = 0; c < D / 8; ++c) {
+                        uint32_t y[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] = pack_f16(__uint_as_float(y[i] << 16) * up, __uint_as_float(y[i] & 0xFFFF0000u) * up);
+                        x[c] = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
                 }
                 // (a scale of zero moves into the queries: hidden scores of minus infinity stay what they are)
-                if (p.scale == 0.f) up = 0.f;
                 cs = (p.scale == 0.f ? 1.f : fabsf(p.scale)) * f;
-#pragma unroll 4
-                for (int c = 0; c < D / 8; ++c) {
-                    float x[8] = {};
-                    if (real) io_load8(q + 8 * c, x);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] *= up;
-                    uint4 v;
-                    if constexpr (T::BF) v = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-                    else v = make_uint4(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
-                    *reinterpret_cast<uint4 *>(qt + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-                }
+                for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4 *>(qt + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) = x[c];
                 skn_fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) skn_mbar_arrive(&q_full[tile]);
@@ -294,9 +333,15 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         for (int c = 0; c < PP_KEYS; ++c)
                             if (c > hi || (c < lo && c >= sk)) v[c] = -INFINITY;
                     }
-                    float top = fmaxf(v[0], v[1]);
+                    float top = pp_max3(v[0], v[1], v[2]), top2 = pp_max3(v[3], v[4], v[5]);     // (a NaN stays one)
 #pragma unroll
-                    for (int c = 2; c < PP_KEYS; c += 2) top = fmaxf(top, fmaxf(v[c], v[c + 1]));
+                    for (int c = 6; c < 126; c += 4) {
+                        top = pp_max3(top, v[c], v[c + 1]);
+                        top2 = pp_max3(top2, v[c + 2], v[c + 3]);
+                    }
+                    top = pp_max3(top, v[126], v[127]);
+                    top = pp_max3(top, top2, top2);
+                    if (top != top) l = top;
                     top *= cs;
                     if (__any_sync(0xffffffffu, top > m + (float)T::SLACK)) {
                         const float fresh = fmaxf(m, top), fix = pp_ex2(m - fresh);
@@ -317,25 +362,36 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                             tc_wait_st();
                         }
                     }
-                    const float off = T::LIFT - m;
-                    float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    const uint64_t cs2 = skn_pack2(cs, cs), off2 = skn_pack2(T::LIFT - m, T::LIFT - m);
+                    uint64_t sum = 0;
+                    auto half = [&](int h, auto all) {
+                        constexpr bool ALL = decltype(all)::value;
                         uint32_t pk[32];
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            const float a = pp_ex2(fmaf(v[64 * h + 2 * c], cs, off)), b = pp_ex2(fmaf(v[64 * h + 2 * c + 1], cs, off));
-                            sum0 += a;
-                            sum1 += b;
+                            const uint64_t x = skn_fma2(skn_pack2(v[64 * h + 2 * c], v[64 * h + 2 * c + 1]), cs2, off2);
+                            const uint64_t y = ALL || c % 8 < 5 ? pp_ex2_unit(x) : pp_ex2_fma(x);
+                            sum = skn_add2(sum, y);
+                            float a, b;
+                            skn_unpack2(y, a, b);
                             pk[c] = T::BF ? pack_bf16(a, b) : pack_f16(a, b);
                         }
                         pp_st32(ts + 32 * h, pk);
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) skn_mbar_arrive(&p_full[2 * tile + h]);
+                    };
+                    if (whole) {
+                        half(0, std::false_type());
+                        half(1, std::false_type());
+                    } else {                         // hidden weights are exactly zero
+                        half(0, std::true_type());
+                        half(1, std::true_type());
                     }
-                    l += sum0 + sum1;
-                    tc_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) skn_mbar_arrive(&p_full[tile]);
+                    float a, b;
+                    skn_unpack2(sum, a, b);
+                    l += a + b;
                 }
                 if (ok && g.u1 > g.u0) ok = tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane);
                 if (!ok) {
@@ -350,31 +406,41 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             if (used && ok) {
                 tc_fence_after();
                 const float inv = l == 0.f ? 0.f : 1.f / l;
+                uint8_t *const qt = q_tile + tile * TILE + r * 128;          // the tile's queries are done with: rows gather there
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
                     pp_ld32(to + c, o);
                     pp_wait_ld<32>(o);
                     float s = 0.f;
-                    if (shared) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) {
-                            s += (o[k] + o[k + 1]) + (o[k + 2] + o[k + 3]);
+                    for (int k = 0; k < 32; k += 8) {
+                        if (shared) {
                             reinterpret_cast<float4 *>(part)[((c + k) / 4) * PP_ROWS + R] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                        }
-                    } else {
+                            reinterpret_cast<float4 *>(part)[((c + k) / 4 + 1) * PP_ROWS + R] = make_float4(o[k + 4], o[k + 5], o[k + 6], o[k + 7]);
+                        } else {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            float x[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                x[e] = l == 0.f ? 0.f : o[k + e] * inv;
-                                s += x[e];
-                            }
-                            if (real) io_store8(out + c + k, x);
+                            for (int e = 0; e < 8; ++e) o[k + e] = l == 0.f ? 0.f : o[k + e] * inv;
+                            const int cc = (c + k) / 8;
+                            *reinterpret_cast<uint4 *>(qt + (cc >> 3) * 16384 + (((cc & 7) ^ (r & 7)) << 4)) =
+                                make_uint4(pack_bf16(o[k], o[k + 1]), pack_bf16(o[k + 2], o[k + 3]), pack_bf16(o[k + 4], o[k + 5]), pack_bf16(o[k + 6], o[k + 7]));
                         }
+                        s += ((o[k] + o[k + 1]) + (o[k + 2] + o[k + 3])) + ((o[k + 4] + o[k + 5]) + (o[k + 6] + o[k + 7]));
                     }
                     odd |= !(fabsf(s) < INFINITY);
+                }
+                if (!shared) {                       // and leave it whole
+                    __syncwarp();
+                    const uint64_t mine = real ? reinterpret_cast<uint64_t>(out) : 0;
+                    const uint8_t *from = q_tile + tile * TILE + (r & ~31) * 128;
+#pragma unroll 4
+                    for (int it = 0; it < D / 8; ++it) {
+                        const int row = it * 32 / (D / 8) + lane / (D / 8), cc = lane % (D / 8);
+                        const uint64_t at = __shfl_sync(0xffffffffu, mine, row);
+                        const uint4 y = *reinterpret_cast<const uint4 *>(from + row * 128 + (cc >> 3) * 16384 + (((cc & 7) ^ (row & 7)) << 4));
+                        if (at) *reinterpret_cast<uint4 *>(at + 16 * cc) = y;
+                    }
+                    __syncwarp();
                 }
                 odd = real && (odd || !(fabsf(l) < INFINITY));
                 if (shared) {
@@ -401,23 +467,21 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             if (shared) {
                 __threadfence();
                 pp_bar();
-                const long long a = w.u - g.u1;                    // where the block begins
-                auto slot_of = [&](int c) { return 2 * c + (c == g.c0 && w.total * c / w.n_cta < a); };
-                if (tid == 0) ticket = atomicInc(&p.tickets[slot_of(g.c0)], (unsigned)g.n_parts - 1);
+                if (tid == 0) ticket = atomicInc(&p.tickets[paged_slot(g, g.c0)], (unsigned)g.n_parts - 1);
                 pp_bar();
                 if (ticket == (unsigned)g.n_parts - 1 && real) {
                     __threadfence();
                     float top = PA_NONE, sum = 0.f;
-                    for (int k = 0; k < g.n_parts; ++k) top = fmaxf(top, __ldcg(p.parts + (int64_t)slot_of(g.c0 + k) * PP_ROWS * (D + 4) + D * PP_ROWS + R));
+                    for (int k = 0; k < g.n_parts; ++k) top = fmaxf(top, __ldcg(p.parts + (int64_t)paged_slot(g, g.c0 + k) * PP_ROWS * (D + 4) + D * PP_ROWS + R));
                     for (int k = 0; k < g.n_parts; ++k) {
-                        const float *from = p.parts + (int64_t)slot_of(g.c0 + k) * PP_ROWS * (D + 4);
+                        const float *from = p.parts + (int64_t)paged_slot(g, g.c0 + k) * PP_ROWS * (D + 4);
                         sum = fmaf(__ldcg(from + (D + 1) * PP_ROWS + R), exp2f(__ldcg(from + D * PP_ROWS + R) - top), sum);
                     }
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         float4 o[8] = {};
                         for (int k = 0; k < g.n_parts; ++k) {
-                            const float *from = p.parts + (int64_t)slot_of(g.c0 + k) * PP_ROWS * (D + 4);
+                            const float *from = p.parts + (int64_t)paged_slot(g, g.c0 + k) * PP_ROWS * (D + 4);
                             const float f = exp2f(__ldcg(from + D * PP_ROWS + R) - top);
                             if (f == 0.f) continue;
 #pragma unroll
@@ -439,7 +503,9 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         }
     }
     // ---- MMAs: warp 8 --------------------------------------------------------------------------------------------------------
-    else if (warp == 8) {
+    else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::REGS_MMA));
+    if (warp == 8) {
         constexpr uint32_t FMT = T::BF ? 1u << 7 | 1u << 10 : 0u;
         constexpr uint32_t ID_S = 1u << 4 | FMT | (PP_KEYS >> 3) << 17 | 8u << 24, ID_O = 1u << 4 | FMT | 1u << 16 | (D >> 3) << 17 | 8u << 24;
         int slot = 0, parity = 0;                    // of the next K or V
@@ -482,19 +548,24 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 k_slot = slot;
                 const uint32_t va = skn_smem_u32(ring + v_slot * TILE);
                 for (int x = 0; x < tiles && ok; ++x) {
-                    ok = tc_wait_warp(&p_full[x], units[x] & 1, lane);
-                    if (ok && j == 0 && segs[x] > 0) ok = tc_wait_warp(&o_free[x], (segs[x] - 1) & 1, lane);
+                    for (int h = 0; h < 2 && ok; ++h) {          // the weights come in halves
+                        ok = tc_wait_warp(&p_full[2 * x + h], units[x] & 1, lane);
+                        if (ok && j == 0 && h == 0 && segs[x] > 0) ok = tc_wait_warp(&o_free[x], (segs[x] - 1) & 1, lane);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (tc_elect()) {
+#pragma unroll
+                            for (int k = 4 * h; k < 4 * h + 4; ++k)
+                                tc_mma_ts(tmem + 256 + x * D, tmem + x * 128 + 8 * k, pp_desc_n(va + k * 2048, PP_KEYS * 128), ID_O, j > 0 || k > 0);
+                            if (h) {
+                                tc_commit(&pv_done[x]);
+                                if (x == tiles - 1) tc_commit(&empty[v_slot]);
+                            }
+                        }
+                        __syncwarp();
+                    }
                     if (!ok) break;
                     ++units[x];
-                    tc_fence_after();
-                    if (tc_elect()) {
-#pragma unroll
-                        for (int k = 0; k < PP_KEYS / 16; ++k)
-                            tc_mma_ts(tmem + 256 + x * D, tmem + x * 128 + 8 * k, pp_desc_n(va + k * 2048, PP_KEYS * 128), ID_O, j > 0 || k > 0);
-                        tc_commit(&pv_done[x]);
-                        if (x == tiles - 1) tc_commit(&empty[v_slot]);
-                    }
-                    __syncwarp();
                     if (more) {
                         if (x == 0) ok = tc_wait_warp(&full[k_slot], parity, lane);
                         if (!ok) break;
@@ -617,8 +688,10 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         }
         if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
     }
+    }
     // ---- Q4_0: quants to fp16, warps 12 .. 15, a key per thread -----------------------------------------------------------------------
-    else if (T::Q4 && warp >= 12) {
+    else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::REGS_UNPACK));
         int slot = 0, parity = 0, raw = 0, raw_parity = 0;
         uint32_t tiles = 0;
         bool ok = true;

@@ -15,7 +15,7 @@
 #pragma once
 #include "skn_paged_attn.cuh"
 
-constexpr int PP_ROWS = 256, PP_KEYS = 128;
+constexpr int PP_ROWS = 256, PP_KEYS = 128, PP_SUB = 64;
 constexpr int PP_COST = 3;        // units that a block's start and end are worth on the line
 
 template <class CT, int D> struct PpTraits {
@@ -169,7 +169,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     uint8_t *const base = reinterpret_cast<uint8_t *>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
     uint8_t *const q_tile = base, *const ring = base + 2 * TILE, *const raw_ring = ring + SLOTS * TILE;
     __shared__ uint64_t full[SLOTS], empty[SLOTS], raw_full[4], raw_empty[4];
-    __shared__ uint64_t s_full[2], p_full[4], pv_done[2], q_full[2], o_free[2], clean[SLOTS];
+    __shared__ uint64_t s_full[4], p_full[4], pv_done[2], q_full[2], o_free[2], clean[SLOTS];
     __shared__ long long warp_sum[THREADS / 32];
     __shared__ long long found_at;
     __shared__ int found[2];
@@ -190,9 +190,10 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             skn_mbar_init(&raw_empty[i], 4);
         }
         for (int i = 0; i < 2; ++i) {
-            skn_mbar_init(&s_full[i], 1);
-            skn_mbar_init(&p_full[2 * i], 4);
-            skn_mbar_init(&p_full[2 * i + 1], 4);
+            for (int b = 0; b < 2; ++b) {
+                skn_mbar_init(&s_full[2 * i + b], 1);
+                skn_mbar_init(&p_full[2 * i + b], 4);
+            }
             skn_mbar_init(&pv_done[i], 1);
             skn_mbar_init(&q_full[i], 4);
             skn_mbar_init(&o_free[i], 4);
@@ -269,7 +270,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         const int tile = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const uint32_t ts = tmem + tile * 128 + lanes, to = tmem + 256 + tile * D + lanes;
-        uint32_t n_units = 0;                        // of this tile so far
+        uint32_t n_subs = 0;                         // of this tile so far
         bool ok = true;                              // once a wait has run out the share is only walked: the barriers below want every warp
         while (pp_next(p, w, g)) {
             const int R = tile * 128 + r;
@@ -318,28 +319,30 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 const int ta = (g.row0 + tile * 128) / p.group, tb = (g.row0 + min(tile * 128 + 127, g.rows - 1)) / p.group;
                 const int pmin = g.len - g.n + ta, pmax = g.len - g.n + tb;
 
-                for (int j = 0; j < g.u1 - g.u0; ++j, ++n_units) {
-                    const int i = g.u0 + j, k0 = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS;
-                    if (!tc_wait_warp(&s_full[tile], n_units & 1, lane)) { ok = false; break; }
+                // 64 keys at a time, in two places that take turns: the scores of the next are there before these are done with
+                for (int k = 0; k < 2 * (g.u1 - g.u0); ++k, ++n_subs) {
+                    const int i = g.u0 + (k >> 1), k0 = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS + (k & 1) * PP_SUB;
+                    const uint32_t at = ts + (k & 1) * PP_SUB;
+                    if (!tc_wait_warp(&s_full[2 * tile + (k & 1)], (n_subs >> 1) & 1, lane)) { ok = false; break; }
                     tc_fence_after();
-                    float v[PP_KEYS];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) pp_ld32(ts + 32 * c, v + 32 * c);
-                    pp_wait_ld<PP_KEYS>(v);
-                    const bool whole = k0 + PP_KEYS - 1 <= pmin && (!p.window || k0 > pmax - p.window || k0 + PP_KEYS <= p.sinks);
+                    float v[PP_SUB];
+                    pp_ld32(at, v);
+                    pp_ld32(at + 32, v + 32);
+                    pp_wait_ld<PP_SUB>(v);
+                    const bool whole = k0 + PP_SUB - 1 <= pmin && (!p.window || k0 > pmax - p.window || k0 + PP_SUB <= p.sinks);
                     if (!whole) {
                         const int hi = pos - k0, lo = p.window ? pos - p.window + 1 - k0 : -1, sk = p.sinks - k0;
 #pragma unroll
-                        for (int c = 0; c < PP_KEYS; ++c)
+                        for (int c = 0; c < PP_SUB; ++c)
                             if (c > hi || (c < lo && c >= sk)) v[c] = -INFINITY;
                     }
                     float top = pp_max3(v[0], v[1], v[2]), top2 = pp_max3(v[3], v[4], v[5]);     // (a NaN stays one)
 #pragma unroll
-                    for (int c = 6; c < 126; c += 4) {
+                    for (int c = 6; c < 62; c += 4) {
                         top = pp_max3(top, v[c], v[c + 1]);
                         top2 = pp_max3(top2, v[c + 2], v[c + 3]);
                     }
-                    top = pp_max3(top, v[126], v[127]);
+                    top = pp_max3(top, v[62], v[63]);
                     top = pp_max3(top, top2, top2);
                     if (top != top) l = top;
                     top *= cs;
@@ -347,8 +350,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         const float fresh = fmaxf(m, top), fix = pp_ex2(m - fresh);
                         m = fresh;
                         l *= fix;
-                        if (j > 0) {
-                            if (!tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane)) { ok = false; break; }
+                        if (k > 0) {
+                            if (!tc_wait_warp(&pv_done[tile], (n_subs - 1) & 1, lane)) { ok = false; break; }
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < D; c += 32) {
@@ -356,7 +359,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                                 pp_ld32(to + c, o);
                                 pp_wait_ld<32>(o);
 #pragma unroll
-                                for (int k = 0; k < 32; ++k) o[k] *= fix;
+                                for (int e = 0; e < 32; ++e) o[e] *= fix;
                                 pp_st32(to + c, reinterpret_cast<uint32_t *>(o));
                             }
                             tc_wait_st();
@@ -364,36 +367,32 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     }
                     const uint64_t cs2 = skn_pack2(cs, cs), off2 = skn_pack2(T::LIFT - m, T::LIFT - m);
                     uint64_t sum = 0;
-                    auto half = [&](int h, auto all) {
+                    auto weigh = [&](auto all) {
                         constexpr bool ALL = decltype(all)::value;
                         uint32_t pk[32];
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            const uint64_t x = skn_fma2(skn_pack2(v[64 * h + 2 * c], v[64 * h + 2 * c + 1]), cs2, off2);
+                            const uint64_t x = skn_fma2(skn_pack2(v[2 * c], v[2 * c + 1]), cs2, off2);
                             const uint64_t y = ALL || c % 8 < 5 ? pp_ex2_unit(x) : pp_ex2_fma(x);
                             sum = skn_add2(sum, y);
                             float a, b;
                             skn_unpack2(y, a, b);
                             pk[c] = T::BF ? pack_bf16(a, b) : pack_f16(a, b);
                         }
-                        pp_st32(ts + 32 * h, pk);
-                        tc_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) skn_mbar_arrive(&p_full[2 * tile + h]);
+                        pp_st32(at, pk);
                     };
-                    if (whole) {
-                        half(0, std::false_type());
-                        half(1, std::false_type());
-                    } else {                         // hidden weights are exactly zero
-                        half(0, std::true_type());
-                        half(1, std::true_type());
-                    }
+                    if (whole) weigh(std::false_type());
+                    else weigh(std::true_type());    // hidden weights are exactly zero
                     float a, b;
                     skn_unpack2(sum, a, b);
                     l += a + b;
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) skn_mbar_arrive(&p_full[2 * tile + (k & 1)]);
                 }
-                if (ok && g.u1 > g.u0) ok = tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane);
+                // (one after the other: the last scores say that the product before the last two is done, and a parity tells a phase from the one before it only)
+                if (ok) ok = tc_wait_warp(&pv_done[tile], n_subs & 1, lane) && tc_wait_warp(&pv_done[tile], (n_subs - 1) & 1, lane);
                 if (!ok) {
                     if (lane == 0) *st.status = SKN_ERR_TIMEOUT;
                 }
@@ -451,8 +450,9 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 __syncwarp();
                 if (lane == 0) skn_mbar_arrive(&o_free[tile]);
             }
-            if (pp_any(odd))
-                paged_redo<CT, D, IO>(p, g, PP_KEYS, scratch, [] { pp_bar(); }, [&](int row, float rm, float rl, float acc) {
+            if (pp_any(odd)) {
+                const PagedSegment mine = g;         // (a copy: the address of the one that the loops use is not taken)
+                paged_redo<CT, D, IO>(p, mine, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
                     const int tr = (g.row0 + row) / p.group;
                     if (shared) {
                         if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;
@@ -464,6 +464,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         static_cast<IO *>(p.out)[(int64_t)(g.first + tr) * p.out_stride + (g.head * p.group + (g.row0 + row) % p.group) * D + tid] =
                             __float2bfloat16_rn(rl == 0.f ? 0.f : acc / rl);
                 });
+            }
             if (shared) {
                 __threadfence();
                 pp_bar();
@@ -507,9 +508,9 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::REGS_MMA));
     if (warp == 8) {
         constexpr uint32_t FMT = T::BF ? 1u << 7 | 1u << 10 : 0u;
-        constexpr uint32_t ID_S = 1u << 4 | FMT | (PP_KEYS >> 3) << 17 | 8u << 24, ID_O = 1u << 4 | FMT | 1u << 16 | (D >> 3) << 17 | 8u << 24;
+        constexpr uint32_t ID_S = 1u << 4 | FMT | (PP_SUB >> 3) << 17 | 8u << 24, ID_O = 1u << 4 | FMT | 1u << 16 | (D >> 3) << 17 | 8u << 24;
         int slot = 0, parity = 0;                    // of the next K or V
-        uint32_t units[2] = {0, 0}, segs[2] = {0, 0};
+        uint32_t segs[2] = {0, 0}, done[2] = {0, 0};        // done: pieces of a tile before this segment
         bool ok = true;
         auto step = [&] {
             if (++slot == SLOTS) {
@@ -517,69 +518,67 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 parity ^= 1;
             }
         };
-        auto scores = [&](int tile, int at) {        // S of a tile from the keys in slot `at`
-            const uint32_t qa = skn_smem_u32(q_tile + tile * TILE), ka = skn_smem_u32(ring + at * TILE);
+        // S of a tile against half b of the keys in slot `at`
+        auto scores = [&](int tile, int b, int at) {
+            const uint32_t qa = skn_smem_u32(q_tile + tile * TILE), ka = skn_smem_u32(ring + at * TILE) + b * PP_SUB * 128;
             if (tc_elect()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-                    tc_mma_bf16(tmem + tile * 128, tc_smem_desc(qa + off), tc_smem_desc(ka + off), ID_S, k > 0);
+                    tc_mma_bf16(tmem + tile * 128 + b * PP_SUB, tc_smem_desc(qa + off), tc_smem_desc(ka + off), ID_S, k > 0);
                 }
-                tc_commit(&s_full[tile]);
+                tc_commit(&s_full[2 * tile + b]);
             }
             __syncwarp();
         };
         while (ok && pp_next(p, w, g)) {
             const int n = g.u1 - g.u0, tiles = g.rows > 128 ? 2 : 1;
-            int k_slot = slot;
             for (int x = 0; x < tiles && ok; ++x) ok = tc_wait_warp(&q_full[x], segs[x] & 1, lane);
             ok = ok && tc_wait_warp(&full[slot], parity, lane);
             if (!ok) break;
             tc_fence_after();
-            for (int x = 0; x < tiles; ++x) scores(x, slot);
-            if (tc_elect()) tc_commit(&empty[k_slot]);
+            for (int b = 0; b < 2; ++b)
+                for (int x = 0; x < tiles; ++x) scores(x, b, slot);
+            if (tc_elect()) tc_commit(&empty[slot]);
             __syncwarp();
             step();
             for (int j = 0; j < n && ok; ++j) {
                 const int v_slot = slot;
                 ok = tc_wait_warp(T::Q4 ? &full[slot] : &clean[slot], parity, lane);
                 step();
-                const bool more = j + 1 < n;
-                k_slot = slot;
+                const bool more = j + 1 < n;         // the keys of the next unit lie in `slot`
                 const uint32_t va = skn_smem_u32(ring + v_slot * TILE);
-                for (int x = 0; x < tiles && ok; ++x) {
-                    for (int h = 0; h < 2 && ok; ++h) {          // the weights come in halves
-                        ok = tc_wait_warp(&p_full[2 * x + h], units[x] & 1, lane);
-                        if (ok && j == 0 && h == 0 && segs[x] > 0) ok = tc_wait_warp(&o_free[x], (segs[x] - 1) & 1, lane);
+                for (int b = 0; b < 2 && ok; ++b)
+                    for (int x = 0; x < tiles && ok; ++x) {
+                        ok = tc_wait_warp(&p_full[2 * x + b], ((done[x] >> 1) + j) & 1, lane);
+                        if (ok && j == 0 && b == 0 && segs[x] > 0) ok = tc_wait_warp(&o_free[x], (segs[x] - 1) & 1, lane);
                         if (!ok) break;
                         tc_fence_after();
                         if (tc_elect()) {
 #pragma unroll
-                            for (int k = 4 * h; k < 4 * h + 4; ++k)
-                                tc_mma_ts(tmem + 256 + x * D, tmem + x * 128 + 8 * k, pp_desc_n(va + k * 2048, PP_KEYS * 128), ID_O, j > 0 || k > 0);
-                            if (h) {
-                                tc_commit(&pv_done[x]);
-                                if (x == tiles - 1) tc_commit(&empty[v_slot]);
-                            }
+                            for (int k = 0; k < 4; ++k)
+                                tc_mma_ts(tmem + 256 + x * D, tmem + x * 128 + b * PP_SUB + 8 * k, pp_desc_n(va + (4 * b + k) * 2048, PP_KEYS * 128), ID_O, j > 0 || b > 0 || k > 0);
+                            tc_commit(&pv_done[x]);
+                            if (b && x == tiles - 1) tc_commit(&empty[v_slot]);
                         }
                         __syncwarp();
-                    }
-                    if (!ok) break;
-                    ++units[x];
-                    if (more) {
-                        if (x == 0) ok = tc_wait_warp(&full[k_slot], parity, lane);
-                        if (!ok) break;
-                        tc_fence_after();
-                        scores(x, k_slot);
-                        if (x == tiles - 1) {
-                            if (tc_elect()) tc_commit(&empty[k_slot]);
-                            __syncwarp();
+                        if (more) {
+                            if (x == 0 && b == 0) ok = tc_wait_warp(&full[slot], parity, lane);
+                            if (!ok) break;
+                            tc_fence_after();
+                            scores(x, b, slot);
+                            if (b && x == tiles - 1) {
+                                if (tc_elect()) tc_commit(&empty[slot]);
+                                __syncwarp();
+                            }
                         }
                     }
-                }
                 if (more) step();
             }
-            for (int x = 0; x < tiles; ++x) ++segs[x];
+            for (int x = 0; x < tiles; ++x) {
+                ++segs[x];
+                done[x] += 2 * n;
+            }
         }
         if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
     }

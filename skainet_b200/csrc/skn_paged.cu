@@ -209,6 +209,7 @@ static int32_t check_batch(skn_ctx *ctx, const skn_paged_batch *b, bool *nothing
     if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_new < 0 || b->max_pages < 0) return skn_fail(ctx, SKN_ERR_ARG, "negative count in the batch");
     *nothing = b->n_seqs == 0 || b->n_tokens == 0 || (b->max_new == 0 && !host);
     if (*nothing) return SKN_OK;
+    if (b->n_tokens > (1 << 24)) return skn_fail(ctx, SKN_ERR_SHAPE, "%d rows in a step; 2^24 at most", b->n_tokens);
     if (b->n_seqs > 65535) return skn_fail(ctx, SKN_ERR_SHAPE, "%d sequences in a step; 65535 at most", b->n_seqs);
     if (!b->token_start || !b->lengths || (!b->page_table && b->max_pages)) return skn_fail(ctx, SKN_ERR_ARG, "NULL array in the batch");
     return SKN_OK;

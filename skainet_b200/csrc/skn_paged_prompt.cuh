@@ -15,8 +15,8 @@
 #pragma once
 #include "skn_paged_attn.cuh"
 
-constexpr int PP_ROWS = 256, PP_KEYS = 128, PP_SUB = 64;
-constexpr int PP_COST = 3;        // units that a block's start and end are worth on the line
+constexpr int PP_ROWS = 256, PP_KEYS = 128;
+constexpr int PP_COST = 4;        // units that a block's start and end are worth on the line
 
 template <class CT, int D> struct PpTraits {
     static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
@@ -72,6 +72,18 @@ __device__ __forceinline__ void pp_st32(uint32_t taddr, const uint32_t *u) {
           "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ uint32_t pp_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }      // bits 0 .. n - 1
+// 32 bytes of a row, in one store where rows begin at multiples of 32
+__device__ __forceinline__ void pp_store32(__nv_bfloat16 *to, const uint32_t *y, bool wide) {
+    if (wide)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     ::"l"(to), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+                     : "memory");
+    else {
+        reinterpret_cast<uint4 *>(to)[0] = make_uint4(y[0], y[1], y[2], y[3]);
+        reinterpret_cast<uint4 *>(to)[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+}
 __device__ __forceinline__ float pp_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -85,7 +97,7 @@ __device__ __forceinline__ float pp_max3(float a, float b, float c) {
 }
 // 2^x of two values: on the special-function units, which at 16 a clock and SM would take as long as the products, and with FMAs.
 // The latter: x = n + f with f in -1/2 .. 1/2 (n from the sum with 1.5 2^23), a cubic of least relative error 7.5e-5 there (fp16 weights
-// are off by 2.4e-4, bf16 by more), n added to the exponent; from 2^-126 on.
+// are off by 2.4e-4, bf16 by more), n added to the exponent.  What lies below -126, hidden scores among it, ends at one value, which is taken off: zero.
 __device__ __forceinline__ uint64_t pp_ex2_unit(uint64_t x) {
     float a, b;
     skn_unpack2(x, a, b);
@@ -103,7 +115,8 @@ __device__ __forceinline__ uint64_t pp_ex2_fma(uint64_t x) {
     float ya, yb, na, nb;
     skn_unpack2(y, ya, yb);
     skn_unpack2(n, na, nb);
-    return skn_pack2u(__float_as_uint(ya) + (__float_as_uint(na) << 23), __float_as_uint(yb) + (__float_as_uint(nb) << 23));
+    const float least = __uint_as_float(__float_as_uint(0.9999280735394012f) - (126u << 23));        // of x = -126: n = -126, f = 0
+    return skn_add2(skn_pack2u(__float_as_uint(ya) + (__float_as_uint(na) << 23), __float_as_uint(yb) + (__float_as_uint(nb) << 23)), skn_pack2(-least, -least));
 }
 
 // A CTA's share of the line, segment by segment; every role walks it for itself
@@ -112,10 +125,10 @@ struct PpWalk {
     int n_cta, seq, rb, head;
     PagedSeq sq;
 };
-__device__ __forceinline__ int pp_blocks(const PagedAttn &p, const PagedSeq &q) { return (int)(((long long)q.n * p.group + PP_ROWS - 1) / PP_ROWS); }
+__device__ __forceinline__ int pp_blocks(const PagedAttn &p, const PagedSeq &q) { return (q.n * p.group + PP_ROWS - 1) / PP_ROWS; }     // (fewer than 2^30 rows)
 __device__ __forceinline__ PagedSpan pp_span(const PagedAttn &p, const PagedSeq &q, int rb) {
-    const long long r0 = (long long)rb * PP_ROWS, r1 = min(r0 + PP_ROWS, (long long)q.n * p.group) - 1;
-    return paged_span(p, q.len - q.n + (int)(r0 / p.group), q.len - q.n + (int)(r1 / p.group), PP_KEYS);
+    const int r0 = rb * PP_ROWS, r1 = min(r0 + PP_ROWS, q.n * p.group) - 1;
+    return paged_span(p, q.len - q.n + r0 / p.group, q.len - q.n + r1 / p.group, PP_KEYS);
 }
 __device__ __forceinline__ bool pp_next(const PagedAttn &p, PpWalk &w, PagedSegment &g) {
     for (;;) {                                   // the next block of which this share has units
@@ -143,6 +156,11 @@ __device__ __forceinline__ bool pp_next(const PagedAttn &p, PpWalk &w, PagedSegm
     g.seq = w.seq; g.head = w.head; g.first = w.sq.first; g.n = w.sq.n; g.len = w.sq.len;
     g.row0 = w.rb * PP_ROWS;
     g.rows = min(PP_ROWS, w.sq.n * p.group - g.row0);
+    if (g.u0 == 0 && g.u1 == g.span.units) {     // (the divisions are not free)
+        g.c0 = (int)blockIdx.x;
+        g.n_parts = 1;
+        return true;
+    }
     const long long a = w.a + PP_COST;
     g.c0 = (int)(((a + 1) * w.n_cta - 1) / w.total);
     g.n_parts = (int)(((a + g.span.units) * w.n_cta - 1) / w.total) - g.c0 + 1;
@@ -169,7 +187,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     uint8_t *const base = reinterpret_cast<uint8_t *>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
     uint8_t *const q_tile = base, *const ring = base + 2 * TILE, *const raw_ring = ring + SLOTS * TILE;
     __shared__ uint64_t full[SLOTS], empty[SLOTS], raw_full[4], raw_empty[4];
-    __shared__ uint64_t s_full[4], p_full[4], pv_done[2], q_full[2], o_free[2], clean[SLOTS];
+    __shared__ uint64_t s_full[2], p_full[4], pv_done[2], q_full[2], o_free[2], clean[SLOTS];
     __shared__ long long warp_sum[THREADS / 32];
     __shared__ long long found_at;
     __shared__ int found[2];
@@ -190,10 +208,9 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             skn_mbar_init(&raw_empty[i], 4);
         }
         for (int i = 0; i < 2; ++i) {
-            for (int b = 0; b < 2; ++b) {
-                skn_mbar_init(&s_full[2 * i + b], 1);
-                skn_mbar_init(&p_full[2 * i + b], 4);
-            }
+            skn_mbar_init(&s_full[i], 1);
+            skn_mbar_init(&p_full[2 * i], 4);
+            skn_mbar_init(&p_full[2 * i + 1], 4);
             skn_mbar_init(&pv_done[i], 1);
             skn_mbar_init(&q_full[i], 4);
             skn_mbar_init(&o_free[i], 4);
@@ -205,49 +222,57 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     // ---- the line: items are the blocks of all sequences, each of them units x heads long ----------------------------------
     PpWalk w;
     {
-        // total first, then the block in which this CTA's share begins
-        long long share = -1;
+        // total first, then the block in which this CTA's share begins (which is known at once where there are no more blocks than threads)
+        long long share = -1, at = 0, x = 0;
+        int seq = 0, skip = tid, rounds = 0;         // this thread's item: block `skip` counted from sequence `seq`
         for (int pass = 0; pass < 2; ++pass) {
-            long long run = 0;
-            int seq = 0, skip = tid;                 // this thread's item: block `skip` counted from sequence `seq`
-            PagedSeq sq = paged_seq(st, 0);
-            for (;;) {
-                while (seq < st.n_seqs && skip >= pp_blocks(p, sq)) {
-                    skip -= pp_blocks(p, sq);
-                    if (++seq < st.n_seqs) sq = paged_seq(st, seq);
-                }
-                const bool have = seq < st.n_seqs;
-                const long long x = have ? (long long)(pp_span(p, sq, skip).units + PP_COST) * st.heads : 0;
-                long long inc = x;
+            if (pass == 0 || rounds > 1) {
+                long long run = 0;
+                PagedSeq sq = paged_seq(st, 0);
+                seq = 0;
+                skip = tid;
+                for (bool more = true; more;) {
+                    while (seq < st.n_seqs && skip >= pp_blocks(p, sq)) {
+                        skip -= pp_blocks(p, sq);
+                        if (++seq < st.n_seqs) sq = paged_seq(st, seq);
+                    }
+                    const bool have = seq < st.n_seqs;
+                    x = have ? (long long)(pp_span(p, sq, skip).units + PP_COST) * st.heads : 0;
+                    long long inc = x;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-                    if (lane >= o) inc += y;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+                        if (lane >= o) inc += y;
+                    }
+                    if (lane == 31) warp_sum[warp] = inc;
+                    more = __syncthreads_or(have && tid == THREADS - 1);       // the last thread has an item: there may be others
+                    at = run + inc - x;
+                    for (int i = 0; i < THREADS / 32; ++i) {
+                        if (i < warp) at += warp_sum[i];
+                        run += warp_sum[i];
+                    }
+                    if (pass && at <= share && share < at + x) {
+                        found[0] = seq;
+                        found[1] = skip;
+                        found_at = at;
+                    }
+                    if (pass == 0) ++rounds;
+                    if (more) skip += THREADS;
+                    __syncthreads();
                 }
-                __syncthreads();
-                if (lane == 31) warp_sum[warp] = inc;
-                __syncthreads();
-                long long at = run + inc - x;
-                for (int i = 0; i < THREADS / 32; ++i) {
-                    if (i < warp) at += warp_sum[i];
-                    run += warp_sum[i];
+                if (pass == 0) {
+                    w.total = run;
+                    if (run == 0) return;
+                    const long long want = (run + PP_COST) / (PP_COST + 1);        // a CTA for each block of a unit
+                    w.n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
+                    if ((int)blockIdx.x >= w.n_cta) return;
+                    share = w.u = run * blockIdx.x / w.n_cta;
+                    w.u_end = run * (blockIdx.x + 1) / w.n_cta;
                 }
-                if (pass && have && at <= share && share < at + x) {
-                    found[0] = seq;
-                    found[1] = skip;
-                    found_at = at;
-                }
-                skip += THREADS;
-                if (!__syncthreads_or(have)) break;
-            }
-            if (pass == 0) {
-                w.total = run;
-                if (run == 0) return;
-                const long long want = (run + PP_COST + 3) / (PP_COST + 4);        // four units a CTA at least
-                w.n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
-                if ((int)blockIdx.x >= w.n_cta) return;
-                share = w.u = run * blockIdx.x / w.n_cta;
-                w.u_end = run * (blockIdx.x + 1) / w.n_cta;
+            } else if (at <= share && share < at + x) {
+                found[0] = seq;
+                found[1] = skip;
+                found_at = at;
             }
         }
         __syncthreads();
@@ -262,7 +287,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    PagedSegment g;
+    PagedSegment g = {};
 
     // ---- softmax: warps 0 .. 3 rows 0 .. 127 of a block, warps 4 .. 7 the others ---------------------------------------------
     if (warp < 8) {
@@ -270,79 +295,91 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         const int tile = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         const uint32_t ts = tmem + tile * 128 + lanes, to = tmem + 256 + tile * D + lanes;
-        uint32_t n_subs = 0;                         // of this tile so far
+        uint32_t n_units = 0;                        // of this tile so far
+        const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(2 * p.out_stride)) & 31) == 0;
         bool ok = true;                              // once a wait has run out the share is only walked: the barriers below want every warp
-        while (pp_next(p, w, g)) {
-            const int R = tile * 128 + r;
-            const bool real = R < g.rows, used = tile * 128 < g.rows;
-            const int t = (g.row0 + R) / p.group, pos = real ? g.len - g.n + t : -1;
-            float m = PA_NONE, l = 0.f, cs = 0.f;
-            if (used && ok) {
-                // the tile's queries, for fp16 products times a power of two that brings a row's largest to 2^14 .. 2^15
-                const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + R) % p.group) * D);
-                uint8_t *const qt = q_tile + tile * TILE + r * 128;
-                uint4 x[D / 8];
+        // A segment's queries, this thread's row: for fp16 products times a power of two that brings the row's largest to 2^14 .. 2^15; returns the
+        // factor of its scores
+        auto load_queries = [&] {
+            const int R = tile * 128 + r, t = (g.row0 + R) / p.group;
+            const bool real = R < g.rows;
+            const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + R) % p.group) * D);
+            uint8_t *const qt = q_tile + tile * TILE + r * 128;
+            uint4 x[D / 8];
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) x[c] = real ? q[c] : make_uint4(0, 0, 0, 0);
-                float f = 1.f;
-                if constexpr (T::BF) {
-                    const uint32_t keep = p.scale == 0.f ? 0u : 0xFFFFFFFFu, flip = p.scale < 0.f ? 0x80008000u : 0u;
+            for (int c = 0; c < D / 8; ++c) x[c] = real ? q[c] : make_uint4(0, 0, 0, 0);
+            float f = 1.f;
+            if constexpr (T::BF) {
+                const uint32_t keep = p.scale == 0.f ? 0u : 0xFFFFFFFFu, flip = p.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c) x[c] = make_uint4((x[c].x ^ flip) & keep, (x[c].y ^ flip) & keep, (x[c].z ^ flip) & keep, (x[c].w ^ flip) & keep);
-                } else {
-                    uint32_t top = 0;                // largest size, as the bits of a bf16
+                for (int c = 0; c < D / 8; ++c) x[c] = make_uint4((x[c].x ^ flip) & keep, (x[c].y ^ flip) & keep, (x[c].z ^ flip) & keep, (x[c].w ^ flip) & keep);
+            } else {
+                uint32_t top = 0;                    // largest size, as the bits of a bf16
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
-                        const uint32_t a = __vmaxu2(x[c].x & 0x7FFF7FFFu, x[c].y & 0x7FFF7FFFu), b = __vmaxu2(x[c].z & 0x7FFF7FFFu, x[c].w & 0x7FFF7FFFu);
-                        top = __vmaxu2(top, __vmaxu2(a, b));
-                    }
-                    top = max(top & 0xFFFFu, top >> 16);
-                    int e = 14 - ((int)(top >> 7) - 127);
-                    e = top > 0 && top < 0x7F80u ? max(-120, min(120, e)) : 0;
-                    const float up = p.scale == 0.f ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale < 0.f ? -1.f : 1.f);
-                    f = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
-                        uint32_t y[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) y[i] = pack_f16(__uint_as_float(y[i] << 16) * up, __uint_as_float(y[i] & 0xFFFF0000u) * up);
-                        x[c] = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
+                for (int c = 0; c < D / 8; ++c) {
+                    const uint32_t a = __vmaxu2(x[c].x & 0x7FFF7FFFu, x[c].y & 0x7FFF7FFFu), b = __vmaxu2(x[c].z & 0x7FFF7FFFu, x[c].w & 0x7FFF7FFFu);
+                    top = __vmaxu2(top, __vmaxu2(a, b));
                 }
-                // (a scale of zero moves into the queries: hidden scores of minus infinity stay what they are)
-                cs = (p.scale == 0.f ? 1.f : fabsf(p.scale)) * f;
+                top = max(top & 0xFFFFu, top >> 16);
+                int e = 14 - ((int)(top >> 7) - 127);
+                e = top > 0 && top < 0x7F80u ? max(-120, min(120, e)) : 0;
+                const float up = p.scale == 0.f ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23) * (p.scale < 0.f ? -1.f : 1.f);
+                f = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4 *>(qt + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) = x[c];
-                skn_fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) skn_mbar_arrive(&q_full[tile]);
-                const int ta = (g.row0 + tile * 128) / p.group, tb = (g.row0 + min(tile * 128 + 127, g.rows - 1)) / p.group;
-                const int pmin = g.len - g.n + ta, pmax = g.len - g.n + tb;
+                for (int c = 0; c < D / 8; ++c) {
+                    uint32_t y[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = pack_f16(__uint_as_float(y[i] << 16) * up, __uint_as_float(y[i] & 0xFFFF0000u) * up);
+                    x[c] = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4 *>(qt + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) = x[c];
+            skn_fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) skn_mbar_arrive(&q_full[tile]);
+            // (a scale of zero moves into the queries: hidden scores of minus infinity stay what they are)
+            return (p.scale == 0.f ? 1.f : fabsf(p.scale)) * f;
+        };
+        bool more = pp_next(p, w, g);
+        float cs_next = 0.f;
+        if (more && tile * 128 < g.rows) cs_next = load_queries();
+        while (more) {
+            const PagedSegment now = g;              // g: the next one, whose queries are handed over before this one's outputs are written
+            const int R = tile * 128 + r;
+            const bool real = R < now.rows, used = tile * 128 < now.rows;
+            const int t = (now.row0 + R) / p.group, pos = real ? now.len - now.n + t : -1;
+            const float cs = cs_next;
+            float m = PA_NONE, l = 0.f;
+            if (used && ok) {
+                const int ta = (now.row0 + tile * 128) / p.group, tb = (now.row0 + min(tile * 128 + 127, now.rows - 1)) / p.group;
+                const int pmin = now.len - now.n + ta, pmax = now.len - now.n + tb;
 
-                // 64 keys at a time, in two places that take turns: the scores of the next are there before these are done with
-                for (int k = 0; k < 2 * (g.u1 - g.u0); ++k, ++n_subs) {
-                    const int i = g.u0 + (k >> 1), k0 = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS + (k & 1) * PP_SUB;
-                    const uint32_t at = ts + (k & 1) * PP_SUB;
-                    if (!tc_wait_warp(&s_full[2 * tile + (k & 1)], (n_subs >> 1) & 1, lane)) { ok = false; break; }
+                for (int j = 0; j < now.u1 - now.u0; ++j, ++n_units) {
+                    const int i = now.u0 + j, k0 = (i < now.span.a ? i : i + now.span.gap) * PP_KEYS;
+                    if (!tc_wait_warp(&s_full[tile], n_units & 1, lane)) { ok = false; break; }
                     tc_fence_after();
-                    float v[PP_SUB];
-                    pp_ld32(at, v);
-                    pp_ld32(at + 32, v + 32);
-                    pp_wait_ld<PP_SUB>(v);
-                    const bool whole = k0 + PP_SUB - 1 <= pmin && (!p.window || k0 > pmax - p.window || k0 + PP_SUB <= p.sinks);
+                    float v[PP_KEYS];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) pp_ld32(ts + 32 * c, v + 32 * c);
+                    pp_wait_ld<PP_KEYS>(v);
+                    const bool whole = k0 + PP_KEYS - 1 <= pmin && (!p.window || k0 > pmax - p.window || k0 + PP_KEYS <= p.sinks);
                     if (!whole) {
                         const int hi = pos - k0, lo = p.window ? pos - p.window + 1 - k0 : -1, sk = p.sinks - k0;
 #pragma unroll
-                        for (int c = 0; c < PP_SUB; ++c)
-                            if (c > hi || (c < lo && c >= sk)) v[c] = -INFINITY;
+                        for (int b = 0; b < PP_KEYS; b += 32) {
+                            const uint32_t seen = pp_below(hi + 1 - b) & (~pp_below(lo - b) | pp_below(sk - b));
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) v[b + c] = seen >> c & 1 ? v[b + c] : -INFINITY;
+                        }
                     }
                     float top = pp_max3(v[0], v[1], v[2]), top2 = pp_max3(v[3], v[4], v[5]);     // (a NaN stays one)
 #pragma unroll
-                    for (int c = 6; c < 62; c += 4) {
+                    for (int c = 6; c < 126; c += 4) {
                         top = pp_max3(top, v[c], v[c + 1]);
                         top2 = pp_max3(top2, v[c + 2], v[c + 3]);
                     }
-                    top = pp_max3(top, v[62], v[63]);
+                    top = pp_max3(top, v[126], v[127]);
                     top = pp_max3(top, top2, top2);
                     if (top != top) l = top;
                     top *= cs;
@@ -350,8 +387,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         const float fresh = fmaxf(m, top), fix = pp_ex2(m - fresh);
                         m = fresh;
                         l *= fix;
-                        if (k > 0) {
-                            if (!tc_wait_warp(&pv_done[tile], (n_subs - 1) & 1, lane)) { ok = false; break; }
+                        if (j > 0) {
+                            if (!tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane)) { ok = false; break; }
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < D; c += 32) {
@@ -359,7 +396,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                                 pp_ld32(to + c, o);
                                 pp_wait_ld<32>(o);
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] *= fix;
+                                for (int k = 0; k < 32; ++k) o[k] *= fix;
                                 pp_st32(to + c, reinterpret_cast<uint32_t *>(o));
                             }
                             tc_wait_st();
@@ -367,93 +404,79 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     }
                     const uint64_t cs2 = skn_pack2(cs, cs), off2 = skn_pack2(T::LIFT - m, T::LIFT - m);
                     uint64_t sum = 0;
-                    auto weigh = [&](auto all) {
-                        constexpr bool ALL = decltype(all)::value;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
                         uint32_t pk[32];
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            const uint64_t x = skn_fma2(skn_pack2(v[2 * c], v[2 * c + 1]), cs2, off2);
-                            const uint64_t y = ALL || c % 8 < 5 ? pp_ex2_unit(x) : pp_ex2_fma(x);
+                            const uint64_t x = skn_fma2(skn_pack2(v[64 * h + 2 * c], v[64 * h + 2 * c + 1]), cs2, off2);
+                            const uint64_t y = c % 8 < 5 ? pp_ex2_unit(x) : pp_ex2_fma(x);
                             sum = skn_add2(sum, y);
                             float a, b;
                             skn_unpack2(y, a, b);
                             pk[c] = T::BF ? pack_bf16(a, b) : pack_f16(a, b);
                         }
-                        pp_st32(at, pk);
-                    };
-                    if (whole) weigh(std::false_type());
-                    else weigh(std::true_type());    // hidden weights are exactly zero
+                        pp_st32(ts + 32 * h, pk);
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) skn_mbar_arrive(&p_full[2 * tile + h]);
+                    }
                     float a, b;
                     skn_unpack2(sum, a, b);
                     l += a + b;
-                    tc_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) skn_mbar_arrive(&p_full[2 * tile + (k & 1)]);
-                }
-                // (one after the other: the last scores say that the product before the last two is done, and a parity tells a phase from the one before it only)
-                if (ok) ok = tc_wait_warp(&pv_done[tile], n_subs & 1, lane) && tc_wait_warp(&pv_done[tile], (n_subs - 1) & 1, lane);
-                if (!ok) {
-                    if (lane == 0) *st.status = SKN_ERR_TIMEOUT;
                 }
             }
+            // the next segment's queries: these are done with since the last scores
+            more = pp_next(p, w, g);
+            if (more && tile * 128 < g.rows) cs_next = load_queries();
             // ---- out, or to the other CTAs of the block -------------------------------------------------------------------------
-            const bool shared = g.n_parts > 1;
-            float *part = p.parts + (int64_t)g.slot * PP_ROWS * (D + 4);          // [D / 4][256] float4, then [256] maximum, [256] sum
-            IO *const out = static_cast<IO *>(p.out) + (int64_t)(g.first + t) * p.out_stride + (g.head * p.group + (g.row0 + R) % p.group) * D;
+            const bool shared = now.n_parts > 1;
+            float *part = p.parts + (int64_t)now.slot * PP_ROWS * (D + 4);          // [D / 4][256] float4, then [256] maximum, [256] sum
+            IO *const out = static_cast<IO *>(p.out) + (int64_t)(now.first + t) * p.out_stride + (now.head * p.group + (now.row0 + R) % p.group) * D;
             bool odd = false;
-            if (used && ok) {
+            if (used) {
+                if (ok) ok = tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane);
+                if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
                 tc_fence_after();
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                uint8_t *const qt = q_tile + tile * TILE + r * 128;          // the tile's queries are done with: rows gather there
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
                     pp_ld32(to + c, o);
                     pp_wait_ld<32>(o);
+                    if (c + 32 == D) {               // the accumulators may be written again
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) skn_mbar_arrive(&o_free[tile]);
+                    }
                     float s = 0.f;
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        if (shared) {
-                            reinterpret_cast<float4 *>(part)[((c + k) / 4) * PP_ROWS + R] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                            reinterpret_cast<float4 *>(part)[((c + k) / 4 + 1) * PP_ROWS + R] = make_float4(o[k + 4], o[k + 5], o[k + 6], o[k + 7]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) o[k + e] = l == 0.f ? 0.f : o[k + e] * inv;
-                            const int cc = (c + k) / 8;
-                            *reinterpret_cast<uint4 *>(qt + (cc >> 3) * 16384 + (((cc & 7) ^ (r & 7)) << 4)) =
-                                make_uint4(pack_bf16(o[k], o[k + 1]), pack_bf16(o[k + 2], o[k + 3]), pack_bf16(o[k + 4], o[k + 5]), pack_bf16(o[k + 6], o[k + 7]));
-                        }
-                        s += ((o[k] + o[k + 1]) + (o[k + 2] + o[k + 3])) + ((o[k + 4] + o[k + 5]) + (o[k + 6] + o[k + 7]));
-                    }
+                    for (int k = 0; k < 32; ++k) s += o[k];
                     odd |= !(fabsf(s) < INFINITY);
-                }
-                if (!shared) {                       // and leave it whole
-                    __syncwarp();
-                    const uint64_t mine = real ? reinterpret_cast<uint64_t>(out) : 0;
-                    const uint8_t *from = q_tile + tile * TILE + (r & ~31) * 128;
-#pragma unroll 4
-                    for (int it = 0; it < D / 8; ++it) {
-                        const int row = it * 32 / (D / 8) + lane / (D / 8), cc = lane % (D / 8);
-                        const uint64_t at = __shfl_sync(0xffffffffu, mine, row);
-                        const uint4 y = *reinterpret_cast<const uint4 *>(from + row * 128 + (cc >> 3) * 16384 + (((cc & 7) ^ (row & 7)) << 4));
-                        if (at) *reinterpret_cast<uint4 *>(at + 16 * cc) = y;
+                    if (shared) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) reinterpret_cast<float4 *>(part)[((c + k) / 4) * PP_ROWS + R] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                    } else {
+                        uint32_t y[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) y[k] = l == 0.f ? 0u : pack_bf16(o[2 * k] * inv, o[2 * k + 1] * inv);
+                        if (real) {
+#pragma unroll
+                            for (int k = 0; k < 16; k += 8) pp_store32(out + c + 2 * k, y + k, wide);
+                        }
                     }
-                    __syncwarp();
                 }
                 odd = real && (odd || !(fabsf(l) < INFINITY));
                 if (shared) {
                     part[D * PP_ROWS + R] = m;
                     part[(D + 1) * PP_ROWS + R] = l;
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) skn_mbar_arrive(&o_free[tile]);
             }
             if (pp_any(odd)) {
-                const PagedSegment mine = g;         // (a copy: the address of the one that the loops use is not taken)
-                paged_redo<CT, D, IO>(p, mine, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
-                    const int tr = (g.row0 + row) / p.group;
+                const PagedSegment again = now;      // (a copy: the address of the one that the loops use is not taken)
+                paged_redo<CT, D, IO>(p, again, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
+                    const int tr = (now.row0 + row) / p.group;
                     if (shared) {
                         if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;
                         if (tid == 0) {
@@ -461,42 +484,50 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                             part[(D + 1) * PP_ROWS + row] = rl;
                         }
                     } else if (tid < D)
-                        static_cast<IO *>(p.out)[(int64_t)(g.first + tr) * p.out_stride + (g.head * p.group + (g.row0 + row) % p.group) * D + tid] =
+                        static_cast<IO *>(p.out)[(int64_t)(now.first + tr) * p.out_stride + (now.head * p.group + (now.row0 + row) % p.group) * D + tid] =
                             __float2bfloat16_rn(rl == 0.f ? 0.f : acc / rl);
                 });
             }
             if (shared) {
                 __threadfence();
                 pp_bar();
-                if (tid == 0) ticket = atomicInc(&p.tickets[paged_slot(g, g.c0)], (unsigned)g.n_parts - 1);
+                if (tid == 0) ticket = atomicInc(&p.tickets[paged_slot(now, now.c0)], (unsigned)now.n_parts - 1);
                 pp_bar();
-                if (ticket == (unsigned)g.n_parts - 1 && real) {
+                if (ticket == (unsigned)now.n_parts - 1 && real) {
                     __threadfence();
+                    auto part_of = [&](int k) { return p.parts + (int64_t)paged_slot(now, now.c0 + min(k, now.n_parts - 1)) * PP_ROWS * (D + 4); };
                     float top = PA_NONE, sum = 0.f;
-                    for (int k = 0; k < g.n_parts; ++k) top = fmaxf(top, __ldcg(p.parts + (int64_t)paged_slot(g, g.c0 + k) * PP_ROWS * (D + 4) + D * PP_ROWS + R));
-                    for (int k = 0; k < g.n_parts; ++k) {
-                        const float *from = p.parts + (int64_t)paged_slot(g, g.c0 + k) * PP_ROWS * (D + 4);
-                        sum = fmaf(__ldcg(from + (D + 1) * PP_ROWS + R), exp2f(__ldcg(from + D * PP_ROWS + R) - top), sum);
-                    }
+                    for (int k = 0; k < now.n_parts; ++k) top = fmaxf(top, __ldcg(part_of(k) + D * PP_ROWS + R));
+                    for (int k = 0; k < now.n_parts; ++k) sum = fmaf(__ldcg(part_of(k) + (D + 1) * PP_ROWS + R), exp2f(__ldcg(part_of(k) + D * PP_ROWS + R) - top), sum);
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        float4 o[8] = {};
-                        for (int k = 0; k < g.n_parts; ++k) {
-                            const float *from = p.parts + (int64_t)paged_slot(g, g.c0 + k) * PP_ROWS * (D + 4);
-                            const float f = exp2f(__ldcg(from + D * PP_ROWS + R) - top);
-                            if (f == 0.f) continue;
+                    for (int c = 0; c < D; c += 16) {
+                        float4 o[4] = {};
+                        for (int k = 0; k < now.n_parts; k += 4) {       // four parts' loads on their way at once
+                            float4 y[4][4];
+                            float f[4];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float4 y = __ldcg(reinterpret_cast<const float4 *>(from) + (c / 4 + e) * PP_ROWS + R);
-                                o[e].x = fmaf(y.x, f, o[e].x); o[e].y = fmaf(y.y, f, o[e].y); o[e].z = fmaf(y.z, f, o[e].z); o[e].w = fmaf(y.w, f, o[e].w);
+                            for (int b = 0; b < 4; ++b) {
+                                f[b] = k + b < now.n_parts ? exp2f(__ldcg(part_of(k + b) + D * PP_ROWS + R) - top) : 0.f;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) y[b][e] = __ldcg(reinterpret_cast<const float4 *>(part_of(k + b)) + (c / 4 + e) * PP_ROWS + R);
                             }
-                        }
-                        const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) {
-                            const float x[8] = {o[e].x * inv, o[e].y * inv, o[e].z * inv, o[e].w * inv, o[e + 1].x * inv, o[e + 1].y * inv, o[e + 1].z * inv, o[e + 1].w * inv};
-                            io_store8(out + c + 4 * e, x);
+                            for (int b = 0; b < 4; ++b)
+                                if (f[b] != 0.f)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        o[e].x = fmaf(y[b][e].x, f[b], o[e].x); o[e].y = fmaf(y[b][e].y, f[b], o[e].y);
+                                        o[e].z = fmaf(y[b][e].z, f[b], o[e].z); o[e].w = fmaf(y[b][e].w, f[b], o[e].w);
+                                    }
                         }
+                        uint32_t y[8];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            y[2 * e] = pack_bf16(o[e].x * inv, o[e].y * inv);
+                            y[2 * e + 1] = pack_bf16(o[e].z * inv, o[e].w * inv);
+                        }
+                        pp_store32(out + c, y, wide);
                     }
                 }
                 pp_bar();                            // (the ticket is read)
@@ -508,9 +539,9 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::REGS_MMA));
     if (warp == 8) {
         constexpr uint32_t FMT = T::BF ? 1u << 7 | 1u << 10 : 0u;
-        constexpr uint32_t ID_S = 1u << 4 | FMT | (PP_SUB >> 3) << 17 | 8u << 24, ID_O = 1u << 4 | FMT | 1u << 16 | (D >> 3) << 17 | 8u << 24;
+        constexpr uint32_t ID_S = 1u << 4 | FMT | (PP_KEYS >> 3) << 17 | 8u << 24, ID_O = 1u << 4 | FMT | 1u << 16 | (D >> 3) << 17 | 8u << 24;
         int slot = 0, parity = 0;                    // of the next K or V
-        uint32_t segs[2] = {0, 0}, done[2] = {0, 0};        // done: pieces of a tile before this segment
+        uint32_t units[2] = {0, 0}, segs[2] = {0, 0};
         bool ok = true;
         auto step = [&] {
             if (++slot == SLOTS) {
@@ -518,67 +549,69 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 parity ^= 1;
             }
         };
-        // S of a tile against half b of the keys in slot `at`
-        auto scores = [&](int tile, int b, int at) {
-            const uint32_t qa = skn_smem_u32(q_tile + tile * TILE), ka = skn_smem_u32(ring + at * TILE) + b * PP_SUB * 128;
+        auto scores = [&](int tile, int at) {        // S of a tile from the keys in slot `at`
+            const uint32_t qa = skn_smem_u32(q_tile + tile * TILE), ka = skn_smem_u32(ring + at * TILE);
             if (tc_elect()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-                    tc_mma_bf16(tmem + tile * 128 + b * PP_SUB, tc_smem_desc(qa + off), tc_smem_desc(ka + off), ID_S, k > 0);
+                    tc_mma_bf16(tmem + tile * 128, tc_smem_desc(qa + off), tc_smem_desc(ka + off), ID_S, k > 0);
                 }
-                tc_commit(&s_full[2 * tile + b]);
+                tc_commit(&s_full[tile]);
             }
             __syncwarp();
         };
         while (ok && pp_next(p, w, g)) {
             const int n = g.u1 - g.u0, tiles = g.rows > 128 ? 2 : 1;
+            int k_slot = slot;
             for (int x = 0; x < tiles && ok; ++x) ok = tc_wait_warp(&q_full[x], segs[x] & 1, lane);
             ok = ok && tc_wait_warp(&full[slot], parity, lane);
             if (!ok) break;
             tc_fence_after();
-            for (int b = 0; b < 2; ++b)
-                for (int x = 0; x < tiles; ++x) scores(x, b, slot);
-            if (tc_elect()) tc_commit(&empty[slot]);
+            for (int x = 0; x < tiles; ++x) scores(x, slot);
+            if (tc_elect()) tc_commit(&empty[k_slot]);
             __syncwarp();
             step();
             for (int j = 0; j < n && ok; ++j) {
                 const int v_slot = slot;
                 ok = tc_wait_warp(T::Q4 ? &full[slot] : &clean[slot], parity, lane);
                 step();
-                const bool more = j + 1 < n;         // the keys of the next unit lie in `slot`
+                const bool more = j + 1 < n;
+                k_slot = slot;
                 const uint32_t va = skn_smem_u32(ring + v_slot * TILE);
-                for (int b = 0; b < 2 && ok; ++b)
-                    for (int x = 0; x < tiles && ok; ++x) {
-                        ok = tc_wait_warp(&p_full[2 * x + b], ((done[x] >> 1) + j) & 1, lane);
-                        if (ok && j == 0 && b == 0 && segs[x] > 0) ok = tc_wait_warp(&o_free[x], (segs[x] - 1) & 1, lane);
+                for (int x = 0; x < tiles && ok; ++x) {
+                    for (int h = 0; h < 2 && ok; ++h) {          // the weights come in halves
+                        ok = tc_wait_warp(&p_full[2 * x + h], units[x] & 1, lane);
+                        if (ok && j == 0 && h == 0 && segs[x] > 0) ok = tc_wait_warp(&o_free[x], (segs[x] - 1) & 1, lane);
                         if (!ok) break;
                         tc_fence_after();
                         if (tc_elect()) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                tc_mma_ts(tmem + 256 + x * D, tmem + x * 128 + b * PP_SUB + 8 * k, pp_desc_n(va + (4 * b + k) * 2048, PP_KEYS * 128), ID_O, j > 0 || b > 0 || k > 0);
-                            tc_commit(&pv_done[x]);
-                            if (b && x == tiles - 1) tc_commit(&empty[v_slot]);
-                        }
-                        __syncwarp();
-                        if (more) {
-                            if (x == 0 && b == 0) ok = tc_wait_warp(&full[slot], parity, lane);
-                            if (!ok) break;
-                            tc_fence_after();
-                            scores(x, b, slot);
-                            if (b && x == tiles - 1) {
-                                if (tc_elect()) tc_commit(&empty[slot]);
-                                __syncwarp();
+                            for (int k = 4 * h; k < 4 * h + 4; ++k)
+                                tc_mma_ts(tmem + 256 + x * D, tmem + x * 128 + 8 * k, pp_desc_n(va + k * 2048, PP_KEYS * 128), ID_O, j > 0 || k > 0);
+                            if (h) {
+                                tc_commit(&pv_done[x]);
+                                if (x == tiles - 1) tc_commit(&empty[v_slot]);
                             }
                         }
+                        __syncwarp();
                     }
+                    if (!ok) break;
+                    ++units[x];
+                    if (more) {
+                        if (x == 0) ok = tc_wait_warp(&full[k_slot], parity, lane);
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(x, k_slot);
+                        if (x == tiles - 1) {
+                            if (tc_elect()) tc_commit(&empty[k_slot]);
+                            __syncwarp();
+                        }
+                    }
+                }
                 if (more) step();
             }
-            for (int x = 0; x < tiles; ++x) {
-                ++segs[x];
-                done[x] += 2 * n;
-            }
+            for (int x = 0; x < tiles; ++x) ++segs[x];
         }
         if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
     }

@@ -21,7 +21,7 @@ struct skn_paged {
     double *d_turns;             // [rot_dims / 2] half turns per position
     // Attention's workspace (skn_paged_attn.cu): tensor maps of the pools and, for rows whose keys several CTAs share, their partial results
     CUtensorMap map[4];          // K, V; of Q4_0 their quants, then their scales
-    CUtensorMap wide[2];         // K, V in whole pages and half rows (prompts)
+    CUtensorMap wide[4];         // the same in larger boxes (prompts): whole pages of half rows; of Q4_0 up to 32 rows
     int n_parts;                 // CTAs that share a launch's work
     float *d_parts;              // decoding: [2 n_parts][SKN_PAGED_PART_ROWS][head_dim + 4]: output, maximum, sum; prompts: rows of two CTAs' blocks per SM
     unsigned *d_tickets;         // [2 n_parts], zero between launches

@@ -28,15 +28,17 @@ cudaError_t skn_paged_attn_prepare(skn_paged *pc) {
             const cuuint32_t whole[3] = {64, (cuuint32_t)P, 1};
             if (e == cudaSuccess) e = encode(&pc->wide[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, pool, dim, stride, whole, CU_TENSOR_MAP_SWIZZLE_128B);
         } else {
-            const cuuint32_t rows = P < 32 ? P : 32;
-            // quants of 16 or 32 rows, in words: [D / 32][rows][4]; scales [rows][D / 32], two to a word
-            const cuuint64_t dim[3] = {(cuuint64_t)P * 4, (cuuint64_t)D / 32, heads}, stride[2] = {(cuuint64_t)P * 16, (cuuint64_t)pc->head_bytes};
-            const cuuint32_t box[3] = {rows * 4, (cuuint32_t)D / 32, 1};
-            e = encode(&pc->map[i], CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, pool, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_NONE);
-            pc->wide[i] = pc->map[i];
-            const cuuint64_t sdim[2] = {(cuuint64_t)P * D / 64, heads}, sstride[1] = {(cuuint64_t)pc->head_bytes};
-            const cuuint32_t sbox[2] = {rows * (cuuint32_t)D / 64, 1};
-            if (e == cudaSuccess) e = encode(&pc->map[2 + i], CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, pool + (size_t)P * D / 2, sdim, sstride, sbox, CU_TENSOR_MAP_SWIZZLE_NONE);
+            // quants of 16 rows (wide: up to 32), in words: [D / 32][rows][4]; scales [rows][D / 32], two to a word
+            for (int w = 0; w < 2 && e == cudaSuccess; ++w) {
+                const cuuint32_t rows = w && P > 16 ? 32 : 16;
+                CUtensorMap *to = w ? pc->wide : pc->map;
+                const cuuint64_t dim[3] = {(cuuint64_t)P * 4, (cuuint64_t)D / 32, heads}, stride[2] = {(cuuint64_t)P * 16, (cuuint64_t)pc->head_bytes};
+                const cuuint32_t box[3] = {rows * 4, (cuuint32_t)D / 32, 1};
+                e = encode(&to[i], CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, pool, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+                const cuuint64_t sdim[2] = {(cuuint64_t)P * D / 64, heads}, sstride[1] = {(cuuint64_t)pc->head_bytes};
+                const cuuint32_t sbox[2] = {rows * (cuuint32_t)D / 64, 1};
+                if (e == cudaSuccess) e = encode(&to[2 + i], CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, pool + (size_t)P * D / 2, sdim, sstride, sbox, CU_TENSOR_MAP_SWIZZLE_NONE);
+            }
         }
     }
     pc->n_parts = 2 * pc->ctx->sm_count;

@@ -27,13 +27,24 @@
 #include <math.h>
 
 constexpr int PA_WARPS = 8, PA_THREADS = 32 * PA_WARPS;
-constexpr int PA_MAX_SEQS = 1024;            // sequences whose work is shared out; more of them take a CTA per segment
+constexpr int PA_MAX_SEQS = 512;            // sequences whose work is shared out; more of them take a CTA per segment
 constexpr float PA_NONE = -1e30f;            // running maximum before the first score
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d = a b + c
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ float pa_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 template <class CT> __device__ __forceinline__ void mma_as(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<CT, __nv_bfloat16>::value) mma_bf16(c, a, b0, b1);
@@ -191,6 +202,16 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
     bar();
 }
 
+// four dimensions of a segment's row to the output
+template <class IO> __device__ __forceinline__ void paged_out4(const PagedAttn &p, const PagedSegment &g, int r, int d, int dims, float4 x, float sum) {
+    const int t = (g.row0 + r) / p.group;
+    IO *to = static_cast<IO *>(p.out) + (int64_t)(g.first + t) * p.out_stride + (g.head * p.group + (g.row0 + r) % p.group) * dims + d;
+    if (sum == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
+    else x = make_float4(x.x / sum, x.y / sum, x.z / sum, x.w / sum);
+    if constexpr (sizeof(IO) == 4) *reinterpret_cast<float4 *>(to) = x;
+    else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+}
+
 template <class CT, int D, int NB, bool EX> struct PaTraits {
     static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
     static constexpr int UNIT = Q4 ? 32 : 16;
@@ -205,8 +226,8 @@ template <class CT, int D, int NB, bool EX> struct PaTraits {
     // Weights reach 2^SLACK before the maximum moves.  In fp16 they are lifted to 2^15 at most, so that a weight of 2^-24 - 15 + SLACK of its row's largest is
     // the last one there; fp32 rows, whose second term ends there too, pay for a smaller SLACK with more moves
     static constexpr int SLACK = EX ? 1 : 4;
-    static constexpr float LIFT = BF ? 1.f : EX ? 16384.f : 2048.f;
-    static constexpr int V_UP = EX ? 12 : 7;                                      // Q4_0: the largest d, times 2^-E, is 2^V_UP .. 2^(V_UP + 1) when E is set
+    static constexpr int LIFT = BF ? 0 : EX ? 14 : 11;                            // exponent; the maximum that weights are taken from is that much less
+    static constexpr int V_UP = EX ? 12 : 7;                                      // Q4_0: the largest d, times 2^lift, is 2^V_UP .. 2^(V_UP + 1) when the lift is set
     static constexpr bool Q_SMEM = NB > 1 || (Q4 && EX);                          // query fragments in shared memory instead of registers
     static constexpr int KS = D / 16;
     static constexpr int RING = PA_WARPS * STAGES * STAGE;
@@ -228,6 +249,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
     uint2 *qf = reinterpret_cast<uint2 *>(ring + T::BODY);
     __shared__ uint64_t full[PA_WARPS * STAGES];
     __shared__ long long before[PA_MAX_SEQS + 1];
+    __shared__ int seq_first[PA_MAX_SEQS], seq_n[PA_MAX_SEQS], seq_len[PA_MAX_SEQS];
     __shared__ float wml[PA_WARPS][2 * ROWS], rml[2 * ROWS];
     __shared__ float scratch[D + PA_THREADS + PA_WARPS];
     __shared__ long long wsum_s[PA_WARPS];
@@ -250,7 +272,10 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             long long x = 0;
             if (s < st.n_seqs) {
                 const PagedSeq sq = paged_seq(st, s);
-                if (sq.n > 0) x = paged_span(p, sq.len - sq.n, sq.len - 1, UNIT).units;
+                seq_first[s] = sq.first;
+                seq_n[s] = sq.n;
+                seq_len[s] = sq.len;
+                if (sq.n > 0) x = paged_span(p, sq.len - sq.n, sq.len - 1, UNIT).units + (1LL << 40);      // and one segment a head
             }
             long long inc = x;
 #pragma unroll
@@ -265,15 +290,14 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 if (w < warp) base += wsum_s[w];
                 run += wsum_s[w];
             }
-            if (s < st.n_seqs) before[s] = (base + inc - x) * st.heads;
+            if (s < st.n_seqs) before[s] = ((base + inc - x) & ((1LL << 40) - 1)) * st.heads;
             __syncthreads();
         }
-        total = run * st.heads;
-        if (tid == 0) before[st.n_seqs] = total;
-        __syncthreads();
+        total = (run & ((1LL << 40) - 1)) * st.heads;
         if (total == 0) return;
-        // fewer CTAs where each would get less than a unit per warp
-        const long long want = (total + PA_WARPS - 1) / PA_WARPS;
+        // fewer CTAs where each would get less than a unit per warp; short segments get one each (nothing to join)
+        const long long segments = (run >> 40) * st.heads;
+        const long long want = total <= 2 * PA_WARPS * segments ? segments : (total + PA_WARPS - 1) / PA_WARPS;
         n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
         if ((int)blockIdx.x >= n_cta) return;
         u = total * blockIdx.x / n_cta;
@@ -306,23 +330,58 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 if (before[mid] <= u) lo = mid; else hi = mid - 1;
             }
             s_at = g.seq = lo;
-            const PagedSeq sq = paged_seq(st, g.seq);
-            g.n = sq.n; g.len = sq.len; g.first = sq.first;
-            g.row0 = 0; g.rows = sq.n * p.group;
-            g.span = paged_span(p, sq.len - sq.n, sq.len - 1, UNIT);
+            g.n = seq_n[lo]; g.len = seq_len[lo]; g.first = seq_first[lo];
+            g.row0 = 0; g.rows = g.n * p.group;
+            g.span = paged_span(p, g.len - g.n, g.len - 1, UNIT);
             const long long off = u - before[lo];
             g.head = (int)(off / g.span.units);
             g.u0 = (int)(off - (long long)g.head * g.span.units);
             const long long left = u_end - u;
             g.u1 = left < g.span.units - g.u0 ? g.u0 + (int)left : g.span.units;
-            const long long a = u - g.u0;
-            g.c0 = (int)(((a + 1) * n_cta - 1) / total);
-            g.n_parts = (int)(((a + g.span.units) * n_cta - 1) / total) - g.c0 + 1;
+            g.c0 = (int)blockIdx.x;
+            g.n_parts = 1;
+            if (g.u0 > 0 || g.u1 < g.span.units) {
+                const long long a = u - g.u0;
+                g.c0 = (int)(((a + 1) * n_cta - 1) / total);
+                g.n_parts = (int)(((a + g.span.units) * n_cta - 1) / total) - g.c0 + 1;
+            }
             g.slot = paged_slot(g, (int)blockIdx.x);
             u += g.u1 - g.u0;
         }
         const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
         const int n_mine = (g.u1 - g.u0 - warp + PA_WARPS - 1) / PA_WARPS;         // units g.u0 + warp + PA_WARPS j
+
+        // ---- queries, on their way while the pages are looked up: this lane's part of row g8 of each block of eight ---------------
+        // 16-bit caches: dims 16 k + 2 t, + 1, + 8, + 9.  Q4_0: of block k / 2, its lower (k even) or upper 16: 4 t, + 2, + 1, + 3
+        float x[NB][KS][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = 8 * nb + g8, t = (g.row0 + r) / p.group;
+            const IO *q = static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + r) % p.group) * D;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                float a[4] = {};
+                if (r < g.rows) {
+                    if constexpr (EX && T::Q4) {
+                        const float4 y = *reinterpret_cast<const float4 *>(q + 16 * k + 4 * t4);
+                        a[0] = y.x; a[1] = y.z; a[2] = y.y; a[3] = y.w;
+                    } else if constexpr (EX) {
+                        const float2 y = *reinterpret_cast<const float2 *>(q + 16 * k + 2 * t4), z = *reinterpret_cast<const float2 *>(q + 16 * k + 8 + 2 * t4);
+                        a[0] = y.x; a[1] = y.y; a[2] = z.x; a[3] = z.y;
+                    } else if constexpr (T::Q4) {
+                        const uint2 y = *reinterpret_cast<const uint2 *>(q + 16 * k + 4 * t4);
+                        a[0] = __uint_as_float(y.x << 16); a[1] = __uint_as_float(y.y << 16);
+                        a[2] = __uint_as_float(y.x & 0xFFFF0000u); a[3] = __uint_as_float(y.y & 0xFFFF0000u);
+                    } else {
+                        const uint32_t y = *reinterpret_cast<const uint32_t *>(q + 16 * k + 2 * t4), z = *reinterpret_cast<const uint32_t *>(q + 16 * k + 8 + 2 * t4);
+                        a[0] = __uint_as_float(y << 16); a[1] = __uint_as_float(y & 0xFFFF0000u);
+                        a[2] = __uint_as_float(z << 16); a[3] = __uint_as_float(z & 0xFFFF0000u);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[nb][k][i] = a[i];
+            }
+        }
 
         // ---- loads of the warp's units: lane j of `pages` holds the pages of unit j (mod 32) ---------------------------------
         int page0 = -1, page1 = -1;
@@ -346,39 +405,26 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         look_up(0);
         uint8_t *const mine = ring + warp * STAGES * T::STAGE;
         uint32_t there = 0;                        // two bits a stage: which 16 keys of its unit have a page
-        auto issue = [&](int j, int at) {          // every lane calls it, the first one works
+        auto issue = [&](int j, int at) {          // a lane per box of 16 rows: K and V, Q4_0: quants and scales of both halves
             const int pg0 = __shfl_sync(0xffffffffu, page0, j & 31), pg1 = T::Q4 ? __shfl_sync(0xffffffffu, page1, j & 31) : -1;
             there = (there & ~(3u << (2 * at))) | ((uint32_t)(pg0 >= 0) << (2 * at)) | ((uint32_t)(pg1 >= 0) << (2 * at + 1));
+            uint64_t *bar = &full[warp * STAGES + at];
+            const int row = key_of(j) & ((1 << st.page_shift) - 1);
+            uint8_t *const to = mine + at * T::STAGE + (lane & 1) * T::TILE;
             if (lane == 0) {
-                uint64_t *bar = &full[warp * STAGES + at];
-                uint8_t *k = mine + at * T::STAGE, *v = k + T::TILE;
-                const int row = key_of(j) & ((1 << st.page_shift) - 1);
-                if constexpr (!T::Q4) {
-                    if (pg0 < 0) skn_mbar_arrive(bar);
-                    else {
-                        skn_mbar_expect_tx(bar, 2 * UNIT * T::ROW);
-                        const int y = ((pg0 * st.heads + g.head) << st.page_shift) + row;
-                        tma_3d(k, &mk, 0, y, 0, bar);
-                        tma_3d(v, &mv, 0, y, 0, bar);
-                    }
-                } else {
-                    // pages of 16: a box each for the two halves; else one box of 32 rows.  Quants [D / 32][rows][16], then scales [rows][D / 32]
-                    const bool two = st.page_shift == 4;
-                    const int bytes = (two ? 16 : 32) * T::ROW * 2;
-                    const int n = two ? (pg0 >= 0) + (pg1 >= 0) : (pg0 >= 0 || pg1 >= 0);
-                    if (n == 0) skn_mbar_arrive(bar);
-                    else {
-                        skn_mbar_expect_tx(bar, n * bytes);
-                        for (int h = 0; h < (two ? 2 : 1); ++h) {
-                            const int pg = h || (!two && pg0 < 0) ? pg1 : pg0;
-                            if (pg < 0) continue;
-                            const int z = pg * st.heads + g.head, off = h * T::HALF, sc = (two ? 16 : 32) * (D / 2);
-                            tma_3d(k + off, &mk, row * 4, 0, z, bar);
-                            tma_3d(v + off, &mv, row * 4, 0, z, bar);
-                            tc_tma_load_2d(k + off + sc, &mks, row * (D / 64), z, bar);
-                            tc_tma_load_2d(v + off + sc, &mvs, row * (D / 64), z, bar);
-                        }
-                    }
+                const int n = (pg0 >= 0) + (pg1 >= 0);
+                if (n) skn_mbar_expect_tx(bar, n * 32 * T::ROW);
+                else skn_mbar_arrive(bar);
+            }
+            __syncwarp();
+            if constexpr (!T::Q4) {
+                if (lane < 2 && pg0 >= 0) tma_3d(to, lane ? &mv : &mk, 0, ((pg0 * st.heads + g.head) << st.page_shift) + row, 0, bar);
+            } else {
+                // quants [D / 32][16][16 bytes], then scales [16][D / 32]
+                const int h = (lane >> 2) & 1, pg = h ? pg1 : pg0, z = pg * st.heads + g.head, r = (row + 16 * h) & ((1 << st.page_shift) - 1);
+                if (lane < 8 && pg >= 0) {
+                    if (lane & 2) tc_tma_load_2d(to + h * T::HALF + 16 * (D / 2), lane & 1 ? &mvs : &mks, r * (D / 64), z, bar);
+                    else tma_3d(to + h * T::HALF, lane & 1 ? &mv : &mk, r * 4, 0, z, bar);
                 }
             }
         };
@@ -386,40 +432,20 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         int issued = dead ? n_mine : 0;
         for (int i = 0; i < STAGES && issued < n_mine; ++i, ++issued) issue(issued, (stage + i) % STAGES);
 
-        // ---- queries: fragments of the second operand, lane (row g8 of each block of eight, t4) ------------------------------
-        // fp16 products take them times a power of two that brings a row's largest to 2^14 .. 2^15
+        // ---- fragments of the second operand: fp16 products take queries times a power of two that brings a row's largest to 2^14 .. 2^15 ---
         uint32_t qr[T::Q_SMEM ? 1 : NT][T::Q_SMEM ? 1 : NB][KS][2];
         float cs[NB][2];                           // factor of the scores of rows 2 t4, 2 t4 + 1
         float bias[T::Q4 ? NB : 1][T::Q4 ? NBLK : 1][2];
         int pos[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const int r = 8 * nb + g8;
-            const bool real = r < g.rows;
-            const int t = (g.row0 + r) / p.group;
-            const IO *q = static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + r) % p.group) * D;
-            float x[KS][4];
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // 16-bit caches: dims 16 k + 2 t, + 1, + 8, + 9.  Q4_0: of block k / 2, its lower (k even) or upper 16: 4 t, + 2, + 1, + 3
-                    const int d = T::Q4 ? 16 * k + 4 * t4 + ((i & 1) << 1) + (i >> 1) : 16 * k + 2 * t4 + (i & 1) + 8 * (i >> 1);
-                    x[k][i] = 0.f;
-                    if constexpr (EX) {
-                        if (real) x[k][i] = q[d];
-                    } else {
-                        if (real) x[k][i] = __bfloat162float(q[d]);
-                    }
-                }
-            }
             float f = 1.f;
             if constexpr (!T::BF) {
                 float top = 0.f;
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[k][i]));
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(x[nb][k][i]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 int e = 14 - ((int)(__float_as_uint(top) >> 23) - 127);
@@ -429,22 +455,22 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[k][i] *= up;
+                    for (int i = 0; i < 4; ++i) x[nb][k][i] *= up;
             }
             float bs[T::Q4 ? NBLK : 1];
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 if constexpr (T::Q4) {
-                    const float sum = (x[k][0] + x[k][1]) + (x[k][2] + x[k][3]);
+                    const float sum = (x[nb][k][0] + x[nb][k][1]) + (x[nb][k][2] + x[nb][k][3]);
                     if (k & 1) bs[k >> 1] += sum; else bs[k >> 1] = sum;
                     if (k & 1) {                    // the upper nibble stands 16 times higher
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) x[k][i] *= 0.0625f;
+                        for (int i = 0; i < 4; ++i) x[nb][k][i] *= 0.0625f;
                     }
                 }
                 uint32_t a[NT], b[NT];
-                terms_of<CT, NT>(x[k][0], x[k][1], a);
-                terms_of<CT, NT>(x[k][2], x[k][3], b);
+                terms_of<CT, NT>(x[nb][k][0], x[nb][k][1], a);
+                terms_of<CT, NT>(x[nb][k][2], x[nb][k][3], b);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if constexpr (T::Q_SMEM) {
@@ -477,7 +503,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         if constexpr (T::Q_SMEM) __syncthreads();
 
         // ---- the units ------------------------------------------------------------------------------------------------------
-        float o[D / 16][NB][4], m[NB][2], l[NB][2];
+        float o[D / 16][NB][4], m[NB][2], mlim[NB][2], l[NB][2];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -488,12 +514,11 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                m[nb][c] = PA_NONE;
+                m[nb][c] = mlim[nb][c] = PA_NONE;
                 l[nb][c] = 0.f;
             }
-        float ve = 1.f;                            // Q4_0: 2^-E
-        float ve_inv = 1.f;
-        __half2 vlim = __floats2half2_rn(0.f, 0.f); // and the largest |d| that it takes
+        int lift = T::Q4 ? 0 : T::LIFT;            // m: the maximum less this; mlim: the maximum and SLACK
+        __half2 vlim = __floats2half2_rn(0.f, 0.f); // Q4_0: the largest |d| that the lift takes
         for (int j = 0; j < n_mine && !dead; ++j) {
             const int kbase = key_of(j);
             bool gone = false;
@@ -551,18 +576,12 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 const bool hidden_page = !(sub ? has1 : has0);
                 float s[NB][4];
                 // ---- scores ------------------------------------------------------------------------------------------------
-                const uint8_t *vq = nullptr;       // Q4_0: this half's rows of V, and between blocks
-                int bstep = 0;
+                const uint8_t *vq = nullptr;       // Q4_0: this half's rows of V
                 float dv[2][T::Q4 ? NBLK : 1];
                 __half2 dtop = vlim;
                 if constexpr (T::Q4) {
-                    const bool two = st.page_shift == 4;
-                    bstep = two ? 256 : 512;
-                    const int off = two ? sub * T::HALF : sub * 256;
-                    const uint8_t *kq = kt + off;
-                    const uint8_t *kd = kt + (two ? sub * T::HALF + 16 * (D / 2) : 32 * (D / 2) + sub * 16 * (D / 16));
-                    vq = vt + off;
-                    const uint8_t *vd = vt + (kd - kt);
+                    const uint8_t *kq = kt + sub * T::HALF, *kd = kq + 16 * (D / 2), *vd = vt + sub * T::HALF + 16 * (D / 2);
+                    vq = vt + sub * T::HALF;
                     float dk[2][NBLK];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -590,13 +609,13 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                         for (int c = 0; c < 4; ++c) s[nb][c] = 0.f;
 #pragma unroll
                     for (int b = 0; b < NBLK; ++b) {
-                        const uint32_t w0 = *reinterpret_cast<const uint32_t *>(kq + b * bstep + g8 * 16 + t4 * 4);
-                        const uint32_t w1 = *reinterpret_cast<const uint32_t *>(kq + b * bstep + (g8 + 8) * 16 + t4 * 4);
+                        const uint32_t w0 = *reinterpret_cast<const uint32_t *>(kq + b * 256 + g8 * 16 + t4 * 4);
+                        const uint32_t w1 = *reinterpret_cast<const uint32_t *>(kq + b * 256 + (g8 + 8) * 16 + t4 * 4);
                         const uint32_t lo[4] = {w0 & 0x000F000Fu, w1 & 0x000F000Fu, (w0 >> 8) & 0x000F000Fu, (w1 >> 8) & 0x000F000Fu};
                         const uint32_t hi[4] = {w0 & 0x00F000F0u, w1 & 0x00F000F0u, (w0 >> 8) & 0x00F000F0u, (w1 >> 8) & 0x00F000F0u};
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            float acc[4] = {bias[nb][b][0], bias[nb][b][1], bias[nb][b][0], bias[nb][b][1]};
+                            float acc[4];
 #pragma unroll
                             for (int n = NT - 1; n >= 0; --n) {
                                 uint2 f0, f1;
@@ -607,7 +626,8 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                                     f0 = make_uint2(qr[n][nb][2 * b][0], qr[n][nb][2 * b][1]);
                                     f1 = make_uint2(qr[n][nb][2 * b + 1][0], qr[n][nb][2 * b + 1][1]);
                                 }
-                                mma_f16(acc, lo, f0.x, f0.y);
+                                if (n == NT - 1) mma_f16_from(acc, lo, f0.x, f0.y, bias[nb][b][0], bias[nb][b][1]);
+                                else mma_f16(acc, lo, f0.x, f0.y);
                                 mma_f16(acc, hi, f1.x, f1.y);
                             }
                             s[nb][0] = fmaf(acc[0], dk[0][b], s[nb][0]);
@@ -647,7 +667,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                     for (int c = 0; c < 4; ++c) {
                         s[nb][c] *= cs[nb][c & 1];
                         if (!whole && (hidden_page || !paged_sees(p, key0 + g8 + 8 * (c >> 1), pos[nb][c & 1]))) s[nb][c] = -INFINITY;
-                        move |= s[nb][c] > m[nb][c & 1] + (float)T::SLACK;
+                        move |= s[nb][c] > mlim[nb][c & 1];
                     }
                 if constexpr (T::Q4) move |= !__hble2(dtop, vlim);
                 if (__any_sync(0xffffffffu, move)) {
@@ -659,9 +679,10 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                            top = fmaxf(top, m[nb][c]);
-                            const float fix = exp2f(m[nb][c] - top);
+                            top = fmaxf(top, mlim[nb][c] - (float)T::SLACK) - (float)lift;
+                            const float fix = pa_ex2(m[nb][c] - top);
                             m[nb][c] = top;
+                            mlim[nb][c] = top + (float)(lift + T::SLACK);
                             l[nb][c] *= fix;
 #pragma unroll
                             for (int i = 0; i < D / 16; ++i) {
@@ -686,18 +707,23 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
 #pragma unroll
                         for (int o2 = 1; o2 < 32; o2 <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
                         if (top > __half2float(__low2half(vlim))) {
-                            // up to LIFT: weights stay within 2^15
-                            const int e = (int)(__float_as_uint(top) >> 23) - 127 - T::V_UP;
-                            const float fresh = __uint_as_float((uint32_t)(127 - e) << 23), fix = fresh * ve_inv;
-                            ve = fresh;
-                            ve_inv = __uint_as_float((uint32_t)(127 + e) << 23);
-                            vlim = __float2half2_rn(fminf(ve_inv * T::LIFT, 65504.f));
+                            // up to 2^LIFT: weights stay within 2^15
+                            const int fresh = T::V_UP + 127 - (int)(__float_as_uint(top) >> 23), by = fresh - lift;
+                            const float fix = __uint_as_float((uint32_t)(127 + by) << 23);
+                            lift = fresh;
+                            vlim = __float2half2_rn(fminf(__uint_as_float((uint32_t)(127 + T::LIFT - fresh) << 23), 65504.f));
 #pragma unroll
-                            for (int nb = 0; nb < NB; ++nb)
+                            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    m[nb][c] -= (float)by;
+                                    l[nb][c] *= fix;
+                                }
 #pragma unroll
                                 for (int i = 0; i < D / 16; ++i)
 #pragma unroll
                                     for (int c = 0; c < 4; ++c) o[i][nb][c] *= fix;
+                            }
                         }
                     }
                 }
@@ -705,7 +731,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        s[nb][c] = exp2f(s[nb][c] - m[nb][c & 1]);
+                        s[nb][c] = pa_ex2(s[nb][c] - m[nb][c & 1]);
                         l[nb][c & 1] += s[nb][c];
                     }
                 // ---- values ------------------------------------------------------------------------------------------------
@@ -723,8 +749,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                         uint32_t pb[NB][NT][2];
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            const float d0 = dv[0][b] * ve, d1 = dv[1][b] * ve;
-                            const float w0 = s[nb][0] * d0, w1 = s[nb][1] * d0, w2 = s[nb][2] * d1, w3 = s[nb][3] * d1;
+                            const float w0 = s[nb][0] * dv[0][b], w1 = s[nb][1] * dv[0][b], w2 = s[nb][2] * dv[1][b], w3 = s[nb][3] * dv[1][b];
                             uint32_t a[NT], c[NT];
                             terms_of<CT, NT>(w0, w1, a);
                             terms_of<CT, NT>(w2, w3, c);
@@ -734,7 +759,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                                 pb[nb][n][1] = movm(c[n]);
                             }
                         }
-                        const uint8_t *at = vq + b * bstep + 2 * t4 * 16 + (g8 & 3) * 4;
+                        const uint8_t *at = vq + b * 256 + 2 * t4 * 16 + (g8 & 3) * 4;
                         const uint32_t x0 = *reinterpret_cast<const uint32_t *>(at), x1 = *reinterpret_cast<const uint32_t *>(at + 16);
                         const uint32_t x2 = *reinterpret_cast<const uint32_t *>(at + 128), x3 = *reinterpret_cast<const uint32_t *>(at + 144);
                         const uint32_t lo = __byte_perm(x0, x1, 0x5410), lo2 = __byte_perm(x2, x3, 0x5410), hi = __byte_perm(x0, x1, 0x7632), hi2 = __byte_perm(x2, x3, 0x7632);
@@ -753,8 +778,8 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         uint32_t a[NT], c[NT];
-                        terms_of<CT, NT>(s[nb][0] * T::LIFT, s[nb][1] * T::LIFT, a);
-                        terms_of<CT, NT>(s[nb][2] * T::LIFT, s[nb][3] * T::LIFT, c);
+                        terms_of<CT, NT>(s[nb][0], s[nb][1], a);
+                        terms_of<CT, NT>(s[nb][2], s[nb][3], c);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             pb[nb][n][0] = movm(a[n]);
@@ -806,32 +831,28 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                     float *to = comb + (warp * ROWS + r) * (D + 4);
                     if constexpr (T::Q4) {
 #pragma unroll
-                        for (int b = 0; b < NBLK; ++b) {
+                        for (int b = 0; b < NBLK; ++b)
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const int d = 32 * b + 4 * (g8 & 3) + 16 * (g8 >> 2) + 2 * i;
-                                *reinterpret_cast<float2 *>(to + d) = make_float2(o[2 * b + i][nb][c] * ve_inv, o[2 * b + i][nb][c + 2] * ve_inv);
-                            }
-                        }
+                            for (int i = 0; i < 2; ++i)
+                                *reinterpret_cast<float2 *>(to + 32 * b + 4 * (g8 & 3) + 16 * (g8 >> 2) + 2 * i) = make_float2(o[2 * b + i][nb][c], o[2 * b + i][nb][c + 2]);
                     } else {
-                        constexpr float DOWN = 1.f / T::LIFT;
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i) {
-                            to[16 * i + g8] = o[i][nb][c] * DOWN;
-                            to[16 * i + g8 + 8] = o[i][nb][c + 2] * DOWN;
+                            to[16 * i + g8] = o[i][nb][c];
+                            to[16 * i + g8 + 8] = o[i][nb][c + 2];
                         }
                     }
                 }
             __syncthreads();
-            // maximum, sum and output of all warps
+            // maximum, sum and output of all warps, out or to the other CTAs of the segment
             if (tid < ROWS) {
                 float top = PA_NONE;
 #pragma unroll
-                for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, wml[w][2 * tid]);
+                for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, wml[w][2 * tid + 1] != 0.f ? wml[w][2 * tid] : PA_NONE);
                 float sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < PA_WARPS; ++w) {
-                    const float f = exp2f(wml[w][2 * tid] - top);
+                    const float f = wml[w][2 * tid + 1] != 0.f ? exp2f(wml[w][2 * tid] - top) : 0.f;
                     sum += wml[w][2 * tid + 1] * f;
                     wml[w][2 * tid] = f;
                 }
@@ -839,80 +860,84 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 rml[2 * tid + 1] = sum;
             }
             __syncthreads();
-            for (int i = tid; i < ROWS * (D / 4); i += PA_THREADS) {
-                const int r = i / (D / 4), d = i % (D / 4) * 4;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int w = 0; w < PA_WARPS; ++w) {
-                    const float f = wml[w][2 * r];
-                    const float4 y = *reinterpret_cast<const float4 *>(comb + (w * ROWS + r) * (D + 4) + d);
-                    if (f != 0.f) { x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w); }
-                }
-                *reinterpret_cast<float4 *>(comb + r * (D + 4) + d) = x;        // (warp 0's place: read by this thread alone)
-                const float sum = (x.x + x.y) + (x.z + x.w) + rml[2 * r + 1];
-                if (!(fabsf(sum) < INFINITY) && r < g.rows) flags[0] = 1;       // (a sum of finite values that overflows is computed again for nothing)
-            }
-            __syncthreads();
-            if (flags[0]) {
-                paged_redo<CT, D, IO>(p, g, UNIT, scratch, [] { __syncthreads(); }, [&](int r, float rm, float rl, float acc) {
-                    if (tid < D) comb[r * (D + 4) + tid] = acc;
-                    if (tid == 0) {
-                        rml[2 * r] = rm;
-                        rml[2 * r + 1] = rl;
-                    }
-                });
-                if (tid == 0) flags[0] = 0;
-            }
         }
-        // ---- out, or to the other CTAs of the segment ---------------------------------------------------------------------------
-        bool last = true;
-        if (g.n_parts > 1) {
-            float *part = p.parts + (int64_t)g.slot * SKN_PAGED_PART_ROWS * (D + 4);
+        float *const part = p.parts + (int64_t)g.slot * SKN_PAGED_PART_ROWS * (D + 4);
+        auto put4 = [&](int r, int d, float4 x, float m, float sum) {       // four dimensions of a row's result
+            if (g.n_parts > 1) {
+                *reinterpret_cast<float4 *>(part + r * (D + 4) + d) = x;
+                if (d == 0) *reinterpret_cast<float2 *>(part + r * (D + 4) + D) = make_float2(m, sum);
+            } else
+                paged_out4<IO>(p, g, r, d, D, x, sum);
+        };
+        for (int i = tid; i < g.rows * (D / 4); i += PA_THREADS) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; ++w) {
+                const float f = wml[w][2 * r];
+                const float4 y = *reinterpret_cast<const float4 *>(comb + (w * ROWS + r) * (D + 4) + d);
+                if (f != 0.f) { x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w); }
+            }
+            const float sum = rml[2 * r + 1], all = (x.x + x.y) + (x.z + x.w) + sum;
+            if (!(fabsf(all) < INFINITY)) flags[0] = 1;             // (a sum of finite values that overflows is computed again for nothing)
+            put4(r, d, x, rml[2 * r], sum);
+        }
+        if (g.n_parts > 1) __threadfence();
+        __syncthreads();
+        if (flags[0]) {
+            const PagedSegment again = g;          // (a copy: the address of the one that the loops use is not taken)
+            paged_redo<CT, D, IO>(p, again, UNIT, scratch, [] { __syncthreads(); }, [=](int r, float rm, float rl, float acc) {
+                if (tid < D) comb[r * (D + 4) + tid] = acc;
+                if (tid == 0) {
+                    comb[r * (D + 4) + D] = rm;
+                    comb[r * (D + 4) + D + 1] = rl;
+                }
+            });
             for (int i = tid; i < g.rows * (D / 4); i += PA_THREADS) {
                 const int r = i / (D / 4), d = i % (D / 4) * 4;
-                const float4 x = *reinterpret_cast<const float4 *>(comb + r * (D + 4) + d);
-                *reinterpret_cast<float4 *>(part + r * (D + 4) + d) = x;
+                put4(r, d, *reinterpret_cast<const float4 *>(comb + r * (D + 4) + d), comb[r * (D + 4) + D], comb[r * (D + 4) + D + 1]);
             }
-            if (tid < g.rows) {
-                part[tid * (D + 4) + D] = rml[2 * tid];
-                part[tid * (D + 4) + D + 1] = rml[2 * tid + 1];
-            }
+            if (tid == 0) flags[0] = 0;
             __threadfence();
             __syncthreads();
+        }
+        // ---- the last CTA of a segment joins what all of them left ------------------------------------------------------------------
+        if (g.n_parts > 1) {
             if (tid == 0) ticket = atomicInc(&p.tickets[paged_slot(g, g.c0)], (unsigned)g.n_parts - 1);
             __syncthreads();
-            last = ticket == (unsigned)g.n_parts - 1;
-            if (last) {
+            if (ticket == (unsigned)g.n_parts - 1) {
                 __threadfence();
                 for (int i = tid; i < g.rows * (D / 4); i += PA_THREADS) {
                     const int r = i / (D / 4), d = i % (D / 4) * 4;
-                    float top = PA_NONE;
-                    for (int k = 0; k < g.n_parts; ++k)
-                        top = fmaxf(top, __ldcg(p.parts + ((int64_t)paged_slot(g, g.c0 + k) * SKN_PAGED_PART_ROWS + r) * (D + 4) + D));
-                    float sum = 0.f;
+                    float top = PA_NONE, sum = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int k = 0; k < g.n_parts; ++k) {
-                        const float *from = p.parts + ((int64_t)paged_slot(g, g.c0 + k) * SKN_PAGED_PART_ROWS + r) * (D + 4);
-                        const float f = exp2f(__ldcg(from + D) - top);
-                        if (f == 0.f) continue;
-                        sum = fmaf(__ldcg(from + D + 1), f, sum);
-                        const float4 y = __ldcg(reinterpret_cast<const float4 *>(from + d));
-                        x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
-                    }
-                    *reinterpret_cast<float4 *>(comb + r * (D + 4) + d) = x;
-                    if (d == 0) rml[2 * r + 1] = sum;
-                }
-                __syncthreads();
-            }
-        }
-        if (last) {
-            for (int i = tid; i < g.rows * (D / 8); i += PA_THREADS) {
-                const int r = i / (D / 8), d = i % (D / 8) * 8, t = (g.row0 + r) / p.group;
-                const float sum = rml[2 * r + 1];
-                float x[8];
+                    for (int k = 0; k < g.n_parts; k += 8) {        // eight parts' loads on their way at once
+                        float2 ml[8];
+                        float4 y[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = sum == 0.f ? 0.f : comb[r * (D + 4) + d + k] / sum;
-                io_store8(static_cast<IO *>(p.out) + (int64_t)(g.first + t) * p.out_stride + (g.head * p.group + (g.row0 + r) % p.group) * D + d, x);
+                        for (int b = 0; b < 8; ++b) {
+                            const float *from = p.parts + ((int64_t)paged_slot(g, g.c0 + min(k + b, g.n_parts - 1)) * SKN_PAGED_PART_ROWS + r) * (D + 4);
+                            ml[b] = __ldcg(reinterpret_cast<const float2 *>(from + D));
+                            y[b] = __ldcg(reinterpret_cast<const float4 *>(from + d));
+                        }
+                        float high = top;
+#pragma unroll
+                        for (int b = 0; b < 8; ++b)
+                            if (k + b < g.n_parts && ml[b].y != 0.f) high = fmaxf(high, ml[b].x);
+                        const float fix = exp2f(top - high);
+                        top = high;
+                        sum *= fix;
+                        x.x *= fix; x.y *= fix; x.z *= fix; x.w *= fix;
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) {
+                            if (k + b >= g.n_parts || ml[b].y == 0.f) continue;
+                            const float f = exp2f(ml[b].x - top);
+                            sum = fmaf(ml[b].y, f, sum);
+                            x.x = fmaf(y[b].x, f, x.x); x.y = fmaf(y[b].y, f, x.y); x.z = fmaf(y[b].z, f, x.z); x.w = fmaf(y[b].w, f, x.w);
+                        }
+                    }
+                    paged_out4<IO>(p, g, r, d, D, x, sum);
+                }
             }
         }
         skn_fence_proxy_async();                   // the rings were written to as results
@@ -921,10 +946,18 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
+// once per kernel and device (`done`: a bit each; setting it twice does no harm)
+template <class K> static cudaError_t paged_attributes(K *kern, size_t smem, int device, uint64_t *done) {
+    if (device < 64 && __atomic_load_n(done, __ATOMIC_RELAXED) >> device & 1) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && device < 64) __atomic_fetch_or(done, (uint64_t)1 << device, __ATOMIC_RELAXED);
+    return e;
+}
 template <class CT, int D, int NB, bool EX> static cudaError_t attn_launch(const skn_paged *pc, const PagedAttn &p) {
     using T = PaTraits<CT, D, NB, EX>;
     auto *kern = skn_paged_attn_kernel<CT, D, NB, EX>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM);
+    static uint64_t done = 0;
+    const cudaError_t e = paged_attributes(kern, T::SMEM, pc->ctx->device, &done);
     if (e != cudaSuccess) return e;
     const int64_t rows = (int64_t)p.st.max_new * p.group;
     const dim3 grid = p.direct ? dim3((unsigned)((rows + T::ROWS - 1) / T::ROWS), (unsigned)p.st.heads, (unsigned)p.st.n_seqs) : dim3((unsigned)(T::PER_SM * pc->ctx->sm_count));

@@ -794,8 +794,9 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
 template <class CT, int D> static cudaError_t prompt_launch(const skn_paged *pc, const PagedAttn &p) {
     using T = PpTraits<CT, D>;
     auto *kern = skn_paged_prompt_kernel<CT, D>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM);
+    static uint64_t done = 0;
+    const cudaError_t e = paged_attributes(kern, T::SMEM, pc->ctx->device, &done);
     if (e != cudaSuccess) return e;
-    kern<<<pc->ctx->sm_count, T::THREADS, T::SMEM, pc->ctx->stream>>>(p, pc->wide[0], pc->wide[1], pc->map[2], pc->map[3]);
+    kern<<<pc->ctx->sm_count, T::THREADS, T::SMEM, pc->ctx->stream>>>(p, pc->wide[0], pc->wide[1], pc->wide[2], pc->wide[3]);
     return cudaGetLastError();
 }

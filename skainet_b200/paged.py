@@ -10,21 +10,18 @@ import numpy as np
 from . import _ffi
 from .tensor import Context, SKN_OK, _check, _ptr, _raise
 
-_IO = {"float32": 0, "bfloat16": 3}
+_IO = {"torch.float32": 0, "torch.bfloat16": 3}
+_io_of_dtype = {}                # torch's own objects, as they are met (torch is not imported here)
 
 
 def _io_of(t) -> int:
-    io = _IO.get(str(t.dtype).rpartition(".")[2])
+    io = _io_of_dtype.get(t.dtype)
     if io is None:
-        raise ValueError("rows are float32 or bfloat16")
+        io = _IO.get(str(t.dtype))
+        if io is None:
+            raise ValueError("rows are float32 or bfloat16")
+        _io_of_dtype[t.dtype] = io
     return io
-
-
-def _row_stride(t, n_tokens: int, heads: int, dim: int) -> int:
-    """elements between the rows of a device tensor [n_tokens, heads, dim] whose rows are dense"""
-    if t.shape != (n_tokens, heads, dim) or t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
-        raise ValueError("Shapes do not align.")
-    return t.stride(0) if n_tokens > 1 else heads * dim
 
 
 class PagedBatch:
@@ -142,31 +139,47 @@ class PagedKVCache:
         return out
 
     # ---- device tensors -----------------------------------------------------------------------------------------------------
-    def _same(self, batch, io, *tensors):
-        if batch.device != self.ctx.device or any(not t.is_cuda or t.device.index != self.ctx.device or _io_of(t) != io for t in tensors):
-            raise ValueError("the step's tensors are on the context's device and of one type")
+    def _row_stride(self, t, dtype, n: int, heads: int) -> int:
+        """elements between the rows of a device tensor [n, heads, head_dim] whose rows are dense"""
+        D, stride = self.head_dim, t.stride()
+        if t.dtype is not dtype or t.get_device() != self.ctx.device or tuple(t.shape) != (n, heads, D) or stride[2] != 1 or (stride[1] != D and heads > 1):
+            raise ValueError("Shapes do not align." if t.dtype is dtype and t.get_device() == self.ctx.device
+                             else "the step's tensors are on the context's device and of one type")
+        return stride[0] if n > 1 else heads * D
 
     def append_dev(self, batch: PagedBatch, k, v, q=None, q_out=None):
         """rows may be parts of wider ones (a joint projection); q_out may be q"""
-        io, n, kv, D = _io_of(k), batch.n_tokens, self.n_kv_heads, self.head_dim
-        self._same(batch, io, k, v, *(() if q is None else (q, q_out)))
-        heads = 0 if q is None else q.shape[1]
-        more = (None, 0, 0, None, 0) if q is None else (q.data_ptr(), _row_stride(q, n, heads, D), heads, q_out.data_ptr(), _row_stride(q_out, n, heads, D))
-        _check(self.ctx.handle, self._lib.skn_paged_append_dev(self._h, batch._ref, io, k.data_ptr(), _row_stride(k, n, kv, D), v.data_ptr(),
-                                                              _row_stride(v, n, kv, D), *more))
+        io, n, kv, dt, row = _io_of(k), batch.n_tokens, self.n_kv_heads, k.dtype, self._row_stride
+        if batch.device != self.ctx.device:
+            raise ValueError("the step's tensors are on the context's device and of one type")
+        if q is None:
+            more = (None, 0, 0, None, 0)
+        else:
+            heads = q.shape[1]
+            more = (q.data_ptr(), row(q, dt, n, heads), heads, q_out.data_ptr(), row(q_out, dt, n, heads))
+        rc = self._lib.skn_paged_append_dev(self._h, batch._ref, io, k.data_ptr(), row(k, dt, n, kv), v.data_ptr(), row(v, dt, n, kv), *more)
+        if rc:
+            _raise(self.ctx.handle, rc)
 
     def gather_dev(self, batch: PagedBatch, k_out, v_out):
         io, shape = _io_of(k_out), (batch.n_tokens, self.n_kv_heads, self.head_dim)
-        self._same(batch, io, k_out, v_out)
+        if batch.device != self.ctx.device or any(t.get_device() != self.ctx.device or t.dtype is not k_out.dtype for t in (k_out, v_out)):
+            raise ValueError("the step's tensors are on the context's device and of one type")
         if k_out.shape != shape or v_out.shape != shape or not k_out.is_contiguous() or not v_out.is_contiguous():
             raise ValueError("Shapes do not align.")
-        _check(self.ctx.handle, self._lib.skn_paged_gather_dev(self._h, batch._ref, io, k_out.data_ptr(), v_out.data_ptr()))
+        rc = self._lib.skn_paged_gather_dev(self._h, batch._ref, io, k_out.data_ptr(), v_out.data_ptr())
+        if rc:
+            _raise(self.ctx.handle, rc)
 
     def attend_dev(self, batch: PagedBatch, q, out, scale: Optional[float] = None, window: int = 0, sinks: int = 0):
-        io, n, heads, D = _io_of(q), batch.n_tokens, q.shape[1], self.head_dim
-        self._same(batch, io, q, out)
-        _check(self.ctx.handle, self._lib.skn_paged_attn_dev(self._h, batch._ref, io, q.data_ptr(), _row_stride(q, n, heads, D), heads,
-                                                            self._scale if scale is None else scale, window, sinks, out.data_ptr(), _row_stride(out, n, heads, D)))
+        """out may be q"""
+        io, n, heads, row = _io_of(q), batch.n_tokens, q.shape[1], self._row_stride
+        if batch.device != self.ctx.device:
+            raise ValueError("the step's tensors are on the context's device and of one type")
+        rc = self._lib.skn_paged_attn_dev(self._h, batch._ref, io, q.data_ptr(), row(q, q.dtype, n, heads), heads, self._scale if scale is None else scale,
+                                          window, sinks, out.data_ptr(), row(out, q.dtype, n, heads))
+        if rc:
+            _raise(self.ctx.handle, rc)
 
     def close(self):
         if self._h:

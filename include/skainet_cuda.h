@@ -346,7 +346,7 @@ typedef struct skn_paged skn_paged;
 #define SKN_ROT_ADJACENT 0  /* dimension 2 i turns with 2 i + 1 */
 #define SKN_ROT_HALVES 1    /* dimension i turns with i + rot_dims / 2 */
 typedef struct skn_paged_spec {
-    int32_t n_kv_heads, head_dim;    /* head_dim 64 or 128 */
+    int32_t n_kv_heads, head_dim;    /* up to 256 heads of 64 or 128 */
     int32_t page_tokens;             /* 16, 32, 64 or 128 */
     int32_t kv_dtype;                /* SKN_KV_F16, SKN_KV_BF16, SKN_KV_Q4_0 */
     int32_t n_pages;
@@ -379,7 +379,7 @@ int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_
 int32_t skn_paged_destroy(skn_paged *pc);
 int32_t skn_paged_info(const skn_paged *pc, void **k_pool_dev, void **v_pool_dev, int64_t *pool_bytes);
 /* Append the step's keys and values, the keys rotated to their positions; q (optional) is rotated into q_out, which may be q.
- * `_dev`: io is the element type of k, v, q and q_out (SKN_KV_F32 or SKN_KV_BF16), a row [heads][head_dim]; strides are the elements from one
+ * `_dev`: at most 2^24 rows a step; io is the element type of k, v, q and q_out (SKN_KV_F32 or SKN_KV_BF16), a row [heads][head_dim]; strides are the elements from one
  * row to the next (rows of a joint projection need no copy).  Pointers and rows are 16-byte aligned.  A page that a step appends to belongs to
  * one of its sequences only.  The host form takes dense fp32 rows and answers every mistake before anything has run. */
 int32_t skn_paged_append(skn_paged *pc, const skn_paged_batch *batch, const float *k_host, const float *v_host, const float *q_host,

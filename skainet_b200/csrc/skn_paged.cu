@@ -5,10 +5,13 @@
 #include <new>
 
 // ---- append -------------------------------------------------------------------------------------------------------------
-// One CTA per token: its sequence is looked up, the sines and cosines of its position are formed once in shared memory (in 64 bits: the angle of a
-// far position, and keys that land next to a border of the cache's rounding), and its threads take 16 dimensions of a head at a time, eight and
-// the eight they turn with, so that the rotation may happen in place.
-constexpr int PAGED_APPEND_THREADS = 128;
+// A CTA takes one token, or four of a long step (TOKENS).  Where each of them goes is looked up and the sines and cosines of its position are formed
+// once, in shared memory (in 64 bits: the angle of a far position, and keys that land next to a border of the cache's rounding); its threads
+// take 16 dimensions of a head at a time, eight and the eight they turn with, so that the rotation may happen in place.  The rows are
+// requested a unit ahead, the first before all that.
+// Bound by HBM from a few thousand tokens on: 8192 tokens of 32 + 2 x 8 heads of 128, bf16 rows and cache, one token a CTA and requests behind
+// the sines 96 us, four and ahead of them in the tables below.
+constexpr int PAGED_LONG_STEP = 2048;        // tokens from which a CTA takes four: with fewer the GPU is not full of CTAs of one
 
 // sequence of row i: the last one that starts at or before it (-1: none).  Every warp counts the starts for itself, 32 at a time.
 __device__ __forceinline__ int paged_find(const PagedStep &st, int i) {
@@ -23,9 +26,13 @@ __device__ __forceinline__ int paged_find(const PagedStep &st, int i) {
     return n - 1 < st.n_seqs ? n - 1 : -1;
 }
 
-// q of one value: x * fp32(1 / d) + 8.5 in 64 bits, cut off
+// q of one value: x * fp32(1 / d) + 8.5 in 64 bits, cut off.  The sum with one rounding in fp32 is off by 2^-21 at most, so that 64 bits are
+// needed within 2^-18 of a whole number only.
 __device__ __forceinline__ uint32_t q4_of(float x, float inv) {
-    const int q = (int)__dadd_rn(__dmul_rn((double)x, (double)inv), 8.5);
+    const float t = fmaf(x, inv, 8.5f);
+    int q = (int)t;
+    const float f = t - (float)q;
+    if (f < 0x1p-18f || f > 1.f - 0x1p-18f) q = (int)__dadd_rn(__dmul_rn((double)x, (double)inv), 8.5);
     return (uint32_t)(q < 0 ? 0 : q > 15 ? 15 : q);
 }
 // Eight dims of a 32-dim block in each of four neighbouring lanes (all of them here): quants and scale to the page
@@ -61,123 +68,179 @@ struct PagedRows {                                     // rows of the step's tok
     uint8_t *k_pool, *v_pool;
 };
 
-template <class CT, int D, class IO>
-__global__ void __launch_bounds__(PAGED_APPEND_THREADS) skn_paged_append_kernel(const PagedStep st, const PagedRows r) {
-    constexpr bool Q4 = sizeof(CT) == 1;
-    extern __shared__ float staged[];                  // Q4: the rotated keys, [heads][D]
-    __shared__ double2 turn[D / 2];
-    const int i = blockIdx.x;
-    const int s = paged_find(st, i);
-    if (s < 0) return;
+struct PagedPlace { int pos, page, row; };             // of a token: its position (negative: nowhere), page (negative: none) and row of the page
+// by a whole warp
+__device__ __forceinline__ PagedPlace paged_place(const PagedStep &st, int i) {
+    PagedPlace at = {-1, -1, 0};
+    const int s = i < st.n_tokens ? paged_find(st, i) : -1;
+    if (s < 0) return at;
     const PagedSeq q = paged_seq(st, s);
-    const int pos = q.len - q.n + i - q.first;
-    if (i >= q.first + q.n || pos < 0) return;
-    const int page = paged_page(st, s, pos), row = pos & ((1 << st.page_shift) - 1);
-    for (int j = threadIdx.x; j < r.rot / 2; j += PAGED_APPEND_THREADS) {
-        double2 t;
-        sincospi((double)pos * r.turns[j], &t.y, &t.x);
-        turn[j] = t;
+    if (i >= q.first + q.n) return at;
+    at.pos = q.len - q.n + i - q.first;
+    if (at.pos >= 0) {
+        at.page = paged_page(st, s, at.pos);
+        at.row = at.pos & ((1 << st.page_shift) - 1);
+    }
+    return at;
+}
+
+// eight dimensions and the eight they turn with, by fp32 or (keys) fp64 sines; c: the unit of 16.  Pair 8 c + i lies at [i][c]: the units of a
+// head are neighbouring lanes (at [8 c + i] they met in the same banks: 8192 tokens 52 us instead of the 43 of this form)
+template <int UNITS, class F2, class F> __device__ __forceinline__ void paged_turn(float (&x)[8], float (&y)[8], const F2 *turn, int c, bool halves) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (halves) {
+            const F2 t = turn[j * UNITS + c];
+            const F a = x[j], b = y[j];
+            x[j] = (float)(a * t.x - b * t.y);
+            y[j] = (float)(a * t.y + b * t.x);
+        } else if (!(j & 1)) {
+            const F2 t = turn[(j >> 1) * UNITS + c], w = turn[(4 + (j >> 1)) * UNITS + c];
+            const F x0 = x[j], x1 = x[j + 1], y0 = y[j], y1 = y[j + 1];
+            x[j] = (float)(x0 * t.x - x1 * t.y);
+            x[j + 1] = (float)(x0 * t.y + x1 * t.x);
+            y[j] = (float)(y0 * w.x - y1 * w.y);
+            y[j + 1] = (float)(y0 * w.y + y1 * w.x);
+        }
+    }
+}
+
+// eight elements as they lie in memory
+template <class IO> struct IoRow8 {
+    float f[8];
+    __device__ __forceinline__ void load(const IO *p) { io_load8(p, f); }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = f[i];
+    }
+};
+template <> struct IoRow8<__nv_bfloat16> {
+    uint4 u;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { u = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+
+template <class CT, int D, class IO, int TOKENS>
+__global__ void __launch_bounds__(TOKENS == 1 ? 128 : 256, TOKENS == 1 ? 8 : 4) skn_paged_append_kernel(const PagedStep st, const PagedRows r) {
+    constexpr bool Q4 = sizeof(CT) == 1;
+    constexpr int THREADS = TOKENS == 1 ? 128 : 256, UNITS = D / 16;
+    extern __shared__ float staged[];                  // Q4: the rotated keys, [TOKENS][heads][D]
+    __shared__ double2 turn[TOKENS][D / 2];
+    __shared__ float2 turn32[TOKENS][D / 2];
+    __shared__ PagedPlace place[TOKENS];
+    const int tid = threadIdx.x, first = blockIdx.x * TOKENS;
+    const int per_token = (r.q_heads + (Q4 ? 1 : 2) * st.heads) * UNITS, n_units = per_token * min(TOKENS, st.n_tokens - first);
+    // where a unit's 16 dimensions are: head < 0: of the queries; from st.heads on: of the values
+    auto find = [&](int u, int &tok, int &head, int &c, int &a, int &b) {
+        tok = TOKENS == 1 ? 0 : u / per_token;
+        const int w = TOKENS == 1 ? u : u - tok * per_token;
+        head = w / UNITS - r.q_heads;
+        c = w % UNITS;
+        const bool turned = 16 * c < r.rot && head < st.heads;
+        a = turned && r.halves ? c : 2 * c;
+        b = turned && r.halves ? c + r.rot / 16 : 2 * c + 1;
+        return turned;
+    };
+    IoRow8<IO> x, y;
+    auto request = [&](int u) {
+        if (u < n_units) {
+            int tok, head, c, a, b;
+            find(u, tok, head, c, a, b);
+            const int64_t t = first + tok;
+            const IO *src = head < 0            ? static_cast<const IO *>(r.q) + t * r.q_stride + (head + r.q_heads) * D
+                            : head < st.heads ? static_cast<const IO *>(r.k) + t * r.k_stride + head * D
+                                              : static_cast<const IO *>(r.v) + t * r.v_stride + (head - st.heads) * D;
+            x.load(src + 8 * a);
+            y.load(src + 8 * b);
+        }
+    };
+    request(tid);
+    if (tid < 32 * TOKENS) {
+        const PagedPlace at = paged_place(st, first + (tid >> 5));
+        if ((tid & 31) == 0) place[tid >> 5] = at;
     }
     __syncthreads();
-    const IO *k = static_cast<const IO *>(r.k) + i * r.k_stride, *v = static_cast<const IO *>(r.v) + i * r.v_stride;
-    const IO *qi = static_cast<const IO *>(r.q) + i * r.q_stride;
-    IO *qo = static_cast<IO *>(r.q_out) + i * r.q_out_stride;
-    constexpr int UNITS = D / 16;
-    const int n_units = (r.q_heads + (Q4 ? st.heads : 2 * st.heads)) * UNITS;
-    for (int u = threadIdx.x; u < n_units; u += PAGED_APPEND_THREADS) {
-        const int head = u / UNITS - r.q_heads, c = u % UNITS;             // head < 0: of the queries; from st.heads on: of the values
-        const bool turned = 16 * c < r.rot && head < st.heads;
-        const int a = turned && r.halves ? c : 2 * c, b = turned && r.halves ? c + r.rot / 16 : 2 * c + 1;
-        if (head >= 0 && page < 0 && !Q4) continue;
-        const IO *src = head < 0 ? qi + (head + r.q_heads) * D : head < st.heads ? k + head * D : v + (head - st.heads) * D;
-        float x[8], y[8];
-        io_load8(src + 8 * a, x);
-        io_load8(src + 8 * b, y);
+    for (int j = tid; j < TOKENS * (r.rot / 2); j += THREADS) {
+        const int tok = j / (r.rot / 2), i = j - tok * (r.rot / 2);
+        if (place[tok].pos >= 0) {
+            double2 t;
+            sincospi((double)place[tok].pos * r.turns[i], &t.y, &t.x);
+            const int to = (i & 7) * UNITS + (i >> 3);
+            turn[tok][to] = t;
+            turn32[tok][to] = make_float2((float)t.x, (float)t.y);
+        }
+    }
+    __syncthreads();
+    for (int u = tid; u < n_units; u += THREADS) {
+        int tok, head, c, a, b;
+        const bool turned = find(u, tok, head, c, a, b);
+        const PagedPlace at = place[tok];
+        float xf[8], yf[8];
+        x.get(xf);
+        y.get(yf);
+        request(u + THREADS);
+        if (at.pos < 0 || (head >= 0 && at.page < 0)) continue;
         if (turned) {
-            if (head < 0) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int p = j >> 1;
-                    if (r.halves) {
-                        const float cs = (float)turn[8 * c + j].x, sn = (float)turn[8 * c + j].y, t = x[j];
-                        x[j] = t * cs - y[j] * sn;
-                        y[j] = t * sn + y[j] * cs;
-                    } else if (!(j & 1)) {
-                        const float c0 = (float)turn[8 * c + p].x, s0 = (float)turn[8 * c + p].y, c1 = (float)turn[8 * c + 4 + p].x, s1 = (float)turn[8 * c + 4 + p].y;
-                        const float t = x[j], w = y[j];
-                        x[j] = t * c0 - x[j + 1] * s0;
-                        x[j + 1] = t * s0 + x[j + 1] * c0;
-                        y[j] = w * c1 - y[j + 1] * s1;
-                        y[j + 1] = w * s1 + y[j + 1] * c1;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int p = j >> 1;
-                    if (r.halves) {
-                        const double2 t = turn[8 * c + j];
-                        const double xd = x[j], yd = y[j];
-                        x[j] = (float)(xd * t.x - yd * t.y);
-                        y[j] = (float)(xd * t.y + yd * t.x);
-                    } else if (!(j & 1)) {
-                        const double2 t = turn[8 * c + p], w = turn[8 * c + 4 + p];
-                        const double x0 = x[j], x1 = x[j + 1], y0 = y[j], y1 = y[j + 1];
-                        x[j] = (float)(x0 * t.x - x1 * t.y);
-                        x[j + 1] = (float)(x0 * t.y + x1 * t.x);
-                        y[j] = (float)(y0 * w.x - y1 * w.y);
-                        y[j + 1] = (float)(y0 * w.y + y1 * w.x);
-                    }
-                }
-            }
+            if (head < 0) paged_turn<UNITS, float2, float>(xf, yf, turn32[tok], c, r.halves);
+            else paged_turn<UNITS, double2, double>(xf, yf, turn[tok], c, r.halves);
         }
         if (head < 0) {
-            io_store8(qo + (head + r.q_heads) * D + 8 * a, x);
-            io_store8(qo + (head + r.q_heads) * D + 8 * b, y);
+            IO *to = static_cast<IO *>(r.q_out) + (int64_t)(first + tok) * r.q_out_stride + (head + r.q_heads) * D;
+            io_store8(to + 8 * a, xf);
+            io_store8(to + 8 * b, yf);
         } else if constexpr (Q4) {
-            io_store8(staged + head * D + 8 * a, x);
-            io_store8(staged + head * D + 8 * b, y);
+            io_store8(staged + (tok * st.heads + head) * D + 8 * a, xf);
+            io_store8(staged + (tok * st.heads + head) * D + 8 * b, yf);
         } else {
-            CT *dst = head < st.heads ? reinterpret_cast<CT *>(r.k_pool + paged_at(st, page, head))
-                                      : reinterpret_cast<CT *>(r.v_pool + paged_at(st, page, head - st.heads));
-            io_store8(dst + row * D + 8 * a, x);
-            io_store8(dst + row * D + 8 * b, y);
+            CT *to = reinterpret_cast<CT *>(head < st.heads ? r.k_pool + paged_at(st, at.page, head) : r.v_pool + paged_at(st, at.page, head - st.heads)) + at.row * D;
+            io_store8(to + 8 * a, xf);
+            io_store8(to + 8 * b, yf);
         }
     }
     if constexpr (Q4) {
         __syncthreads();
-        if (page < 0) return;
         // four neighbouring lanes per block of 32 dims; the bound is a multiple of four, so they stay together
-        for (int u = threadIdx.x; u < 2 * st.heads * (D / 8); u += PAGED_APPEND_THREADS) {
-            const int head = u / (D / 8), c = u % (D / 8);
-            float x[8];
-            if (head < st.heads) io_load8(staged + head * D + 8 * c, x);
-            else io_load8(v + (head - st.heads) * D + 8 * c, x);
-            uint8_t *dst = head < st.heads ? r.k_pool + paged_at(st, page, head) : r.v_pool + paged_at(st, page, head - st.heads);
-            q4_store<D>(dst, st.page_shift, row, c >> 2, c & 3, x);
+        const int per = 2 * st.heads * (D / 8);
+        for (int u = tid; u < per * min(TOKENS, st.n_tokens - first); u += THREADS) {
+            const int tok = TOKENS == 1 ? 0 : u / per, w = u - tok * per, head = w / (D / 8), c = w % (D / 8);
+            const PagedPlace at = place[tok];
+            if (at.page < 0) continue;               // (the same for the four)
+            float z[8];
+            if (head < st.heads) io_load8(staged + (tok * st.heads + head) * D + 8 * c, z);
+            else io_load8(static_cast<const IO *>(r.v) + (int64_t)(first + tok) * r.v_stride + (head - st.heads) * D + 8 * c, z);
+            uint8_t *to = head < st.heads ? r.k_pool + paged_at(st, at.page, head) : r.v_pool + paged_at(st, at.page, head - st.heads);
+            q4_store<D>(to, st.page_shift, at.row, c >> 2, c & 3, z);
         }
     }
 }
 
 // ---- gather ---------------------------------------------------------------------------------------------------------------
-template <class CT, int D, class IO>
-__global__ void __launch_bounds__(128) skn_paged_gather_kernel(const PagedStep st, const uint8_t *k_pool, const uint8_t *v_pool, IO *k_out, IO *v_out) {
-    const int i = blockIdx.x;
-    const int s = paged_find(st, i);
-    if (s < 0) return;
-    const PagedSeq q = paged_seq(st, s);
-    const int pos = q.len - q.n + i - q.first;
-    if (i >= q.first + q.n || pos < 0) return;
-    const int page = paged_page(st, s, pos), row = pos & ((1 << st.page_shift) - 1);
-    if (page < 0) return;
-    for (int u = threadIdx.x; u < 2 * st.heads * (D / 8); u += 128) {
-        int head = u / (D / 8);
-        const int c = u % (D / 8);
+template <class CT, int D, class IO, int TOKENS>
+__global__ void __launch_bounds__(256) skn_paged_gather_kernel(const PagedStep st, const uint8_t *k_pool, const uint8_t *v_pool, IO *k_out, IO *v_out) {
+    __shared__ PagedPlace place[TOKENS];
+    const int tid = threadIdx.x, first = blockIdx.x * TOKENS;
+    if (tid < 32 * TOKENS) {
+        const PagedPlace at = paged_place(st, first + (tid >> 5));
+        if ((tid & 31) == 0) place[tid >> 5] = at;
+    }
+    __syncthreads();
+    const int per = 2 * st.heads * (D / 8);
+    for (int u = tid; u < per * TOKENS; u += 256) {
+        const int tok = u / per, w = u - tok * per, head = w / (D / 8), c = w % (D / 8);
+        const PagedPlace at = place[tok];
+        if (at.page < 0) continue;
         const bool is_v = head >= st.heads;
-        head -= is_v ? st.heads : 0;
+        const int h = is_v ? head - st.heads : head;
         float x[8];
-        paged_load8<D>(reinterpret_cast<const CT *>((is_v ? v_pool : k_pool) + paged_at(st, page, head)), st.page_shift, row, c, x);
-        io_store8((is_v ? v_out : k_out) + ((int64_t)i * st.heads + head) * D + 8 * c, x);
+        paged_load8<D>(reinterpret_cast<const CT *>((is_v ? v_pool : k_pool) + paged_at(st, at.page, h)), st.page_shift, at.row, c, x);
+        io_store8((is_v ? v_out : k_out) + ((int64_t)(first + tok) * st.heads + h) * D + 8 * c, x);
     }
 }
 
@@ -188,7 +251,7 @@ static int32_t check_spec(skn_ctx *ctx, const skn_paged_spec *s) {
     if (!s) return skn_fail(ctx, SKN_ERR_ARG, "NULL specification");
     if (s->kv_dtype != SKN_KV_F16 && s->kv_dtype != SKN_KV_BF16 && s->kv_dtype != SKN_KV_Q4_0)
         return skn_fail(ctx, SKN_ERR_TYPE, "a paged cache holds fp16, bf16 or Q4_0, not element type %d", s->kv_dtype);
-    if (s->n_kv_heads < 1 || s->n_kv_heads > 1024 || s->n_pages < 1) return skn_fail(ctx, SKN_ERR_ARG, "pages and heads (at most 1024) must be positive");
+    if (s->n_kv_heads < 1 || s->n_kv_heads > 256 || s->n_pages < 1) return skn_fail(ctx, SKN_ERR_ARG, "pages and heads (at most 256) must be positive");
     if (s->head_dim != 64 && s->head_dim != 128) return skn_fail(ctx, SKN_ERR_SHAPE, "head_dim must be 64 or 128 (got %d)", s->head_dim);
     if (s->page_tokens != 16 && s->page_tokens != 32 && s->page_tokens != 64 && s->page_tokens != 128)
         return skn_fail(ctx, SKN_ERR_SHAPE, "a page holds 16, 32, 64 or 128 tokens, not %d", s->page_tokens);
@@ -231,18 +294,25 @@ static int32_t check_io(skn_ctx *ctx, int32_t io) {
     return SKN_OK;
 }
 
-template <class CT, int D, class IO> static cudaError_t append_launch(const PagedStep &st, const PagedRows &r, cudaStream_t stream) {
-    const size_t smem = sizeof(CT) == 1 ? (size_t)st.heads * D * sizeof(float) : 0;
-    auto *kern = skn_paged_append_kernel<CT, D, IO>;
-    if (smem > 40000) {
+template <class CT, int D, class IO, int TOKENS> static cudaError_t append_with(const PagedStep &st, const PagedRows &r, cudaStream_t stream) {
+    const size_t smem = sizeof(CT) == 1 ? (size_t)TOKENS * st.heads * D * sizeof(float) : 0;
+    auto *kern = skn_paged_append_kernel<CT, D, IO, TOKENS>;
+    if (smem > 32000) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    kern<<<st.n_tokens, PAGED_APPEND_THREADS, smem, stream>>>(st, r);
+    kern<<<(st.n_tokens + TOKENS - 1) / TOKENS, TOKENS == 1 ? 128 : 256, smem, stream>>>(st, r);
     return cudaGetLastError();
 }
+template <class CT, int D, class IO> static cudaError_t append_launch(const PagedStep &st, const PagedRows &r, cudaStream_t stream) {
+    // (four tokens' staged keys of 4 bits have to fit shared memory: up to 96 kv heads of 128)
+    return st.n_tokens >= PAGED_LONG_STEP && (sizeof(CT) > 1 || st.heads * D <= 96 * 128) ? append_with<CT, D, IO, 4>(st, r, stream) : append_with<CT, D, IO, 1>(st, r, stream);
+}
 template <class CT, int D, class IO> static cudaError_t gather_launch(const PagedStep &st, const skn_paged *pc, void *k, void *v, cudaStream_t stream) {
-    skn_paged_gather_kernel<CT, D, IO><<<st.n_tokens, 128, 0, stream>>>(st, pc->k, pc->v, static_cast<IO *>(k), static_cast<IO *>(v));
+    if (st.n_tokens >= PAGED_LONG_STEP)
+        skn_paged_gather_kernel<CT, D, IO, 4><<<(st.n_tokens + 3) / 4, 256, 0, stream>>>(st, pc->k, pc->v, static_cast<IO *>(k), static_cast<IO *>(v));
+    else
+        skn_paged_gather_kernel<CT, D, IO, 1><<<st.n_tokens, 256, 0, stream>>>(st, pc->k, pc->v, static_cast<IO *>(k), static_cast<IO *>(v));
     return cudaGetLastError();
 }
 #define PAGED_BY_IO(fn, CT, D, ...) (io == SKN_KV_F32 ? fn<CT, D, float>(__VA_ARGS__) : fn<CT, D, __nv_bfloat16>(__VA_ARGS__))

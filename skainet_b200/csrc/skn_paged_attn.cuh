@@ -9,6 +9,8 @@
 // x 8 rows): keys are the operand of 16 so that up to eight query heads waste nothing.  Scores go through one running maximum per row that
 // moves only when a weight would exceed 2^SLACK (one vote a unit instead of six shuffles).  Weights are transposed by movmatrix into the second
 // operand of O^T = V^T p^T.  fp32 rows: queries and weights as sums of two fp16 (fp16 and Q4_0 caches) or three bf16 terms.
+// The tensor cores cut their sums off instead of rounding them, so for these rows the small terms have an accumulator of their own, the large ones
+// two for the scores, and a unit's output is formed from zero and added in fp32.
 //
 // Q4_0.  K: a nibble masked out of a word is an fp16 subnormal, q 2^-24 (or 16 q 2^-24), which the tensor cores multiply exactly, so quants need
 // no conversion; one accumulator per block of 32 dims starts at -8 sum q and is scaled by the key's d.  V: weights are multiplied by the
@@ -46,9 +48,26 @@ __device__ __forceinline__ float pa_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// a b from zero
+template <class CT> __device__ __forceinline__ void mma_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<CT, __nv_bfloat16>::value) mma_bf16_first(d, a, b0, b1);
+    else mma_f16_from(d, a, b0, b1, 0.f, 0.f);
+}
 template <class CT> __device__ __forceinline__ void mma_as(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<CT, __nv_bfloat16>::value) mma_bf16(c, a, b0, b1);
     else mma_f16(c, a, b0, b1);
+}
+// o += a b, b in NT terms; fp32 rows: from zero, small terms first, and then added
+template <class CT, bool EX, int NT> __device__ __forceinline__ void pa_add(float (&o)[4], const uint32_t (&a)[4], const uint32_t (&b)[NT][2]) {
+    if constexpr (EX) {
+        float x[4];
+        mma_zero<CT>(x, a, b[NT - 1][0], b[NT - 1][1]);
+#pragma unroll
+        for (int n = NT - 2; n >= 0; --n) mma_as<CT>(x, a, b[n][0], b[n][1]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] += x[c];
+    } else
+        mma_as<CT>(o, a, b[0][0], b[0][1]);
 }
 __device__ __forceinline__ uint32_t movm(uint32_t x) {
     uint32_t y;
@@ -463,7 +482,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 if constexpr (T::Q4) {
                     const float sum = (x[nb][k][0] + x[nb][k][1]) + (x[nb][k][2] + x[nb][k][3]);
                     if (k & 1) bs[k >> 1] += sum; else bs[k >> 1] = sum;
-                    if (k & 1) {                    // the upper nibble stands 16 times higher
+                    if (!EX && (k & 1)) {           // the upper nibble stands 16 times higher
 #pragma unroll
                         for (int i = 0; i < 4; ++i) x[nb][k][i] *= 0.0625f;
                     }
@@ -482,7 +501,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 }
             }
             f *= p.scale;
-            if constexpr (T::Q4) f *= 16777216.f;
+            if constexpr (T::Q4 && !EX) f *= 16777216.f;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int src = 4 * (2 * t4 + c);
@@ -503,7 +522,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         if constexpr (T::Q_SMEM) __syncthreads();
 
         // ---- the units ------------------------------------------------------------------------------------------------------
-        float o[D / 16][NB][4], m[NB][2], mlim[NB][2], l[NB][2];
+        float o[D / 16][NB][4], m[NB][2], most[NB][2], l[NB][2];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -514,10 +533,11 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                m[nb][c] = mlim[nb][c] = PA_NONE;
+                m[nb][c] = 0.f;
+                most[nb][c] = -INFINITY;
                 l[nb][c] = 0.f;
             }
-        int lift = T::Q4 ? 0 : T::LIFT;            // m: the maximum less this; mlim: the maximum and SLACK
+        int lift = T::Q4 ? 0 : T::LIFT;            // m: the maximum less this; most: exponent of the largest weight before it moves
         __half2 vlim = __floats2half2_rn(0.f, 0.f); // Q4_0: the largest |d| that the lift takes
         for (int j = 0; j < n_mine && !dead; ++j) {
             const int kbase = key_of(j);
@@ -611,11 +631,22 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                     for (int b = 0; b < NBLK; ++b) {
                         const uint32_t w0 = *reinterpret_cast<const uint32_t *>(kq + b * 256 + g8 * 16 + t4 * 4);
                         const uint32_t w1 = *reinterpret_cast<const uint32_t *>(kq + b * 256 + (g8 + 8) * 16 + t4 * 4);
-                        const uint32_t lo[4] = {w0 & 0x000F000Fu, w1 & 0x000F000Fu, (w0 >> 8) & 0x000F000Fu, (w1 >> 8) & 0x000F000Fu};
-                        const uint32_t hi[4] = {w0 & 0x00F000F0u, w1 & 0x00F000F0u, (w0 >> 8) & 0x00F000F0u, (w1 >> 8) & 0x00F000F0u};
+                        uint32_t lo[4] = {w0 & 0x000F000Fu, w1 & 0x000F000Fu, (w0 >> 8) & 0x000F000Fu, (w1 >> 8) & 0x000F000Fu};
+                        uint32_t hi[4] = {w0 & 0x00F000F0u, w1 & 0x00F000F0u, (w0 >> 8) & 0x00F000F0u, (w1 >> 8) & 0x00F000F0u};
+                        if constexpr (EX) {        // q - 8 itself: no large sums that cancel
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                lo[i] |= 0x64006400u;
+                                hi[i] |= 0x64006400u;
+                                const __half2 x = __hadd2(*reinterpret_cast<const __half2 *>(&lo[i]), __float2half2_rn(-1032.f));
+                                const __half2 y = __hfma2(*reinterpret_cast<const __half2 *>(&hi[i]), __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+                                lo[i] = *reinterpret_cast<const uint32_t *>(&x);
+                                hi[i] = *reinterpret_cast<const uint32_t *>(&y);
+                            }
+                        }
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            float acc[4];
+                            float acc[4], small[4];
 #pragma unroll
                             for (int n = NT - 1; n >= 0; --n) {
                                 uint2 f0, f1;
@@ -626,9 +657,17 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                                     f0 = make_uint2(qr[n][nb][2 * b][0], qr[n][nb][2 * b][1]);
                                     f1 = make_uint2(qr[n][nb][2 * b + 1][0], qr[n][nb][2 * b + 1][1]);
                                 }
-                                if (n == NT - 1) mma_f16_from(acc, lo, f0.x, f0.y, bias[nb][b][0], bias[nb][b][1]);
-                                else mma_f16(acc, lo, f0.x, f0.y);
-                                mma_f16(acc, hi, f1.x, f1.y);
+                                if constexpr (EX) {
+                                    mma_f16_from(n ? small : acc, lo, f0.x, f0.y, 0.f, 0.f);
+                                    mma_f16(n ? small : acc, hi, f1.x, f1.y);
+                                } else {
+                                    mma_f16_from(acc, lo, f0.x, f0.y, bias[nb][b][0], bias[nb][b][1]);
+                                    mma_f16(acc, hi, f1.x, f1.y);
+                                }
+                            }
+                            if constexpr (EX) {
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) acc[c] += small[c];
                             }
                             s[nb][0] = fmaf(acc[0], dk[0][b], s[nb][0]);
                             s[nb][1] = fmaf(acc[1], dk[0][b], s[nb][1]);
@@ -637,12 +676,9 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                         }
                     }
                 } else {
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) s[nb][c] = 0.f;
                     const int row = (lane & 7) + (lane & 8);
                     const uint32_t base = skn_smem_u32(kt) + row * 128;
+                    float odd[EX ? NB : 1][4], small[EX ? NB : 1][4];
 #pragma unroll
                     for (int k = 0; k < KS; ++k) {
                         const int c = 2 * k + (lane >> 4);
@@ -655,8 +691,19 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                                 uint2 f;
                                 if constexpr (T::Q_SMEM) f = qf[((n * NB + nb) * KS + k) * 32 + lane];
                                 else f = make_uint2(qr[n][nb][k][0], qr[n][nb][k][1]);
-                                mma_as<CT>(s[nb], a, f.x, f.y);
+                                if constexpr (EX) {
+                                    float (&to)[4] = n ? small[nb] : k & 1 ? odd[nb] : s[nb];
+                                    if (n ? k == 0 && n == NT - 1 : k < 2) mma_zero<CT>(to, a, f.x, f.y);
+                                    else mma_as<CT>(to, a, f.x, f.y);
+                                } else if (k == 0) mma_zero<CT>(s[nb], a, f.x, f.y);
+                                else mma_as<CT>(s[nb], a, f.x, f.y);
                             }
+                    }
+                    if constexpr (EX) {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) s[nb][c] = (s[nb][c] + odd[nb][c]) + small[nb][c];
                     }
                 }
                 // ---- weights -----------------------------------------------------------------------------------------------
@@ -665,9 +712,9 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        s[nb][c] *= cs[nb][c & 1];
+                        s[nb][c] = fmaf(s[nb][c], cs[nb][c & 1], -m[nb][c & 1]);
                         if (!whole && (hidden_page || !paged_sees(p, key0 + g8 + 8 * (c >> 1), pos[nb][c & 1]))) s[nb][c] = -INFINITY;
-                        move |= s[nb][c] > mlim[nb][c & 1];
+                        move |= s[nb][c] > most[nb][c & 1];
                     }
                 if constexpr (T::Q4) move |= !__hble2(dtop, vlim);
                 if (__any_sync(0xffffffffu, move)) {
@@ -679,10 +726,13 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                            top = fmaxf(top, mlim[nb][c] - (float)T::SLACK) - (float)lift;
-                            const float fix = pa_ex2(m[nb][c] - top);
-                            m[nb][c] = top;
-                            mlim[nb][c] = top + (float)(lift + T::SLACK);
+                            // the row's maximum, `lift` above m, moves by so much (the first one either way)
+                            const bool begun = most[nb][c] > -INFINITY;
+                            const float by = begun ? fmaxf(top - (float)lift, 0.f) : top > -INFINITY ? top - (float)lift : 0.f, fix = begun ? pa_ex2(-by) : 1.f;
+                            if (top > -INFINITY) most[nb][c] = (float)(lift + T::SLACK);
+                            s[nb][c] -= by;
+                            s[nb][c + 2] -= by;
+                            m[nb][c] += by;
                             l[nb][c] *= fix;
 #pragma unroll
                             for (int i = 0; i < D / 16; ++i) {
@@ -718,6 +768,9 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                                 for (int c = 0; c < 2; ++c) {
                                     m[nb][c] -= (float)by;
                                     l[nb][c] *= fix;
+                                    s[nb][c] += (float)by;
+                                    s[nb][c + 2] += (float)by;
+                                    most[nb][c] += (float)by;            // (minus infinity stays)
                                 }
 #pragma unroll
                                 for (int i = 0; i < D / 16; ++i)
@@ -731,7 +784,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        s[nb][c] = pa_ex2(s[nb][c] - m[nb][c & 1]);
+                        s[nb][c] = pa_ex2(s[nb][c]);
                         l[nb][c & 1] += s[nb][c];
                     }
                 // ---- values ------------------------------------------------------------------------------------------------
@@ -766,12 +819,10 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                         const uint32_t a0[4] = {less8(lo), less8(lo >> 8), less8(lo2), less8(lo2 >> 8)};
                         const uint32_t a1[4] = {less8(hi), less8(hi >> 8), less8(hi2), less8(hi2 >> 8)};
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                            for (int n = NT - 1; n >= 0; --n) {
-                                mma_f16(o[2 * b][nb], a0, pb[nb][n][0], pb[nb][n][1]);
-                                mma_f16(o[2 * b + 1][nb], a1, pb[nb][n][0], pb[nb][n][1]);
-                            }
+                        for (int nb = 0; nb < NB; ++nb) {
+                            pa_add<CT, EX, NT>(o[2 * b][nb], a0, pb[nb]);
+                            pa_add<CT, EX, NT>(o[2 * b + 1][nb], a1, pb[nb]);
+                        }
                     }
                 } else {
                     uint32_t pb[NB][NT][2];
@@ -794,9 +845,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                         uint32_t a[4];
                         ldsm4t(a, base + (c >> 3) * 2048 + (((c & 7) ^ (row & 7)) << 4));
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                            for (int n = NT - 1; n >= 0; --n) mma_as<CT>(o[i][nb], a, pb[nb][n][0], pb[nb][n][1]);
+                        for (int nb = 0; nb < NB; ++nb) pa_add<CT, EX, NT>(o[i][nb], a, pb[nb]);
                     }
                 }
             }

@@ -55,7 +55,7 @@ def test_rotation_turns_by_the_difference_of_positions():
     ({"dtype": 0}, "not element type 0"), ({"dtype": 2}, "not element type 2"), ({"dim": 96}, "head_dim"), ({"page": 24}, "a page holds"),
     ({"page": 256}, "a page holds"), ({"rot": 8}, "multiple of 16"), ({"rot": 144}, "multiple of 16"), ({"rot": -16}, "multiple of 16"),
     ({"pairs": 2}, "pairing"), ({"base": 0.0}, "rot_base"), ({"base": float("nan")}, "rot_base"), ({"pages": 0}, "positive"), ({"heads": 0}, "positive"),
-    ({"heads": 1025}, "positive")])
+    ({"heads": 257}, "positive")])
 def test_specifications_are_refused(over, message):
     s = {"heads": 2, "dim": 64, "page": 16, "dtype": 1, "pages": 4, "rot": 64, "pairs": 0, "base": 10000.0} | over
     spec = _ffi.PagedSpec(s["heads"], s["dim"], s["page"], s["dtype"], s["pages"], s["rot"], s["pairs"], 0, s["base"])

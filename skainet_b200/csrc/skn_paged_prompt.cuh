@@ -95,28 +95,12 @@ __device__ __forceinline__ float pp_max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// 2^x of two values: on the special-function units, which at 16 a clock and SM would take as long as the products, and with FMAs.
-// The latter: x = n + f with f in -1/2 .. 1/2 (n from the sum with 1.5 2^23), a cubic of least relative error 7.5e-5 there (fp16 weights
-// are off by 2.4e-4, bf16 by more), n added to the exponent.  What lies below -126, hidden scores among it, ends at one value, which is taken off: zero.
-__device__ __forceinline__ uint64_t pp_ex2_unit(uint64_t x) {
+// 2^x of two values, on the special-function units.  (16 a clock and SM take as long as the products do; but the warps are short of issue slots first:
+// three in eight by FMAs instead, a cubic in the fraction, 548 -> 606 us for a prompt of 8192 tokens.)
+__device__ __forceinline__ uint64_t pp_ex2_pair(uint64_t x) {
     float a, b;
     skn_unpack2(x, a, b);
     return skn_pack2(pp_ex2(a), pp_ex2(b));
-}
-__device__ __forceinline__ uint64_t pp_ex2_fma(uint64_t x) {
-    float a, b;
-    skn_unpack2(x, a, b);
-    x = skn_pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-    const uint64_t big = skn_pack2(12582912.f, 12582912.f), n = skn_add2(x, big);
-    const uint64_t f = skn_fma2(skn_add2(n, skn_pack2(-12582912.f, -12582912.f)), skn_pack2(-1.f, -1.f), x);
-    uint64_t y = skn_fma2(f, skn_pack2(0.05517166905792616f, 0.05517166905792616f), skn_pack2(0.2426111221932161f, 0.2426111221932161f));
-    y = skn_fma2(y, f, skn_pack2(0.6932609854606553f, 0.6932609854606553f));
-    y = skn_fma2(y, f, skn_pack2(0.9999280735394012f, 0.9999280735394012f));
-    float ya, yb, na, nb;
-    skn_unpack2(y, ya, yb);
-    skn_unpack2(n, na, nb);
-    const float least = __uint_as_float(__float_as_uint(0.9999280735394012f) - (126u << 23));        // of x = -126: n = -126, f = 0
-    return skn_add2(skn_pack2u(__float_as_uint(ya) + (__float_as_uint(na) << 23), __float_as_uint(yb) + (__float_as_uint(nb) << 23)), skn_pack2(-least, -least));
 }
 
 // A CTA's share of the line, segment by segment; every role walks it for itself
@@ -403,15 +387,15 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         }
                     }
                     const uint64_t cs2 = skn_pack2(cs, cs), off2 = skn_pack2(T::LIFT - m, T::LIFT - m);
-                    uint64_t sum = 0;
+                    uint64_t sum = 0, sum2 = 0;      // (two chains of 32 additions; one of 64: 533 -> 547 us for a prompt of 8192 tokens)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t pk[32];
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
                             const uint64_t x = skn_fma2(skn_pack2(v[64 * h + 2 * c], v[64 * h + 2 * c + 1]), cs2, off2);
-                            const uint64_t y = c % 8 < 5 ? pp_ex2_unit(x) : pp_ex2_fma(x);
-                            sum = skn_add2(sum, y);
+                            const uint64_t y = pp_ex2_pair(x);
+                            (c & 1 ? sum : sum2) = skn_add2(c & 1 ? sum : sum2, y);
                             float a, b;
                             skn_unpack2(y, a, b);
                             pk[c] = T::BF ? pack_bf16(a, b) : pack_f16(a, b);
@@ -423,7 +407,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         if (lane == 0) skn_mbar_arrive(&p_full[2 * tile + h]);
                     }
                     float a, b;
-                    skn_unpack2(sum, a, b);
+                    skn_unpack2(skn_add2(sum, sum2), a, b);
                     l += a + b;
                 }
             }

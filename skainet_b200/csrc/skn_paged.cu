@@ -13,17 +13,18 @@
 // the sines 96 us, four and ahead of them in the tables below.
 constexpr int PAGED_LONG_STEP = 2048;        // tokens from which a CTA takes four: with fewer the GPU is not full of CTAs of one
 
-// sequence of row i: the last one that starts at or before it (-1: none).  Every warp counts the starts for itself, 32 at a time.
+// sequence of row i: the last one that starts at or before it (-1: none).  Every warp counts the starts for itself: 32 of them at even distances, then
+// those between two of these.  (One after the other, 32 at a time, they are a chain of loads as long as the batch.)
 __device__ __forceinline__ int paged_find(const PagedStep &st, int i) {
     const int lane = threadIdx.x & 31;
-    int n = 0;
-    for (int b = 0; b <= st.n_seqs; b += 32) {
-        const bool at = b + lane <= st.n_seqs && st.starts[b + lane] <= i;
-        const unsigned m = __ballot_sync(0xffffffffu, at);
-        n += __popc(m);
-        if (m != 0xffffffffu) break;
+    int lo = 0, hi = st.n_seqs + 1;                     // starts before lo are at or before i, from hi on they are not
+    while (lo < hi) {
+        const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step - 1;
+        const int n = __popc(__ballot_sync(0xffffffffu, at < hi && st.starts[at] <= i));
+        hi = min(hi, lo + (n + 1) * step - 1);
+        lo = min(hi, lo + n * step);
     }
-    return n - 1 < st.n_seqs ? n - 1 : -1;
+    return lo - 1 < st.n_seqs ? lo - 1 : -1;
 }
 
 // q of one value: x * fp32(1 / d) + 8.5 in 64 bits, cut off.  The sum with one rounding in fp32 is off by 2^-21 at most, so that 64 bits are
@@ -75,7 +76,7 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedStep &st, int i) {
     const int s = i < st.n_tokens ? paged_find(st, i) : -1;
     if (s < 0) return at;
     const PagedSeq q = paged_seq(st, s);
-    if (i >= q.first + q.n) return at;
+    if (i < q.first || i >= q.first + q.n) return at;
     at.pos = q.len - q.n + i - q.first;
     if (at.pos >= 0) {
         at.page = paged_page(st, s, at.pos);
@@ -274,6 +275,7 @@ static int32_t check_batch(skn_ctx *ctx, const skn_paged_batch *b, bool *nothing
     if (*nothing) return SKN_OK;
     if (b->n_tokens > (1 << 24)) return skn_fail(ctx, SKN_ERR_SHAPE, "%d rows in a step; 2^24 at most", b->n_tokens);
     if (b->n_seqs > 65535) return skn_fail(ctx, SKN_ERR_SHAPE, "%d sequences in a step; 65535 at most", b->n_seqs);
+    if (b->max_pages > (1 << 23)) return skn_fail(ctx, SKN_ERR_SHAPE, "%d pages a sequence; 2^23 at most", b->max_pages);
     if (!b->token_start || !b->lengths || (!b->page_table && b->max_pages)) return skn_fail(ctx, SKN_ERR_ARG, "NULL array in the batch");
     return SKN_OK;
 }
@@ -477,6 +479,7 @@ int32_t skn_paged_destroy(skn_paged *pc) {
     if (pc->d_turns) cudaFree(pc->d_turns);
     if (pc->d_parts) cudaFree(pc->d_parts);
     if (pc->d_tickets) cudaFree(pc->d_tickets);
+    if (pc->d_again) cudaFree(pc->d_again);
     pc->magic = 0;
     delete pc;
     return SKN_OK;
@@ -580,6 +583,13 @@ int32_t skn_paged_attn_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t 
     if (nothing) return SKN_OK;
     const int64_t wq = (int64_t)n_q_heads * pc->spec.head_dim;
     if ((rc = check_rows(ctx, "q", q_dev, q_stride, wq, io)) || (rc = check_rows(ctx, "out", out_dev, out_stride, wq, io))) return rc;
+    // outputs are written while other rows' queries are still to be read, and a query is asked for again where a result is not finite
+    const int64_t size = io == SKN_KV_F32 ? 4 : 2, n = batch->n_tokens - 1;
+    const uintptr_t qa = (uintptr_t)q_dev, oa = (uintptr_t)out_dev, q_end = qa + (n * q_stride + wq) * size, o_end = oa + (n * out_stride + wq) * size;
+    if (qa < o_end && oa < q_end) {
+        const int64_t apart = q_stride == out_stride ? (int64_t)((qa > oa ? qa - oa : oa - qa) % (uintptr_t)(q_stride * size)) : 0;
+        if (q_stride != out_stride || apart < wq * size || apart > (q_stride - wq) * size) return skn_fail(ctx, SKN_ERR_ARG, "out lies over q");
+    }
     SKN_CUDA(ctx, cudaSetDevice(ctx->device));
     return skn_paged_attn_launch(pc, batch, io, q_dev, q_stride, n_q_heads, scale, window, window ? sinks : 0, out_dev, out_stride);
 }

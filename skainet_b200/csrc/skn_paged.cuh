@@ -22,9 +22,11 @@ struct skn_paged {
     // Attention's workspace (skn_paged_attn.cu): tensor maps of the pools and, for rows whose keys several CTAs share, their partial results
     CUtensorMap map[4];          // K, V; of Q4_0 their quants, then their scales
     CUtensorMap wide[4];         // the same in larger boxes (prompts): whole pages of half rows; of Q4_0 up to 32 rows
-    int n_parts;                 // CTAs that share a launch's work
-    float *d_parts;              // decoding: [2 n_parts][SKN_PAGED_PART_ROWS][head_dim + 4]: output, maximum, sum; prompts: rows of two CTAs' blocks per SM
-    unsigned *d_tickets;         // [2 n_parts], zero between launches
+    int n_parts;                 // CTAs that share a launch's work, at most
+    float *d_parts;              // prompts: blocks of rows of two segments per SM; then (from prompt_parts on) decoding: [2 n_parts][SKN_PAGED_PART_ROWS][head_dim + 4]:
+    int64_t prompt_parts;        // output, maximum, sum
+    unsigned *d_tickets;         // [2][2 n_parts], zero between launches
+    uint8_t *d_again;            // prompts: a PagedScratch per SM
 };
 constexpr int SKN_PAGED_PART_ROWS = 32;
 
@@ -113,6 +115,16 @@ template <int D> __device__ __forceinline__ void paged_load8(const skn_q4 *at, i
     const int sh = (c & 2) << 1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = (float)((int)((((i < 4 ? u.x : u.y) >> (8 * (i & 3) + sh)) & 15u)) - 8) * d;
+}
+// one dimension
+template <int D, class CT> __device__ __forceinline__ float paged_load1(const CT *at, int page_shift, int r, int d) {
+    if constexpr (std::is_same<CT, __nv_bfloat16>::value) return __bfloat162float(at[r * D + d]);
+    else if constexpr (std::is_same<CT, __half>::value) return __half2float(at[r * D + d]);
+    else {
+        const uint8_t *p = reinterpret_cast<const uint8_t *>(at);
+        const int q = p[((((d >> 5) << page_shift) + r) << 4) + (d & 15)] >> (d & 16 ? 4 : 0) & 15;
+        return (float)(q - 8) * __half2float(*reinterpret_cast<const __half *>(p + ((D / 2) << page_shift) + (r * (D / 32) + (d >> 5)) * 2));
+    }
 }
 #endif
 

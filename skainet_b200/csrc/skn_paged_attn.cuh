@@ -110,6 +110,9 @@ struct PagedAttn {
     int group, window, sinks;
     float scale;                  // times log2(e)
     int direct;                   // a CTA per segment: no sharing (rows in blocks of 8 NB)
+    int above, upto;              // sequences of other numbers of rows (tokens x group) are left to another launch
+    int split;                    // ... which follows this one, or is this one: it begins while that one ends
+    void *scratch;                // prompts: a PagedScratch for each CTA
     float *parts;
     unsigned *tickets;
 };
@@ -132,6 +135,14 @@ __device__ __forceinline__ bool paged_sees(const PagedAttn &p, int key, int pos)
     return key <= pos && (!p.window || key > pos - p.window || key < p.sinks);
 }
 
+// A sequence's rows for this launch
+__device__ __forceinline__ PagedSeq paged_mine(const PagedAttn &p, int s) {
+    PagedSeq q = paged_seq(p.st, s);
+    const int rows = q.n * p.group;                  // (at most 2^30)
+    if (rows <= p.above || rows > p.upto) q.n = 0;
+    return q;
+}
+
 struct PagedSegment {
     int seq, head, first, rows, row0;     // its rows of the step: token first + r / group, query head head * group + r % group, r = row0 ..
     int n, len;                           // of the sequence
@@ -143,80 +154,120 @@ struct PagedSegment {
 // Where a CTA leaves its part of a segment that others share: a CTA ends in at most one such segment and begins in at most one
 __device__ __forceinline__ int paged_slot(const PagedSegment &g, int cta) { return 2 * cta + (cta == g.c0); }
 
-// A segment from the definition: for rows in turn, a thread per key and then a thread per dimension (PA_THREADS of them, which `bar` brings together).
-// put(row, maximum (base 2), sum, this thread's dimension of the unnormalised output)
+// A segment from the definition, eight rows at a time: a thread per key for the scores, then a thread per dimension (and part of the keys) for the outputs
+// (PA_THREADS of them, which `bar` brings together).  put(row, maximum (base 2), sum, this thread's dimension of the unnormalised output).
+// Eight rows share every load: a block of 256 rows that other roles of its CTA wait for is through its keys at some 15 us per thousand.
+constexpr int PA_REDO = 8;
+template <int D> struct PagedScratch {
+    float q[D][PA_REDO], w[PA_THREADS][PA_REDO], red[PA_WARPS][PA_REDO];
+    int page[PA_THREADS];
+    uint8_t seen[PA_THREADS];                            // a bit per row
+};
 template <class CT, int D, class IO, class Bar, class Put>
-__device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &g, int unit, float *scratch, Bar bar, Put put) {
-    float *qs = scratch, *ps = scratch + D, *red = ps + PA_THREADS;
-    const int tid = threadIdx.x;
-    for (int r = 0; r < g.rows; ++r) {
-        const int t = (g.row0 + r) / p.group, pos = g.len - g.n + t;
-        const IO *q = static_cast<const IO *>(p.q) + (int64_t)(g.first + t) * p.q_stride + (g.head * p.group + (g.row0 + r) % p.group) * D;
+__device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &g, int unit, PagedScratch<D> &sc, Bar bar, Put put) {
+    const int tid = threadIdx.x, dim = tid % D;
+    for (int r0 = 0; r0 < g.rows; r0 += PA_REDO) {
         bar();
-        if (tid < D / 8) {
-            float x[8];
-            io_load8(q + 8 * tid, x);
+        for (int i = tid; i < PA_REDO * (D / 8); i += PA_THREADS) {
+            const int k = i / (D / 8), c = i % (D / 8), R = g.row0 + r0 + k;
+            float x[8] = {};
+            if (r0 + k < g.rows) io_load8(static_cast<const IO *>(p.q) + (int64_t)(g.first + R / p.group) * p.q_stride + (g.head * p.group + R % p.group) * D + 8 * c, x);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) qs[8 * tid + i] = x[i];
+            for (int e = 0; e < 8; ++e) sc.q[8 * c + e][k] = x[e];
         }
         bar();
-        float m = PA_NONE, l = 0.f, acc = 0.f;
+        float m[PA_REDO], l[PA_REDO], acc[PA_REDO];
+#pragma unroll
+        for (int k = 0; k < PA_REDO; ++k) {
+            m[k] = PA_NONE;
+            l[k] = acc[k] = 0.f;
+        }
         for (int b = g.u0 * unit; b < g.u1 * unit; b += PA_THREADS) {
             auto key_of = [&](int i) { const int u = i / unit; return (u < g.span.a ? u : u + g.span.gap) * unit + i % unit; };
-            const int i = b + tid, key = key_of(i);
-            float z = -INFINITY;
-            bool seen = i < g.u1 * unit && paged_sees(p, key, pos);
+            const int key = key_of(b + tid);
+            uint32_t seen = 0;
+            if (b + tid < g.u1 * unit)
+#pragma unroll
+                for (int k = 0; k < PA_REDO; ++k)
+                    seen |= (uint32_t)(r0 + k < g.rows && paged_sees(p, key, g.len - g.n + (g.row0 + r0 + k) / p.group)) << k;
+            float z[PA_REDO] = {};
             if (seen) {
                 const int page = paged_page(p.st, g.seq, key), row = key & ((1 << p.st.page_shift) - 1);
-                seen = page >= 0;
-                if (seen) {
+                if (page >= 0) {
                     const CT *at = reinterpret_cast<const CT *>(p.k_pool + paged_at(p.st, page, g.head));
-                    float dot[8] = {};
                     for (int c = 0; c < D / 8; ++c) {
-                        float x[8];
+                        float x[8], y[PA_REDO] = {};
                         paged_load8<D>(at, p.st.page_shift, row, c, x);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) dot[j] = fmaf(x[j], qs[8 * c + j], dot[j]);
+                        for (int e = 0; e < 8; ++e)
+#pragma unroll
+                            for (int k = 0; k < PA_REDO; ++k) y[k] = fmaf(x[e], sc.q[8 * c + e][k], y[k]);
+#pragma unroll
+                        for (int k = 0; k < PA_REDO; ++k) z[k] += y[k];
                     }
-                    z = (((dot[0] + dot[1]) + (dot[2] + dot[3])) + ((dot[4] + dot[5]) + (dot[6] + dot[7]))) * p.scale;
-                }
+                } else seen = 0;
+                sc.page[tid] = page;
             }
-            float top = z;
+            sc.seen[tid] = (uint8_t)seen;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if ((tid & 31) == 0) red[tid >> 5] = top;
+            for (int k = 0; k < PA_REDO; ++k) {
+                z[k] = seen >> k & 1 ? z[k] * p.scale : -INFINITY;
+                float top = z[k];
+#pragma unroll
+                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if ((tid & 31) == 0) sc.red[tid >> 5][k] = top;
+            }
             bar();
-            top = m;
+            float fix[PA_REDO];
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, red[w]);
-            const float fix = exp2f(m - top), w = seen ? exp2f(z - top) : 0.f;
-            ps[tid] = seen ? w : -1.f;                   // -1: hidden, its row of V is not touched
-            float sum = w;
+            for (int k = 0; k < PA_REDO; ++k) {
+                float top = m[k];
 #pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, sc.red[w][k]);
+                fix[k] = exp2f(m[k] - top);
+                z[k] = seen >> k & 1 ? exp2f(z[k] - top) : 0.f;
+                sc.w[tid][k] = z[k];
+                m[k] = top;
+            }
             bar();
-            if ((tid & 31) == 0) red[tid >> 5] = sum;
+#pragma unroll
+            for (int k = 0; k < PA_REDO; ++k) {
+#pragma unroll
+                for (int o = 16; o; o >>= 1) z[k] += __shfl_xor_sync(0xffffffffu, z[k], o);
+                if ((tid & 31) == 0) sc.red[tid >> 5][k] = z[k];
+            }
             bar();
-            l *= fix;
 #pragma unroll
-            for (int k = 0; k < PA_WARPS; ++k) l += red[k];
-            acc *= fix;
-            m = top;
-            if (tid < D)
-                for (int j = 0; j < PA_THREADS && b + j < g.u1 * unit; ++j) {
-                    if (ps[j] < 0.f) continue;
-                    const int kj = key_of(b + j), page = p.st.table[(int64_t)g.seq * p.st.max_pages + (kj >> p.st.page_shift)];
-                    const CT *at = reinterpret_cast<const CT *>(p.v_pool + paged_at(p.st, page, g.head));
-                    float x[8];
-                    paged_load8<D>(at, p.st.page_shift, kj & ((1 << p.st.page_shift) - 1), tid >> 3, x);
-                    float v = x[0];
+            for (int k = 0; k < PA_REDO; ++k) {
+                l[k] *= fix[k];
+                acc[k] *= fix[k];
 #pragma unroll
-                    for (int e = 1; e < 8; ++e) v = (tid & 7) == e ? x[e] : v;
-                    acc = fmaf(ps[j], v, acc);
-                }
+                for (int w = 0; w < PA_WARPS; ++w) l[k] += sc.red[w][k];
+            }
+            const int end = min(PA_THREADS, g.u1 * unit - b);
+#pragma unroll 4
+            for (int j = tid / D; j < end; j += PA_THREADS / D) {
+                const uint32_t which = sc.seen[j];       // a row of V that is hidden is not touched
+                const float v = which ? paged_load1<D>(reinterpret_cast<const CT *>(p.v_pool + paged_at(p.st, sc.page[j], g.head)), p.st.page_shift,
+                                                       key_of(b + j) & ((1 << p.st.page_shift) - 1), dim)
+                                      : 0.f;
+#pragma unroll
+                for (int k = 0; k < PA_REDO; ++k)
+                    if (which >> k & 1) acc[k] = fmaf(sc.w[j][k], v, acc[k]);
+            }
             bar();
         }
-        put(r, m, l, acc);
+        // the parts of the keys
+#pragma unroll
+        for (int k = 0; k < PA_REDO; ++k) sc.w[tid][k] = acc[k];
+        bar();
+#pragma unroll
+        for (int k = 0; k < PA_REDO; ++k) {
+            acc[k] = 0.f;
+#pragma unroll
+            for (int part = 0; part < PA_THREADS / D; ++part) acc[k] += sc.w[part * D + dim][k];
+            if (r0 + k < g.rows) put(r0 + k, m[k], l[k], acc[k]);
+        }
     }
     bar();
 }
@@ -254,6 +305,7 @@ template <class CT, int D, int NB, bool EX> struct PaTraits {
     static constexpr int BODY = (RING > COMB ? RING : COMB);
     static constexpr int Q_BYTES = Q_SMEM ? NT * NB * KS * 32 * 8 : 0;
     static constexpr size_t SMEM = 1024 + BODY + Q_BYTES;
+    static_assert(ROWS * (D + 4) * 4 + sizeof(PagedScratch<D>) <= BODY, "what a segment is computed again in lies over the ring too");
 };
 
 template <class CT, int D, int NB, bool EX>
@@ -270,7 +322,6 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
     __shared__ long long before[PA_MAX_SEQS + 1];
     __shared__ int seq_first[PA_MAX_SEQS], seq_n[PA_MAX_SEQS], seq_len[PA_MAX_SEQS];
     __shared__ float wml[PA_WARPS][2 * ROWS], rml[2 * ROWS];
-    __shared__ float scratch[D + PA_THREADS + PA_WARPS];
     __shared__ long long wsum_s[PA_WARPS];
     __shared__ int flags[2];                   // [0] a result is not finite, [1] a wait ran out
     __shared__ unsigned ticket;
@@ -290,7 +341,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             const int s = b + tid;
             long long x = 0;
             if (s < st.n_seqs) {
-                const PagedSeq sq = paged_seq(st, s);
+                const PagedSeq sq = paged_mine(p, s);
                 seq_first[s] = sq.first;
                 seq_n[s] = sq.n;
                 seq_len[s] = sq.len;
@@ -313,12 +364,18 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             __syncthreads();
         }
         total = (run & ((1LL << 40) - 1)) * st.heads;
-        if (total == 0) return;
+        if (total == 0) {
+            if (p.split) skn_pdl_wait();
+            return;
+        }
         // fewer CTAs where each would get less than a unit per warp; short segments get one each (nothing to join)
         const long long segments = (run >> 40) * st.heads;
         const long long want = total <= 2 * PA_WARPS * segments ? segments : (total + PA_WARPS - 1) / PA_WARPS;
         n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
-        if ((int)blockIdx.x >= n_cta) return;
+        if ((int)blockIdx.x >= n_cta) {
+            if (p.split) skn_pdl_wait();
+            return;
+        }
         u = total * blockIdx.x / n_cta;
         u_end = total * (blockIdx.x + 1) / n_cta;
     } else __syncthreads();
@@ -331,11 +388,14 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         if (p.direct) {
             g.seq = blockIdx.z;
             g.head = blockIdx.y;
-            const PagedSeq sq = paged_seq(st, g.seq);
+            const PagedSeq sq = paged_mine(p, g.seq);
             g.n = sq.n; g.len = sq.len; g.first = sq.first;
             const int n_blocks = (sq.n * p.group + ROWS - 1) / ROWS;
             const int rb = n_blocks - 1 - (int)blockIdx.x;              // the longest rows first
-            if (rb < 0) return;
+            if (rb < 0) {
+                if (p.split) skn_pdl_wait();
+                return;
+            }
             g.row0 = rb * ROWS;
             g.rows = min(ROWS, sq.n * p.group - g.row0);
             g.span = paged_span(p, sq.len - sq.n + g.row0 / p.group, sq.len - sq.n + (g.row0 + g.rows - 1) / p.group, UNIT);
@@ -934,8 +994,8 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         if (g.n_parts > 1) __threadfence();
         __syncthreads();
         if (flags[0]) {
-            const PagedSegment again = g;          // (a copy: the address of the one that the loops use is not taken)
-            paged_redo<CT, D, IO>(p, again, UNIT, scratch, [] { __syncthreads(); }, [=](int r, float rm, float rl, float acc) {
+            const PagedSegment seg = g;            // (a copy: the address of the one that the loops use is not taken)
+            paged_redo<CT, D, IO>(p, seg, UNIT, *reinterpret_cast<PagedScratch<D> *>(ring + ROWS * (D + 4) * 4), [] { __syncthreads(); }, [=](int r, float rm, float rl, float acc) {
                 if (tid < D) comb[r * (D + 4) + tid] = acc;
                 if (tid == 0) {
                     comb[r * (D + 4) + D] = rm;
@@ -992,6 +1052,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         skn_fence_proxy_async();                   // the rings were written to as results
         __syncthreads();
     }
+    if (p.split) skn_pdl_wait();               // (whoever waits for this launch waits for the one before)
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
@@ -1008,20 +1069,44 @@ template <class CT, int D, int NB, bool EX> static cudaError_t attn_launch(const
     static uint64_t done = 0;
     const cudaError_t e = paged_attributes(kern, T::SMEM, pc->ctx->device, &done);
     if (e != cudaSuccess) return e;
-    const int64_t rows = (int64_t)p.st.max_new * p.group;
-    const dim3 grid = p.direct ? dim3((unsigned)((rows + T::ROWS - 1) / T::ROWS), (unsigned)p.st.heads, (unsigned)p.st.n_seqs) : dim3((unsigned)(T::PER_SM * pc->ctx->sm_count));
-    kern<<<grid, PA_THREADS, T::SMEM, pc->ctx->stream>>>(p, pc->map[0], pc->map[1], pc->map[2], pc->map[3]);
-    return cudaGetLastError();
+    const int64_t rows = (int64_t)p.st.max_new * p.group, most = rows < p.upto ? rows : p.upto;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = p.direct ? dim3((unsigned)((most + T::ROWS - 1) / T::ROWS), (unsigned)p.st.heads, (unsigned)p.st.n_seqs) : dim3((unsigned)(T::PER_SM * pc->ctx->sm_count));
+    cfg.blockDim = dim3(PA_THREADS);
+    cfg.dynamicSmemBytes = T::SMEM;
+    cfg.stream = pc->ctx->stream;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = p.split ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, p, pc->map[0], pc->map[1], pc->map[2], pc->map[3]);
 }
 // bf16 rows of prompts (skn_paged_prompt.cuh); the first argument names the cache type
 cudaError_t skn_paged_prompt(__half, const skn_paged *pc, const PagedAttn &p);
 cudaError_t skn_paged_prompt(__nv_bfloat16, const skn_paged *pc, const PagedAttn &p);
 cudaError_t skn_paged_prompt(skn_q4, const skn_paged *pc, const PagedAttn &p);
 
+// Up to 32 rows a sequence: shared out with the keys.  More: blocks of rows, bf16 on tcgen05, fp32 a CTA each; then the sequences of a step that
+// have no more than 32 (decoding beside prompts) follow in a launch of their own, which begins while the first one ends.  (512 tokens of a prompt
+// beside 256 sequences of 2048 decoding, bf16, 32 / 8 heads of 128: all of them as blocks of 256 rows 643 us.)
 template <class CT, int D, bool EX> static cudaError_t attn_by_rows(const skn_paged *pc, PagedAttn &p) {
     const int64_t rows = (int64_t)p.st.max_new * p.group;
-    if (!EX && rows > SKN_PAGED_PART_ROWS) return skn_paged_prompt(CT(), pc, p);
-    p.direct = rows > SKN_PAGED_PART_ROWS || p.st.n_seqs > PA_MAX_SEQS;
+    p.above = 0;
+    p.upto = INT32_MAX;
+    if (rows > SKN_PAGED_PART_ROWS) {
+        const bool more = p.st.n_seqs > 1;
+        if (more) p.above = SKN_PAGED_PART_ROWS;
+        p.direct = 1;
+        if (!EX) p.split = more;
+        const cudaError_t e = EX ? attn_launch<CT, D, 4, EX>(pc, p) : skn_paged_prompt(CT(), pc, p);
+        if (e != cudaSuccess || !more) return e;
+        p.above = 0;
+        p.upto = SKN_PAGED_PART_ROWS;
+        p.parts = pc->d_parts + pc->prompt_parts;
+        p.tickets = pc->d_tickets + 2 * pc->n_parts;
+    }
+    p.direct = p.st.n_seqs > PA_MAX_SEQS;
     return rows <= 8 ? attn_launch<CT, D, 1, EX>(pc, p) : rows <= 16 ? attn_launch<CT, D, 2, EX>(pc, p) : attn_launch<CT, D, 4, EX>(pc, p);
 }
 template <class CT> static cudaError_t attn_by_type(const skn_paged *pc, int32_t io, PagedAttn &p) {

@@ -134,8 +134,21 @@ __device__ __forceinline__ bool pp_next(const PagedAttn &p, PpWalk &w, PagedSegm
             }
             continue;
         }
-        w.rb = w.head = 0;
-        if (++w.seq < p.st.n_seqs) w.sq = paged_seq(p.st, w.seq);
+        w.rb = w.head = 0;                       // the next sequence with rows for this launch: a lane each
+        for (int s0 = w.seq + 1;; s0 += 32) {
+            const int s = s0 + (int)(threadIdx.x & 31);
+            PagedSeq sq = {0, 0, 0};
+            if (s < p.st.n_seqs) sq = paged_mine(p, s);
+            const unsigned have = __ballot_sync(0xffffffffu, sq.n > 0);
+            if (have || s0 + 32 >= p.st.n_seqs) {
+                const int at = have ? __ffs(have) - 1 : 0;
+                w.seq = have ? s0 + at : p.st.n_seqs;
+                w.sq.first = __shfl_sync(0xffffffffu, sq.first, at);
+                w.sq.n = __shfl_sync(0xffffffffu, sq.n, at);
+                w.sq.len = __shfl_sync(0xffffffffu, sq.len, at);
+                break;
+            }
+        }
     }
     g.seq = w.seq; g.head = w.head; g.first = w.sq.first; g.n = w.sq.n; g.len = w.sq.len;
     g.row0 = w.rb * PP_ROWS;
@@ -177,7 +190,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     __shared__ int found[2];
     __shared__ uint32_t tmem_slot;
     __shared__ unsigned ticket;
-    __shared__ float scratch[D + PA_THREADS + PA_WARPS];
+    __shared__ int starts[THREADS + 1];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedStep &st = p.st;
 
@@ -203,25 +216,55 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         found[0] = -1;
     }
 
+    if (p.split) skn_pdl_launch_dependents();        // the launch for short sequences may take the SMs that this one leaves
+
     // ---- the line: items are the blocks of all sequences, each of them units x heads long ----------------------------------
     PpWalk w;
     {
-        // total first, then the block in which this CTA's share begins (which is known at once where there are no more blocks than threads)
+        // The total first, then the block in which this CTA's share begins (which is known at once where there are no more blocks than threads).
+        // Sequences THREADS at a time: where their blocks start, then a block per thread
         long long share = -1, at = 0, x = 0;
-        int seq = 0, skip = tid, rounds = 0;         // this thread's item: block `skip` counted from sequence `seq`
+        int seq = 0, rb = 0, rounds = 0;             // this thread's block
         for (int pass = 0; pass < 2; ++pass) {
-            if (pass == 0 || rounds > 1) {
-                long long run = 0;
-                PagedSeq sq = paged_seq(st, 0);
-                seq = 0;
-                skip = tid;
-                for (bool more = true; more;) {
-                    while (seq < st.n_seqs && skip >= pp_blocks(p, sq)) {
-                        skip -= pp_blocks(p, sq);
-                        if (++seq < st.n_seqs) sq = paged_seq(st, seq);
+            if (pass && rounds == 1) {
+                if (at <= share && share < at + x) {
+                    found[0] = seq;
+                    found[1] = rb;
+                    found_at = at;
+                }
+                break;
+            }
+            long long run = 0;
+            for (int s0 = 0; s0 < st.n_seqs; s0 += THREADS) {
+                const int mine = s0 + tid < st.n_seqs ? pp_blocks(p, paged_mine(p, s0 + tid)) : 0;
+                int upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                if (lane == 31) warp_sum[warp] = upto;
+                __syncthreads();
+                int n_blocks = 0;
+                for (int i = 0; i < THREADS / 32; ++i) {
+                    if (i < warp) upto += (int)warp_sum[i];
+                    n_blocks += (int)warp_sum[i];
+                }
+                starts[tid] = upto - mine;
+                __syncthreads();
+                for (int b0 = 0; b0 < n_blocks; b0 += THREADS) {
+                    const int b = b0 + tid;
+                    x = 0;
+                    if (b < n_blocks) {              // the last sequence that starts at or before b (those without blocks start where the next one does)
+                        int lo = 0, hi = THREADS - 1;
+                        while (lo < hi) {
+                            const int mid = (lo + hi + 1) >> 1;
+                            if (starts[mid] <= b) lo = mid; else hi = mid - 1;
+                        }
+                        seq = s0 + lo;
+                        rb = b - starts[lo];
+                        x = (long long)(pp_span(p, paged_mine(p, seq), rb).units + PP_COST) * st.heads;
                     }
-                    const bool have = seq < st.n_seqs;
-                    x = have ? (long long)(pp_span(p, sq, skip).units + PP_COST) * st.heads : 0;
                     long long inc = x;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
@@ -229,7 +272,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         if (lane >= o) inc += y;
                     }
                     if (lane == 31) warp_sum[warp] = inc;
-                    more = __syncthreads_or(have && tid == THREADS - 1);       // the last thread has an item: there may be others
+                    __syncthreads();
                     at = run + inc - x;
                     for (int i = 0; i < THREADS / 32; ++i) {
                         if (i < warp) at += warp_sum[i];
@@ -237,26 +280,21 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     }
                     if (pass && at <= share && share < at + x) {
                         found[0] = seq;
-                        found[1] = skip;
+                        found[1] = rb;
                         found_at = at;
                     }
                     if (pass == 0) ++rounds;
-                    if (more) skip += THREADS;
                     __syncthreads();
                 }
-                if (pass == 0) {
-                    w.total = run;
-                    if (run == 0) return;
-                    const long long want = (run + PP_COST) / (PP_COST + 1);        // a CTA for each block of a unit
-                    w.n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
-                    if ((int)blockIdx.x >= w.n_cta) return;
-                    share = w.u = run * blockIdx.x / w.n_cta;
-                    w.u_end = run * (blockIdx.x + 1) / w.n_cta;
-                }
-            } else if (at <= share && share < at + x) {
-                found[0] = seq;
-                found[1] = skip;
-                found_at = at;
+            }
+            if (pass == 0) {
+                w.total = run;
+                if (run == 0) return;
+                const long long want = (run + PP_COST) / (PP_COST + 1);        // a CTA for each block of a unit
+                w.n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
+                if ((int)blockIdx.x >= w.n_cta) return;
+                share = w.u = run * blockIdx.x / w.n_cta;
+                w.u_end = run * (blockIdx.x + 1) / w.n_cta;
             }
         }
         __syncthreads();
@@ -264,7 +302,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         w.rb = found[1];
         w.head = 0;
         w.a = found_at;
-        w.sq = paged_seq(st, w.seq);
+        w.sq = paged_mine(p, w.seq);
     }
     if (warp == 8) tc_alloc(&tmem_slot, 512);
     tc_fence_before();
@@ -459,7 +497,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             }
             if (pp_any(odd)) {
                 const PagedSegment again = now;      // (a copy: the address of the one that the loops use is not taken)
-                paged_redo<CT, D, IO>(p, again, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
+                paged_redo<CT, D, IO>(p, again, PP_KEYS, static_cast<PagedScratch<D> *>(p.scratch)[blockIdx.x], [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
                     const int tr = (now.row0 + row) / p.group;
                     if (shared) {
                         if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;

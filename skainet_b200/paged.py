@@ -155,6 +155,8 @@ class PagedKVCache:
         if q is None:
             more = (None, 0, 0, None, 0)
         else:
+            if q_out is None:
+                raise ValueError("the rotated queries need q_out (which may be q)")
             heads = q.shape[1]
             more = (q.data_ptr(), row(q, dt, n, heads), heads, q_out.data_ptr(), row(q_out, dt, n, heads))
         rc = self._lib.skn_paged_append_dev(self._h, batch._ref, io, k.data_ptr(), row(k, dt, n, kv), v.data_ptr(), row(v, dt, n, kv), *more)
@@ -172,7 +174,7 @@ class PagedKVCache:
             _raise(self.ctx.handle, rc)
 
     def attend_dev(self, batch: PagedBatch, q, out, scale: Optional[float] = None, window: int = 0, sinks: int = 0):
-        """out may be q"""
+        """out lies beside q, not over it"""
         io, n, heads, row = _io_of(q), batch.n_tokens, q.shape[1], self._row_stride
         if batch.device != self.ctx.device:
             raise ValueError("the step's tensors are on the context's device and of one type")

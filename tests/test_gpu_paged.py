@@ -580,3 +580,217 @@ def test_another_stream(ctx):
         ctx.set_stream(None)
     check(out.cpu().numpy(), want, mass, reach, "f32", "f16", False)
     cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "q4_0"])
+@pytest.mark.parametrize("dim,heads,rot,pairs", [(64, 1, 32, "adjacent"), (128, 3, 128, "halves")])
+def test_long_steps(ctx, dtype, dim, heads, rot, pairs):
+    """steps of thousands of rows, of an odd number, over many short sequences (some without a row), padded on both sides"""
+    page = 16
+    g = np.random.default_rng(dim)
+    news = g.integers(0, 30, 150)
+    lens = np.where(news > 0, news + g.integers(0, 40, 150), 3)
+    lens[5], news[5] = 4, 9                                # five padded rows
+    step = Step(9, lens, news, page, padding=6, first=3)
+    step.n += 1 - step.n % 2
+    assert step.n >= 2048 and step.n % 4
+    k, v, q = (g.standard_normal((step.n, h, dim)).astype(np.float32) for h in (heads, heads, 2 * heads))
+    cache, ref = filled(ctx, step, heads, dim, dtype, 11, rot, pairs)
+    got_q = cache.append(k, v, step.table, step.starts, step.lens, q)
+    want_q = ref.append(k, v, step.table, step.starts, step.lens, q)
+    tol = 3 * 2.0 ** -24 * (2 * np.abs(q).max(axis=2, keepdims=True)) + np.zeros_like(want_q)
+    tol[:, :, rot:] = 0
+    assert np.all(np.abs(got_q - want_q) <= tol)
+    b, given = step.batch(), torch.full((step.n, heads, dim), 7.0, device="cuda")
+    kk, vv = given.clone(), given.clone()
+    torch.cuda.synchronize()
+    cache.gather_dev(b, kk, vv)
+    ctx.sync()
+    cache.close()
+    want = [np.full((step.n, heads, dim), 7.0) for _ in range(2)]
+    for i, (s, p) in enumerate(oracle.positions(step.starts, step.lens)):
+        if p >= 0:
+            for w, pool in zip(want, (ref.k, ref.v)):
+                w[3 + i] = pool[step.table[s, p // page], :, p % page]
+    assert np.array_equal(kk.cpu().numpy(), want[0]) and np.array_equal(vv.cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("dtype,io", [("f16", "bf16"), ("bf16", "f32"), ("q4_0", "bf16"), ("q4_0", "f32")])
+@pytest.mark.parametrize("n_seqs,most,group", [(600, 1, 4), (600, 5, 8), (70, 1, 64)])
+def test_many_sequences(ctx, dtype, io, n_seqs, most, group):
+    g = np.random.default_rng(n_seqs + most)
+    lens = g.integers(most, 60, n_seqs)
+    news = g.integers(0, most + 1, n_seqs) if most > 1 else np.ones(n_seqs, dtype=np.int64)
+    step = Step(2, lens, news, 16)
+    kv, dim = 2, 64
+    cache, ref = filled(ctx, step, kv, dim, dtype, 3)
+    k, v = (g.standard_normal((step.n, kv, dim)).astype(np.float32) for _ in range(2))
+    q = bf16(g.standard_normal((step.n, kv * group, dim)))
+    cache.append(k, v, step.table, step.starts, step.lens)
+    ref.append(k, v, step.table, step.starts, step.lens)
+    want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    check(run_attend(cache, step, q, io), want, mass, reach, io, dtype, most * group > 32)
+    cache.close()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "q4_0"])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+def test_scales(ctx, io, dtype, scale):
+    """the mean of what is seen; the smallest products weigh most"""
+    kv, group, dim = 2, 4, 128
+    for lens, news, window in (([150, 3], [1, 1], 0), ([150, 140], [50, 33], 0), ([200], [60], 40)):
+        step = Step(2, lens, news, 32)
+        cache, ref = filled(ctx, step, kv, dim, dtype, 3)
+        g = np.random.default_rng(1)
+        k, v = (g.standard_normal((step.n, kv, dim)).astype(np.float32) for _ in range(2))
+        q = bf16(g.standard_normal((step.n, kv * group, dim)))
+        cache.append(k, v, step.table, step.starts, step.lens)
+        ref.append(k, v, step.table, step.starts, step.lens)
+        want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, scale, window, 2)
+        check(run_attend(cache, step, q, io, scale=scale, window=window, sinks=2), want, mass, reach, io, dtype, max(news) > 1)
+        cache.close()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "q4_0"])
+@pytest.mark.parametrize("lens,news", [([333, 20], [1, 1]), ([333, 200], [150, 9])])
+def test_rows_within_wider_ones(ctx, io, dtype, lens, news):
+    """queries are parts of a joint projection's rows; outputs rows at multiples of 16 bytes that are none of 32, the rest of which stays"""
+    kv, group, dim = 2, 3, 64
+    step = Step(2, lens, news, 32)
+    cache, ref = filled(ctx, step, kv, dim, dtype, 3)
+    g = np.random.default_rng(1)
+    k, v = (g.standard_normal((step.n, kv, dim)).astype(np.float32) for _ in range(2))
+    q = bf16(g.standard_normal((step.n, kv * group, dim)))
+    cache.append(k, v, step.table, step.starts, step.lens)
+    ref.append(k, v, step.table, step.starts, step.lens)
+    want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    H = kv * group
+    joint = torch.full((step.n, H + 2 * kv, dim), 3.0, device="cuda", dtype=IO[io])
+    joint[:, :H] = torch.from_numpy(q).to(IO[io])
+    width = H * dim + 8
+    flat = torch.full((step.n * width + 8,), 5.0, device="cuda", dtype=IO[io])
+    out = flat.as_strided((step.n, H, dim), (width, dim, 1), 8)
+    torch.cuda.synchronize()
+    cache.attend_dev(step.batch(), joint[:, :H], out)
+    ctx.sync()
+    check(out.float().cpu().numpy(), want, mass, reach, io, dtype, max(news) > 1)
+    assert (flat[8:].view(step.n, width)[:, H * dim:] == 5).all() and (flat[:8] == 5).all()
+    cache.close()
+
+
+def test_outputs_beside_their_queries_only(ctx):
+    """outputs in the same rows as the queries are right where they lie beside them, and refused where they lie over them"""
+    kv, group, dim = 2, 4, 64
+    step = Step(2, [90, 40], [20, 1], 16)
+    cache, ref = filled(ctx, step, kv, dim, "bf16", 3)
+    H = kv * group
+    wide = torch.randn(step.n + 1, 2 * H + 1, dim, device="cuda").bfloat16()
+    q = wide[:step.n, 1:H + 1]
+    want, mass, reach = ref.attend(q.float().cpu().numpy(), step.table, step.starts, step.lens, 0.125)
+    b = step.batch()
+    for out in (q, wide[:step.n, :H], wide[:step.n, 2:H + 2], wide[:step.n, H:2 * H], wide[1:, 1:H + 1], wide.view(-1)[:step.n * H * dim].view(step.n, H, dim)):
+        with pytest.raises(skn.SknError, match="over q"):
+            cache.attend_dev(b, q, out)
+    torch.cuda.synchronize()
+    cache.attend_dev(b, q, wide[:step.n, H + 1:])
+    ctx.sync()
+    check(wide[:step.n, H + 1:].float().cpu().numpy(), want, mass, reach, "bf16", "bf16", True)
+    cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_infinity_in_a_long_context(ctx, dtype):
+    """seen by every row of blocks with tens of thousands of keys, in one dimension"""
+    kv, group, dim, page = 1, 8, 64, 64
+    step = Step(4, [40000], [40], page)
+    cache, ref = filled(ctx, step, kv, dim, dtype, 5)
+    g = np.random.default_rng(9)
+    k, v = (g.standard_normal((step.n, kv, dim)).astype(np.float32) for _ in range(2))
+    q = bf16(g.standard_normal((step.n, kv * group, dim)))
+    cache.append(k, v, step.table, step.starts, step.lens)
+    ref.append(k, v, step.table, step.starts, step.lens)
+    want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    row = step.table[:1, :1], [0, 1], [1]
+    was = cache.gather(*row)
+    was[1][0, 0, 3] = np.inf
+    cache.append(was[0], was[1], *row)
+    for io in ("bf16", "f32"):
+        out = run_attend(cache, step, q, io)
+        assert (out[..., 3] == np.inf).all()
+        keep = np.arange(dim) != 3
+        check(out[..., keep], want[..., keep], mass[..., keep], reach[..., np.concatenate([[True], keep])], io, dtype, True)
+    cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "q4_0"])
+def test_captured_prompts(ctx, dtype):
+    """a captured step of up to 24 new tokens a sequence, replayed with other lengths, row counts, tables and windows' beginnings"""
+    kv, group, dim, page, rows = 2, 4, 64, 16, 60
+    g = np.random.default_rng(3)
+    n_pages, cols = 64, 12
+    cache = skn.PagedKVCache(ctx, n_pages, page, kv, dim, dtype)
+    ref = oracle.Pages(n_pages, page, kv, dim, dtype)
+    dt, starts = torch.zeros(3, cols, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    dl = torch.zeros(3, dtype=torch.int32, device="cuda")
+    b = skn.PagedBatch(dt, starts, dl, rows, 24)
+    k, v = (torch.zeros(rows, kv, dim, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    q, out = (torch.zeros(rows, kv * group, dim, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        cache.append_dev(b, k, v)
+        cache.attend_dev(b, q, out, window=50, sinks=2)
+    ctx.set_stream(None)
+    lens = np.zeros(3, dtype=np.int32)
+    for i in range(12):
+        news = np.array([g.integers(0, 25), 0 if i % 3 else 24, g.integers(1, 9)], dtype=np.int32)
+        if i == 6:
+            lens[:] = 0
+        lens = (lens + news).astype(np.int32)
+        assert lens.max() <= cols * page
+        table = g.permutation(n_pages)[:3 * cols].reshape(3, cols).astype(np.int32) if i in (0, 6) else table
+        at = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+        kn, vn, qn = (bf16(g.standard_normal((rows, h, dim))) for h in (kv, kv, kv * group))
+        given = bf16(g.standard_normal(qn.shape))
+        for d, h in ((dt, table), (starts, at), (dl, lens), (k, kn), (v, vn), (q, qn), (out, given)):
+            d.copy_(torch.from_numpy(h))
+        graph.replay()
+        torch.cuda.synchronize()
+        ctx.sync()
+        ref.append(kn, vn, table, at, lens)
+        want, mass, reach = ref.attend(qn, table, at, lens, dim ** -0.5, 50, 2, given=given)
+        got, n = out.float().cpu().numpy(), int(at[-1])
+        assert np.array_equal(got[n:], given[n:])
+        check(got[:n], want[:n], mass[:n], reach[:n], "bf16", dtype, True)
+    del graph
+    cache.close()
+
+
+def test_two_contexts_at_once(ctx):
+    """caches of two contexts work on streams of their own: each has its workspace"""
+    other = skn.Context(0)
+    jobs = []
+    for i, c in enumerate((ctx, other)):
+        for news in ([1, 1, 1], [20, 3, 40]):
+            step = Step(5 + i, [5000 + 900 * i, 300, 2000], news, 32)
+            cache, _ = filled(c, step, 2, 128, "bf16", 5 + i)
+            q = torch.randn(step.n, 8, 128, device="cuda").bfloat16()
+            out = torch.zeros_like(q)
+            torch.cuda.synchronize()
+            b = step.batch()
+            cache.attend_dev(b, q, out)
+            c.sync()
+            jobs.append((cache, b, q, out, out.clone(), c))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for cache, b, q, out, first, c in jobs:
+            cache.attend_dev(b, q, out)
+    ctx.sync()
+    other.sync()
+    for cache, b, q, out, first, c in jobs:
+        assert torch.equal(out, first)
+        cache.close()
+    other.close()

@@ -23,7 +23,7 @@ struct skn_paged {
     CUtensorMap map[4];          // K, V; of Q4_0 their quants, then their scales
     CUtensorMap wide[4];         // the same in larger boxes (prompts): whole pages of half rows; of Q4_0 up to 32 rows
     int n_parts;                 // CTAs that share a launch's work, at most
-    float *d_parts;              // prompts: blocks of rows of two segments per SM; then (from prompt_parts on) decoding: [2 n_parts][SKN_PAGED_PART_ROWS][head_dim + 4]:
+    float *d_parts;              // prompts: blocks of rows of two segments per SM; then (from prompt_parts on) decoding, two per CTA: [rows of a CTA's segment][head_dim + 4]:
     int64_t prompt_parts;        // output, maximum, sum
     unsigned *d_tickets;         // [2][2 n_parts], zero between launches
     uint8_t *d_again;            // prompts: a PagedScratch per SM

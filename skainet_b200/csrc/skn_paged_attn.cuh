@@ -28,7 +28,6 @@
 
 #include <math.h>
 
-constexpr int PA_WARPS = 8, PA_THREADS = 32 * PA_WARPS;
 constexpr int PA_MAX_SEQS = 512;            // sequences whose work is shared out; more of them take a CTA per segment
 constexpr float PA_NONE = -1e30f;            // running maximum before the first score
 
@@ -155,20 +154,20 @@ struct PagedSegment {
 __device__ __forceinline__ int paged_slot(const PagedSegment &g, int cta) { return 2 * cta + (cta == g.c0); }
 
 // A segment from the definition, eight rows at a time: a thread per key for the scores, then a thread per dimension (and part of the keys) for the outputs
-// (PA_THREADS of them, which `bar` brings together).  put(row, maximum (base 2), sum, this thread's dimension of the unnormalised output).
+// (THREADS of them, which `bar` brings together).  put(row, maximum (base 2), sum, this thread's dimension of the unnormalised output).
 // Eight rows share every load: a block of 256 rows that other roles of its CTA wait for is through its keys at some 15 us per thousand.
 constexpr int PA_REDO = 8;
-template <int D> struct PagedScratch {
-    float q[D][PA_REDO], w[PA_THREADS][PA_REDO], red[PA_WARPS][PA_REDO];
-    int page[PA_THREADS];
-    uint8_t seen[PA_THREADS];                            // a bit per row
+template <int D, int THREADS> struct PagedScratch {
+    float q[D][PA_REDO], w[THREADS][PA_REDO], red[THREADS / 32][PA_REDO];
+    int page[THREADS];
+    uint8_t seen[THREADS];                               // a bit per row
 };
-template <class CT, int D, class IO, class Bar, class Put>
-__device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &g, int unit, PagedScratch<D> &sc, Bar bar, Put put) {
+template <class CT, int D, int THREADS, class IO, class Bar, class Put>
+__device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &g, int unit, PagedScratch<D, THREADS> &sc, Bar bar, Put put) {
     const int tid = threadIdx.x, dim = tid % D;
     for (int r0 = 0; r0 < g.rows; r0 += PA_REDO) {
         bar();
-        for (int i = tid; i < PA_REDO * (D / 8); i += PA_THREADS) {
+        for (int i = tid; i < PA_REDO * (D / 8); i += THREADS) {
             const int k = i / (D / 8), c = i % (D / 8), R = g.row0 + r0 + k;
             float x[8] = {};
             if (r0 + k < g.rows) io_load8(static_cast<const IO *>(p.q) + (int64_t)(g.first + R / p.group) * p.q_stride + (g.head * p.group + R % p.group) * D + 8 * c, x);
@@ -182,7 +181,7 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
             m[k] = PA_NONE;
             l[k] = acc[k] = 0.f;
         }
-        for (int b = g.u0 * unit; b < g.u1 * unit; b += PA_THREADS) {
+        for (int b = g.u0 * unit; b < g.u1 * unit; b += THREADS) {
             auto key_of = [&](int i) { const int u = i / unit; return (u < g.span.a ? u : u + g.span.gap) * unit + i % unit; };
             const int key = key_of(b + tid);
             uint32_t seen = 0;
@@ -223,7 +222,7 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
             for (int k = 0; k < PA_REDO; ++k) {
                 float top = m[k];
 #pragma unroll
-                for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, sc.red[w][k]);
+                for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, sc.red[w][k]);
                 fix[k] = exp2f(m[k] - top);
                 z[k] = seen >> k & 1 ? exp2f(z[k] - top) : 0.f;
                 sc.w[tid][k] = z[k];
@@ -242,11 +241,11 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
                 l[k] *= fix[k];
                 acc[k] *= fix[k];
 #pragma unroll
-                for (int w = 0; w < PA_WARPS; ++w) l[k] += sc.red[w][k];
+                for (int w = 0; w < THREADS / 32; ++w) l[k] += sc.red[w][k];
             }
-            const int end = min(PA_THREADS, g.u1 * unit - b);
+            const int end = min(THREADS, g.u1 * unit - b);
 #pragma unroll 4
-            for (int j = tid / D; j < end; j += PA_THREADS / D) {
+            for (int j = tid / D; j < end; j += THREADS / D) {
                 const uint32_t which = sc.seen[j];       // a row of V that is hidden is not touched
                 const float v = which ? paged_load1<D>(reinterpret_cast<const CT *>(p.v_pool + paged_at(p.st, sc.page[j], g.head)), p.st.page_shift,
                                                        key_of(b + j) & ((1 << p.st.page_shift) - 1), dim)
@@ -265,7 +264,7 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
         for (int k = 0; k < PA_REDO; ++k) {
             acc[k] = 0.f;
 #pragma unroll
-            for (int part = 0; part < PA_THREADS / D; ++part) acc[k] += sc.w[part * D + dim][k];
+            for (int part = 0; part < THREADS / D; ++part) acc[k] += sc.w[part * D + dim][k];
             if (r0 + k < g.rows) put(r0 + k, m[k], l[k], acc[k]);
         }
     }
@@ -286,12 +285,15 @@ template <class CT, int D, int NB, bool EX> struct PaTraits {
     static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
     static constexpr int UNIT = Q4 ? 32 : 16;
     static constexpr int NT = EX ? (BF ? 3 : 2) : 1;
+    // A CTA of eight warps per SM; one row block of eight: CTAs of four, two per SM (Q4_0: four), so that one's queries, pages and results are under way
+    // while another computes
+    static constexpr int WARPS = NB == 1 ? 4 : 8, THREADS = 32 * WARPS;
     static constexpr int ROW = Q4 ? D / 2 + D / 16 : 2 * D;
     static constexpr int HALF = (16 * ROW + 127) / 128 * 128;                     // 16 rows, where TMA may put them
     static constexpr int TILE = UNIT / 16 * HALF, STAGE = 2 * TILE;               // K, then V
-    // eight warps' rings: about 190 KB of 16-bit rows in one CTA per SM; of 4 bits 74 KB (D = 128) in each of two
+    // the rings of an SM: about 190 KB of 16-bit rows; of 4 bits 148 KB (D = 128)
     static constexpr int STAGES = Q4 ? (D == 128 ? 2 : 4) : D == 128 ? (NB == 4 ? 2 : 3) : 6;
-    static constexpr int PER_SM = Q4 && NB == 1 ? 2 : 1;
+    static constexpr int PER_SM = NB > 1 ? 1 : Q4 ? 4 : 2;
     static constexpr int ROWS = 8 * NB;
     // Weights reach 2^SLACK before the maximum moves.  In fp16 they are lifted to 2^15 at most, so that a weight of 2^-24 - 15 + SLACK of its row's largest is
     // the last one there; fp32 rows, whose second term ends there too, pay for a smaller SLACK with more moves
@@ -300,35 +302,35 @@ template <class CT, int D, int NB, bool EX> struct PaTraits {
     static constexpr int V_UP = EX ? 12 : 7;                                      // Q4_0: the largest d, times 2^lift, is 2^V_UP .. 2^(V_UP + 1) when the lift is set
     static constexpr bool Q_SMEM = NB > 1 || (Q4 && EX);                          // query fragments in shared memory instead of registers
     static constexpr int KS = D / 16;
-    static constexpr int RING = PA_WARPS * STAGES * STAGE;
-    static constexpr int COMB = PA_WARPS * ROWS * (D + 4) * 4;                    // lies over the ring between segments
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int COMB = WARPS * ROWS * (D + 4) * 4;                     // lies over the ring between segments
     static constexpr int BODY = (RING > COMB ? RING : COMB);
     static constexpr int Q_BYTES = Q_SMEM ? NT * NB * KS * 32 * 8 : 0;
     static constexpr size_t SMEM = 1024 + BODY + Q_BYTES;
-    static_assert(ROWS * (D + 4) * 4 + sizeof(PagedScratch<D>) <= BODY, "what a segment is computed again in lies over the ring too");
+    static_assert(ROWS * (D + 4) * 4 + sizeof(PagedScratch<D, THREADS>) <= BODY, "what a segment is computed again in lies over the ring too");
 };
 
 template <class CT, int D, int NB, bool EX>
-__global__ void __launch_bounds__(PA_THREADS, (PaTraits<CT, D, NB, EX>::PER_SM))
+__global__ void __launch_bounds__((PaTraits<CT, D, NB, EX>::THREADS), (PaTraits<CT, D, NB, EX>::PER_SM))
 skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                       const __grid_constant__ CUtensorMap mks, const __grid_constant__ CUtensorMap mvs) {
     using T = PaTraits<CT, D, NB, EX>;
     using IO = typename std::conditional<EX, float, __nv_bfloat16>::type;
-    constexpr int UNIT = T::UNIT, NT = T::NT, KS = T::KS, STAGES = T::STAGES, ROWS = T::ROWS, NBLK = D / 32;
+    constexpr int UNIT = T::UNIT, NT = T::NT, KS = T::KS, STAGES = T::STAGES, ROWS = T::ROWS, NBLK = D / 32, WARPS = T::WARPS, THREADS = T::THREADS;
     extern __shared__ uint8_t raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     uint2 *qf = reinterpret_cast<uint2 *>(ring + T::BODY);
-    __shared__ uint64_t full[PA_WARPS * STAGES];
+    __shared__ uint64_t full[WARPS * STAGES];
     __shared__ long long before[PA_MAX_SEQS + 1];
     __shared__ int seq_first[PA_MAX_SEQS], seq_n[PA_MAX_SEQS], seq_len[PA_MAX_SEQS];
-    __shared__ float wml[PA_WARPS][2 * ROWS], rml[2 * ROWS];
-    __shared__ long long wsum_s[PA_WARPS];
+    __shared__ float wml[WARPS][2 * ROWS], rml[2 * ROWS];
+    __shared__ long long wsum_s[WARPS];
     __shared__ int flags[2];                   // [0] a result is not finite, [1] a wait ran out
     __shared__ unsigned ticket;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g8 = lane >> 2, t4 = lane & 3;
     const PagedStep &st = p.st;
 
-    if (tid < PA_WARPS * STAGES) skn_mbar_init(&full[tid], 1);
+    if (tid < WARPS * STAGES) skn_mbar_init(&full[tid], 1);
     if (tid < 2) flags[tid] = 0;
     skn_fence_mbar_init();
 
@@ -337,7 +339,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
     int n_cta = 1;
     if (!p.direct) {
         long long run = 0;
-        for (int b = 0; b < st.n_seqs; b += PA_THREADS) {
+        for (int b = 0; b < st.n_seqs; b += THREADS) {
             const int s = b + tid;
             long long x = 0;
             if (s < st.n_seqs) {
@@ -356,7 +358,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             if (lane == 31) wsum_s[warp] = inc;
             __syncthreads();
             long long base = run;
-            for (int w = 0; w < PA_WARPS; ++w) {
+            for (int w = 0; w < WARPS; ++w) {
                 if (w < warp) base += wsum_s[w];
                 run += wsum_s[w];
             }
@@ -370,7 +372,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         }
         // fewer CTAs where each would get less than a unit per warp; short segments get one each (nothing to join)
         const long long segments = (run >> 40) * st.heads;
-        const long long want = total <= 2 * PA_WARPS * segments ? segments : (total + PA_WARPS - 1) / PA_WARPS;
+        const long long want = total <= 2 * WARPS * segments ? segments : (total + WARPS - 1) / WARPS;
         n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
         if ((int)blockIdx.x >= n_cta) {
             if (p.split) skn_pdl_wait();
@@ -428,7 +430,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             u += g.u1 - g.u0;
         }
         const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
-        const int n_mine = (g.u1 - g.u0 - warp + PA_WARPS - 1) / PA_WARPS;         // units g.u0 + warp + PA_WARPS j
+        const int n_mine = (g.u1 - g.u0 - warp + WARPS - 1) / WARPS;         // units g.u0 + warp + WARPS j
 
         // ---- queries, on their way while the pages are looked up: this lane's part of row g8 of each block of eight ---------------
         // 16-bit caches: dims 16 k + 2 t, + 1, + 8, + 9.  Q4_0: of block k / 2, its lower (k even) or upper 16: 4 t, + 2, + 1, + 3
@@ -465,7 +467,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         // ---- loads of the warp's units: lane j of `pages` holds the pages of unit j (mod 32) ---------------------------------
         int page0 = -1, page1 = -1;
         auto key_of = [&](int j) {
-            const int i = g.u0 + warp + PA_WARPS * j;
+            const int i = g.u0 + warp + WARPS * j;
             return (i < g.span.a ? i : i + g.span.gap) * UNIT;
         };
         const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
@@ -957,10 +959,10 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             if (tid < ROWS) {
                 float top = PA_NONE;
 #pragma unroll
-                for (int w = 0; w < PA_WARPS; ++w) top = fmaxf(top, wml[w][2 * tid + 1] != 0.f ? wml[w][2 * tid] : PA_NONE);
+                for (int w = 0; w < WARPS; ++w) top = fmaxf(top, wml[w][2 * tid + 1] != 0.f ? wml[w][2 * tid] : PA_NONE);
                 float sum = 0.f;
 #pragma unroll
-                for (int w = 0; w < PA_WARPS; ++w) {
+                for (int w = 0; w < WARPS; ++w) {
                     const float f = wml[w][2 * tid + 1] != 0.f ? exp2f(wml[w][2 * tid] - top) : 0.f;
                     sum += wml[w][2 * tid + 1] * f;
                     wml[w][2 * tid] = f;
@@ -970,7 +972,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             }
             __syncthreads();
         }
-        float *const part = p.parts + (int64_t)g.slot * SKN_PAGED_PART_ROWS * (D + 4);
+        float *const part = p.parts + (int64_t)g.slot * ROWS * (D + 4);
         auto put4 = [&](int r, int d, float4 x, float m, float sum) {       // four dimensions of a row's result
             if (g.n_parts > 1) {
                 *reinterpret_cast<float4 *>(part + r * (D + 4) + d) = x;
@@ -978,11 +980,11 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             } else
                 paged_out4<IO>(p, g, r, d, D, x, sum);
         };
-        for (int i = tid; i < g.rows * (D / 4); i += PA_THREADS) {
+        for (int i = tid; i < g.rows * (D / 4); i += THREADS) {
             const int r = i / (D / 4), d = i % (D / 4) * 4;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; ++w) {
+            for (int w = 0; w < WARPS; ++w) {
                 const float f = wml[w][2 * r];
                 const float4 y = *reinterpret_cast<const float4 *>(comb + (w * ROWS + r) * (D + 4) + d);
                 if (f != 0.f) { x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w); }
@@ -995,14 +997,14 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
         __syncthreads();
         if (flags[0]) {
             const PagedSegment seg = g;            // (a copy: the address of the one that the loops use is not taken)
-            paged_redo<CT, D, IO>(p, seg, UNIT, *reinterpret_cast<PagedScratch<D> *>(ring + ROWS * (D + 4) * 4), [] { __syncthreads(); }, [=](int r, float rm, float rl, float acc) {
+            paged_redo<CT, D, THREADS, IO>(p, seg, UNIT, *reinterpret_cast<PagedScratch<D, THREADS> *>(ring + ROWS * (D + 4) * 4), [] { __syncthreads(); }, [=](int r, float rm, float rl, float acc) {
                 if (tid < D) comb[r * (D + 4) + tid] = acc;
                 if (tid == 0) {
                     comb[r * (D + 4) + D] = rm;
                     comb[r * (D + 4) + D + 1] = rl;
                 }
             });
-            for (int i = tid; i < g.rows * (D / 4); i += PA_THREADS) {
+            for (int i = tid; i < g.rows * (D / 4); i += THREADS) {
                 const int r = i / (D / 4), d = i % (D / 4) * 4;
                 put4(r, d, *reinterpret_cast<const float4 *>(comb + r * (D + 4) + d), comb[r * (D + 4) + D], comb[r * (D + 4) + D + 1]);
             }
@@ -1016,7 +1018,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             __syncthreads();
             if (ticket == (unsigned)g.n_parts - 1) {
                 __threadfence();
-                for (int i = tid; i < g.rows * (D / 4); i += PA_THREADS) {
+                for (int i = tid; i < g.rows * (D / 4); i += THREADS) {
                     const int r = i / (D / 4), d = i % (D / 4) * 4;
                     float top = PA_NONE, sum = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1025,7 +1027,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                         float4 y[8];
 #pragma unroll
                         for (int b = 0; b < 8; ++b) {
-                            const float *from = p.parts + ((int64_t)paged_slot(g, g.c0 + min(k + b, g.n_parts - 1)) * SKN_PAGED_PART_ROWS + r) * (D + 4);
+                            const float *from = p.parts + ((int64_t)paged_slot(g, g.c0 + min(k + b, g.n_parts - 1)) * ROWS + r) * (D + 4);
                             ml[b] = __ldcg(reinterpret_cast<const float2 *>(from + D));
                             y[b] = __ldcg(reinterpret_cast<const float4 *>(from + d));
                         }
@@ -1072,7 +1074,7 @@ template <class CT, int D, int NB, bool EX> static cudaError_t attn_launch(const
     const int64_t rows = (int64_t)p.st.max_new * p.group, most = rows < p.upto ? rows : p.upto;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = p.direct ? dim3((unsigned)((most + T::ROWS - 1) / T::ROWS), (unsigned)p.st.heads, (unsigned)p.st.n_seqs) : dim3((unsigned)(T::PER_SM * pc->ctx->sm_count));
-    cfg.blockDim = dim3(PA_THREADS);
+    cfg.blockDim = dim3(T::THREADS);
     cfg.dynamicSmemBytes = T::SMEM;
     cfg.stream = pc->ctx->stream;
     cudaLaunchAttribute attr = {};
@@ -1088,25 +1090,27 @@ cudaError_t skn_paged_prompt(__nv_bfloat16, const skn_paged *pc, const PagedAttn
 cudaError_t skn_paged_prompt(skn_q4, const skn_paged *pc, const PagedAttn &p);
 
 // Up to 32 rows a sequence: shared out with the keys.  More: blocks of rows, bf16 on tcgen05, fp32 a CTA each; then the sequences of a step that
-// have no more than 32 (decoding beside prompts) follow in a launch of their own, which begins while the first one ends.  (512 tokens of a prompt
-// beside 256 sequences of 2048 decoding, bf16, 32 / 8 heads of 128: all of them as blocks of 256 rows 643 us.)
+// have few (the rows of one token or a little more: decoding beside prompts) follow in a launch of their own, which begins while the first one ends.
+// (512 tokens of a prompt beside 256 sequences of 2048 decoding, bf16, 32 / 8 heads of 128: all of them as blocks of 256 rows 643 us.)
 template <class CT, int D, bool EX> static cudaError_t attn_by_rows(const skn_paged *pc, PagedAttn &p) {
-    const int64_t rows = (int64_t)p.st.max_new * p.group;
+    int64_t rows = (int64_t)p.st.max_new * p.group;
     p.above = 0;
     p.upto = INT32_MAX;
     if (rows > SKN_PAGED_PART_ROWS) {
         const bool more = p.st.n_seqs > 1;
-        if (more) p.above = SKN_PAGED_PART_ROWS;
+        const int few = p.group <= 8 ? 8 : p.group <= 16 ? 16 : SKN_PAGED_PART_ROWS;
+        if (more) p.above = few;
         p.direct = 1;
         if (!EX) p.split = more;
         const cudaError_t e = EX ? attn_launch<CT, D, 4, EX>(pc, p) : skn_paged_prompt(CT(), pc, p);
         if (e != cudaSuccess || !more) return e;
         p.above = 0;
-        p.upto = SKN_PAGED_PART_ROWS;
+        p.upto = few;
         p.parts = pc->d_parts + pc->prompt_parts;
         p.tickets = pc->d_tickets + 2 * pc->n_parts;
     }
     p.direct = p.st.n_seqs > PA_MAX_SEQS;
+    if (rows > p.upto) rows = p.upto;
     return rows <= 8 ? attn_launch<CT, D, 1, EX>(pc, p) : rows <= 16 ? attn_launch<CT, D, 2, EX>(pc, p) : attn_launch<CT, D, 4, EX>(pc, p);
 }
 template <class CT> static cudaError_t attn_by_type(const skn_paged *pc, int32_t io, PagedAttn &p) {

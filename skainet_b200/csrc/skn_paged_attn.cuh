@@ -150,6 +150,10 @@ struct PagedSegment {
     int c0, n_parts, slot;                // CTAs that have some of it: c0 .. c0 + n_parts - 1
 };
 
+// a / b of numbers that are not negative (a division in 64 bits takes several hundred cycles, and a launch of few units is some thousands)
+__device__ __forceinline__ long long paged_div(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
 // Where a CTA leaves its part of a segment that others share: a CTA ends in at most one such segment and begins in at most one
 __device__ __forceinline__ int paged_slot(const PagedSegment &g, int cta) { return 2 * cta + (cta == g.c0); }
 
@@ -378,8 +382,8 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             if (p.split) skn_pdl_wait();
             return;
         }
-        u = total * blockIdx.x / n_cta;
-        u_end = total * (blockIdx.x + 1) / n_cta;
+        u = paged_div(total * blockIdx.x, n_cta);
+        u_end = paged_div(total * (blockIdx.x + 1), n_cta);
     } else __syncthreads();
 
     int stage = 0, parity = 0;                 // of the warp's next unit
@@ -415,7 +419,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             g.row0 = 0; g.rows = g.n * p.group;
             g.span = paged_span(p, g.len - g.n, g.len - 1, UNIT);
             const long long off = u - before[lo];
-            g.head = (int)(off / g.span.units);
+            g.head = (int)paged_div(off, g.span.units);
             g.u0 = (int)(off - (long long)g.head * g.span.units);
             const long long left = u_end - u;
             g.u1 = left < g.span.units - g.u0 ? g.u0 + (int)left : g.span.units;
@@ -423,8 +427,8 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             g.n_parts = 1;
             if (g.u0 > 0 || g.u1 < g.span.units) {
                 const long long a = u - g.u0;
-                g.c0 = (int)(((a + 1) * n_cta - 1) / total);
-                g.n_parts = (int)(((a + g.span.units) * n_cta - 1) / total) - g.c0 + 1;
+                g.c0 = (int)paged_div((a + 1) * n_cta - 1, total);
+                g.n_parts = (int)paged_div((a + g.span.units) * n_cta - 1, total) - g.c0 + 1;
             }
             g.slot = paged_slot(g, (int)blockIdx.x);
             u += g.u1 - g.u0;

@@ -103,7 +103,7 @@ __device__ __forceinline__ uint64_t pp_ex2_pair(uint64_t x) {
     return skn_pack2(pp_ex2(a), pp_ex2(b));
 }
 
-// A CTA's share of the line, segment by segment; every role walks it for itself
+// A CTA's share of the line, segment by segment: one warp walks it ahead of the others and leaves the segments in shared memory
 struct PpWalk {
     long long u, u_end, total, a;               // a: where the present block and head begin
     int n_cta, seq, rb, head;
@@ -119,16 +119,15 @@ __device__ __forceinline__ bool pp_next(const PagedAttn &p, PpWalk &w, PagedSegm
         if (w.u >= w.u_end || w.seq >= p.st.n_seqs) return false;
         if (w.rb < pp_blocks(p, w.sq)) {
             g.span = pp_span(p, w.sq, w.rb);
-            const int length = g.span.units + PP_COST;
-            if (w.u < w.a + length) {
+            const int length = g.span.units + PP_COST, skip = (int)min((long long)(p.st.heads - w.head), paged_div(w.u - w.a, length));
+            w.a += (long long)skip * length;
+            w.head += skip;
+            if (w.head < p.st.heads) {
                 g.u0 = (int)max(0LL, w.u - w.a - PP_COST);
                 g.u1 = (int)min((long long)g.span.units, w.u_end - w.a - PP_COST);
                 w.u = min(w.u_end, w.a + length);
                 if (g.u1 > g.u0) break;
-                continue;
-            }
-            w.a += length;
-            if (++w.head == p.st.heads) {
+            } else {
                 w.head = 0;
                 ++w.rb;
             }
@@ -159,8 +158,8 @@ __device__ __forceinline__ bool pp_next(const PagedAttn &p, PpWalk &w, PagedSegm
         return true;
     }
     const long long a = w.a + PP_COST;
-    g.c0 = (int)(((a + 1) * w.n_cta - 1) / w.total);
-    g.n_parts = (int)(((a + g.span.units) * w.n_cta - 1) / w.total) - g.c0 + 1;
+    g.c0 = (int)paged_div((a + 1) * w.n_cta - 1, w.total);
+    g.n_parts = (int)paged_div((a + g.span.units) * w.n_cta - 1, w.total) - g.c0 + 1;
     g.slot = paged_slot(g, (int)blockIdx.x);
     return true;
 }
@@ -184,6 +183,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     uint8_t *const base = reinterpret_cast<uint8_t *>(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
     uint8_t *const q_tile = base, *const ring = base + 2 * TILE, *const raw_ring = ring + SLOTS * TILE;
     __shared__ uint64_t full[SLOTS], empty[SLOTS], raw_full[4], raw_empty[4];
+    __shared__ alignas(16) PagedSegment seg_ring[4];      // no rows: the last one
+    __shared__ uint64_t seg_full[4], seg_empty[4];
     __shared__ uint64_t s_full[2], p_full[4], pv_done[2], q_full[2], o_free[2], clean[SLOTS];
     __shared__ long long warp_sum[THREADS / 32];
     __shared__ long long found_at;
@@ -203,6 +204,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         for (int i = 0; i < 4; ++i) {
             skn_mbar_init(&raw_full[i], 1);
             skn_mbar_init(&raw_empty[i], 4);
+            skn_mbar_init(&seg_full[i], 1);
+            skn_mbar_init(&seg_empty[i], T::Q4 ? 14 : 11);        // 8 warps of softmax, MMA, TMA, clearing or 4 of unpacking
         }
         for (int i = 0; i < 2; ++i) {
             skn_mbar_init(&s_full[i], 1);
@@ -290,11 +293,11 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             if (pass == 0) {
                 w.total = run;
                 if (run == 0) return;
-                const long long want = (run + PP_COST) / (PP_COST + 1);        // a CTA for each block of a unit
+                const long long want = paged_div(run + PP_COST, PP_COST + 1);        // a CTA for each block of a unit
                 w.n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
                 if ((int)blockIdx.x >= w.n_cta) return;
-                share = w.u = run * blockIdx.x / w.n_cta;
-                w.u_end = run * (blockIdx.x + 1) / w.n_cta;
+                share = w.u = paged_div(run * blockIdx.x, w.n_cta);
+                w.u_end = paged_div(run * (blockIdx.x + 1), w.n_cta);
             }
         }
         __syncthreads();
@@ -310,6 +313,18 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     PagedSegment g = {};
+    uint32_t n_taken = 0;
+    bool got = true;                                 // no wait for a segment has run out
+    auto take = [&] {                                // the next segment, by a whole warp
+        const uint32_t i = n_taken & 3;
+        got = got && tc_wait_warp(&seg_full[i], n_taken >> 2 & 1, lane);
+        if (!got) return false;
+        g = seg_ring[i];
+        __syncwarp();
+        if (lane == 0) skn_mbar_arrive(&seg_empty[i]);
+        ++n_taken;
+        return g.rows > 0;
+    };
 
     // ---- softmax: warps 0 .. 3 rows 0 .. 127 of a block, warps 4 .. 7 the others ---------------------------------------------
     if (warp < 8) {
@@ -363,7 +378,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             // (a scale of zero moves into the queries: hidden scores of minus infinity stay what they are)
             return (p.scale == 0.f ? 1.f : fabsf(p.scale)) * f;
         };
-        bool more = pp_next(p, w, g);
+        bool more = take();
+        more = !pp_any(!got) && more;                // (the barriers below want every warp)
         float cs_next = 0.f;
         if (more && tile * 128 < g.rows) cs_next = load_queries();
         while (more) {
@@ -450,7 +466,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 }
             }
             // the next segment's queries: these are done with since the last scores
-            more = pp_next(p, w, g);
+            more = take();
             if (more && tile * 128 < g.rows) cs_next = load_queries();
             // ---- out, or to the other CTAs of the block -------------------------------------------------------------------------
             const bool shared = now.n_parts > 1;
@@ -459,7 +475,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             bool odd = false;
             if (used) {
                 if (ok) ok = tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane);
-                if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+                if (!(ok && got) && lane == 0) *st.status = SKN_ERR_TIMEOUT;
                 tc_fence_after();
                 const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
@@ -495,6 +511,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     part[(D + 1) * PP_ROWS + R] = l;
                 }
             }
+            if (pp_any(!got)) more = false;
             if (pp_any(odd)) {
                 const PagedSegment again = now;      // (a copy: the address of the one that the loops use is not taken)
                 paged_redo<CT, D, 256, IO>(p, again, PP_KEYS, static_cast<PagedScratch<D, 256> *>(p.scratch)[blockIdx.x], [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
@@ -583,7 +600,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             }
             __syncwarp();
         };
-        while (ok && pp_next(p, w, g)) {
+        while (ok && take()) {
             const int n = g.u1 - g.u0, tiles = g.rows > 128 ? 2 : 1;
             int k_slot = slot;
             for (int x = 0; x < tiles && ok; ++x) ok = tc_wait_warp(&q_full[x], segs[x] & 1, lane);
@@ -635,14 +652,14 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             }
             for (int x = 0; x < tiles; ++x) ++segs[x];
         }
-        if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+        if (!(ok && got) && lane == 0) *st.status = SKN_ERR_TIMEOUT;
     }
     // ---- loads: warp 9 -----------------------------------------------------------------------------------------------------------
     else if (warp == 9) {
         int slot = 0, parity = 0;
         bool ok = true;
         uint32_t loads = 0;
-        while (ok && pp_next(p, w, g)) {
+        while (ok && take()) {
             const int n = g.u1 - g.u0;
             const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
             const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
@@ -701,9 +718,9 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 }
             }
         }
-        if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+        if (!(ok && got) && lane == 0) *st.status = SKN_ERR_TIMEOUT;
         // nothing is on its way when the CTA ends: every load is waited for by who reads it, unless a wait ran out
-        if (!ok)
+        if (!(ok && got))
             for (int i = 0; i < (T::Q4 ? 4 : SLOTS); ++i) {
                 uint64_t *bar = T::Q4 ? &raw_full[i] : &full[i];
                 tc_wait_warp(bar, i < slot ? parity : parity ^ 1, lane);
@@ -719,7 +736,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 parity ^= 1;
             }
         };
-        while (ok && pp_next(p, w, g)) {
+        while (ok && take()) {
             const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
             const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
             for (int j = 0; j < g.u1 - g.u0 && ok; ++j) {
@@ -740,6 +757,25 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 step();
             }
         }
+        if (!(ok && got) && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+    }
+    // ---- the walk: warp 11 ------------------------------------------------------------------------------------------------------------
+    else if (warp == 11) {
+        bool ok = true;
+        uint32_t k = 0;
+        for (bool more = true; more; ++k) {
+            more = pp_next(p, w, g);
+            if (!more) g.rows = 0;
+            if (k >= 4 && !tc_wait_warp(&seg_empty[k & 3], (k >> 2 & 1) ^ 1, lane)) {
+                ok = false;
+                break;
+            }
+            if (lane == 0) {
+                seg_ring[k & 3] = g;
+                skn_mbar_arrive(&seg_full[k & 3]);
+            }
+            __syncwarp();
+        }
         if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
     }
     }
@@ -750,7 +786,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         uint32_t tiles = 0;
         bool ok = true;
         const int row = tid & 127;
-        while (ok && pp_next(p, w, g)) {
+        while (ok && take()) {
             const int pmin = g.len - g.n + g.row0 / p.group, pmax = g.len - g.n + (g.row0 + g.rows - 1) / p.group;
             const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
             for (int j = 0; j < g.u1 - g.u0 && ok; ++j) {
@@ -806,7 +842,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 }
             }
         }
-        if (!ok && lane == 0) *st.status = SKN_ERR_TIMEOUT;
+        if (!(ok && got) && lane == 0) *st.status = SKN_ERR_TIMEOUT;
     }
     __syncthreads();
     tc_fence_after();

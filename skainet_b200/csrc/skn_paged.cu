@@ -5,13 +5,12 @@
 #include <new>
 
 // ---- append -------------------------------------------------------------------------------------------------------------
-// A CTA takes one token, or four of a long step (TOKENS).  Where each of them goes is looked up and the sines and cosines of its position are formed
-// once, in shared memory (in 64 bits: the angle of a far position, and keys that land next to a border of the cache's rounding); its threads
-// take 16 dimensions of a head at a time, eight and the eight they turn with, so that the rotation may happen in place.  The rows are
-// requested a unit ahead, the first before all that.
-// Bound by HBM from a few thousand tokens on: 8192 tokens of 32 + 2 x 8 heads of 128, bf16 rows and cache, one token a CTA and requests behind
-// the sines 96 us, four and ahead of them in the tables below.
-constexpr int PAGED_LONG_STEP = 2048;        // tokens from which a CTA takes four: with fewer the GPU is not full of CTAs of one
+// A CTA takes one token.  Where it goes is looked up and the sines and cosines of its position are formed once, in shared memory (in 64 bits: the angle of
+// a far position, and keys that land next to a border of the cache's rounding); its threads take 16 dimensions of a head at a time, eight and the
+// eight they turn with, so that the rotation may happen in place.  The rows are requested a unit ahead, the first before all that.
+// Bound by HBM from a few thousand tokens on.  8192 tokens of 32 + 2 x 8 heads of 128, all of them turned: bf16 rows and cache 36.9 us (5.5 TB/s), fp32 rows and
+// a cache of 4 bits 63.1 us (5.5 TB/s); with requests behind the sines 96 us for the first; with four tokens to a CTA of 256 threads 41.4 and 68.3 us, no faster
+// for any smaller step (512 tokens 8.6 us instead of 8.1), and the same for the way back (20.5 us instead of 19.0).  Alone, a token is 3 us of latency.
 
 // sequence of row i: the last one that starts at or before it (-1: none).  Every warp counts the starts for itself: 32 of them at even distances, then
 // those between two of these.  (One after the other, 32 at a time, they are a chain of loads as long as the batch.)
@@ -86,7 +85,7 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedStep &st, int i) {
 }
 
 // eight dimensions and the eight they turn with, by fp32 or (keys) fp64 sines; c: the unit of 16.  Pair 8 c + i lies at [i][c]: the units of a
-// head are neighbouring lanes (at [8 c + i] they met in the same banks: 8192 tokens 52 us instead of the 43 of this form)
+// head are neighbouring lanes (at [8 c + i] they met in the same banks: with four tokens to a CTA 8192 of them took 52 us instead of 43)
 template <int UNITS, class F2, class F> __device__ __forceinline__ void paged_turn(float (&x)[8], float (&y)[8], const F2 *turn, int c, bool halves) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -128,22 +127,20 @@ template <> struct IoRow8<__nv_bfloat16> {
     }
 };
 
-template <class CT, int D, class IO, int TOKENS>
-__global__ void __launch_bounds__(TOKENS == 1 ? 128 : 256, TOKENS == 1 ? 8 : 4) skn_paged_append_kernel(const PagedStep st, const PagedRows r) {
+template <class CT, int D, class IO>
+__global__ void __launch_bounds__(128, 8) skn_paged_append_kernel(const PagedStep st, const PagedRows r) {
     constexpr bool Q4 = sizeof(CT) == 1;
-    constexpr int THREADS = TOKENS == 1 ? 128 : 256, UNITS = D / 16;
-    extern __shared__ float staged[];                  // Q4: the rotated keys, [TOKENS][heads][D]
-    __shared__ double2 turn[TOKENS][D / 2];
-    __shared__ float2 turn32[TOKENS][D / 2];
-    __shared__ PagedPlace place[TOKENS];
-    const int tid = threadIdx.x, first = blockIdx.x * TOKENS;
-    const int per_token = (r.q_heads + (Q4 ? 1 : 2) * st.heads) * UNITS, n_units = per_token * min(TOKENS, st.n_tokens - first);
+    constexpr int THREADS = 128, UNITS = D / 16;
+    extern __shared__ float staged[];                  // Q4: the rotated keys, [heads][D]
+    __shared__ double2 turn[D / 2];
+    __shared__ float2 turn32[D / 2];
+    __shared__ PagedPlace place;
+    const int tid = threadIdx.x, n_units = (r.q_heads + (Q4 ? 1 : 2) * st.heads) * UNITS;
+    const int64_t t = blockIdx.x;
     // where a unit's 16 dimensions are: head < 0: of the queries; from st.heads on: of the values
-    auto find = [&](int u, int &tok, int &head, int &c, int &a, int &b) {
-        tok = TOKENS == 1 ? 0 : u / per_token;
-        const int w = TOKENS == 1 ? u : u - tok * per_token;
-        head = w / UNITS - r.q_heads;
-        c = w % UNITS;
+    auto find = [&](int u, int &head, int &c, int &a, int &b) {
+        head = u / UNITS - r.q_heads;
+        c = u % UNITS;
         const bool turned = 16 * c < r.rot && head < st.heads;
         a = turned && r.halves ? c : 2 * c;
         b = turned && r.halves ? c + r.rot / 16 : 2 * c + 1;
@@ -152,9 +149,8 @@ __global__ void __launch_bounds__(TOKENS == 1 ? 128 : 256, TOKENS == 1 ? 8 : 4) 
     IoRow8<IO> x, y;
     auto request = [&](int u) {
         if (u < n_units) {
-            int tok, head, c, a, b;
-            find(u, tok, head, c, a, b);
-            const int64_t t = first + tok;
+            int head, c, a, b;
+            find(u, head, c, a, b);
             const IO *src = head < 0            ? static_cast<const IO *>(r.q) + t * r.q_stride + (head + r.q_heads) * D
                             : head < st.heads ? static_cast<const IO *>(r.k) + t * r.k_stride + head * D
                                               : static_cast<const IO *>(r.v) + t * r.v_stride + (head - st.heads) * D;
@@ -163,42 +159,40 @@ __global__ void __launch_bounds__(TOKENS == 1 ? 128 : 256, TOKENS == 1 ? 8 : 4) 
         }
     };
     request(tid);
-    if (tid < 32 * TOKENS) {
-        const PagedPlace at = paged_place(st, first + (tid >> 5));
-        if ((tid & 31) == 0) place[tid >> 5] = at;
+    if (tid < 32) {
+        const PagedPlace found = paged_place(st, blockIdx.x);
+        if (tid == 0) place = found;
     }
     __syncthreads();
-    for (int j = tid; j < TOKENS * (r.rot / 2); j += THREADS) {
-        const int tok = j / (r.rot / 2), i = j - tok * (r.rot / 2);
-        if (place[tok].pos >= 0) {
-            double2 t;
-            sincospi((double)place[tok].pos * r.turns[i], &t.y, &t.x);
-            const int to = (i & 7) * UNITS + (i >> 3);
-            turn[tok][to] = t;
-            turn32[tok][to] = make_float2((float)t.x, (float)t.y);
-        }
+    const PagedPlace at = place;
+    if (at.pos < 0) return;
+    for (int i = tid; i < r.rot / 2; i += THREADS) {
+        double2 x;
+        sincospi((double)at.pos * r.turns[i], &x.y, &x.x);
+        const int to = (i & 7) * UNITS + (i >> 3);
+        turn[to] = x;
+        turn32[to] = make_float2((float)x.x, (float)x.y);
     }
     __syncthreads();
     for (int u = tid; u < n_units; u += THREADS) {
-        int tok, head, c, a, b;
-        const bool turned = find(u, tok, head, c, a, b);
-        const PagedPlace at = place[tok];
+        int head, c, a, b;
+        const bool turned = find(u, head, c, a, b);
         float xf[8], yf[8];
         x.get(xf);
         y.get(yf);
         request(u + THREADS);
-        if (at.pos < 0 || (head >= 0 && at.page < 0)) continue;
+        if (head >= 0 && at.page < 0) continue;
         if (turned) {
-            if (head < 0) paged_turn<UNITS, float2, float>(xf, yf, turn32[tok], c, r.halves);
-            else paged_turn<UNITS, double2, double>(xf, yf, turn[tok], c, r.halves);
+            if (head < 0) paged_turn<UNITS, float2, float>(xf, yf, turn32, c, r.halves);
+            else paged_turn<UNITS, double2, double>(xf, yf, turn, c, r.halves);
         }
         if (head < 0) {
-            IO *to = static_cast<IO *>(r.q_out) + (int64_t)(first + tok) * r.q_out_stride + (head + r.q_heads) * D;
+            IO *to = static_cast<IO *>(r.q_out) + t * r.q_out_stride + (head + r.q_heads) * D;
             io_store8(to + 8 * a, xf);
             io_store8(to + 8 * b, yf);
         } else if constexpr (Q4) {
-            io_store8(staged + (tok * st.heads + head) * D + 8 * a, xf);
-            io_store8(staged + (tok * st.heads + head) * D + 8 * b, yf);
+            io_store8(staged + head * D + 8 * a, xf);
+            io_store8(staged + head * D + 8 * b, yf);
         } else {
             CT *to = reinterpret_cast<CT *>(head < st.heads ? r.k_pool + paged_at(st, at.page, head) : r.v_pool + paged_at(st, at.page, head - st.heads)) + at.row * D;
             io_store8(to + 8 * a, xf);
@@ -208,14 +202,12 @@ __global__ void __launch_bounds__(TOKENS == 1 ? 128 : 256, TOKENS == 1 ? 8 : 4) 
     if constexpr (Q4) {
         __syncthreads();
         // four neighbouring lanes per block of 32 dims; the bound is a multiple of four, so they stay together
-        const int per = 2 * st.heads * (D / 8);
-        for (int u = tid; u < per * min(TOKENS, st.n_tokens - first); u += THREADS) {
-            const int tok = TOKENS == 1 ? 0 : u / per, w = u - tok * per, head = w / (D / 8), c = w % (D / 8);
-            const PagedPlace at = place[tok];
-            if (at.page < 0) continue;               // (the same for the four)
+        if (at.page < 0) return;
+        for (int u = tid; u < 2 * st.heads * (D / 8); u += THREADS) {
+            const int head = u / (D / 8), c = u % (D / 8);
             float z[8];
-            if (head < st.heads) io_load8(staged + (tok * st.heads + head) * D + 8 * c, z);
-            else io_load8(static_cast<const IO *>(r.v) + (int64_t)(first + tok) * r.v_stride + (head - st.heads) * D + 8 * c, z);
+            if (head < st.heads) io_load8(staged + head * D + 8 * c, z);
+            else io_load8(static_cast<const IO *>(r.v) + t * r.v_stride + (head - st.heads) * D + 8 * c, z);
             uint8_t *to = head < st.heads ? r.k_pool + paged_at(st, at.page, head) : r.v_pool + paged_at(st, at.page, head - st.heads);
             q4_store<D>(to, st.page_shift, at.row, c >> 2, c & 3, z);
         }
@@ -223,25 +215,23 @@ __global__ void __launch_bounds__(TOKENS == 1 ? 128 : 256, TOKENS == 1 ? 8 : 4) 
 }
 
 // ---- gather ---------------------------------------------------------------------------------------------------------------
-template <class CT, int D, class IO, int TOKENS>
+template <class CT, int D, class IO>
 __global__ void __launch_bounds__(256) skn_paged_gather_kernel(const PagedStep st, const uint8_t *k_pool, const uint8_t *v_pool, IO *k_out, IO *v_out) {
-    __shared__ PagedPlace place[TOKENS];
-    const int tid = threadIdx.x, first = blockIdx.x * TOKENS;
-    if (tid < 32 * TOKENS) {
-        const PagedPlace at = paged_place(st, first + (tid >> 5));
-        if ((tid & 31) == 0) place[tid >> 5] = at;
+    __shared__ PagedPlace place;
+    if (threadIdx.x < 32) {
+        const PagedPlace found = paged_place(st, blockIdx.x);
+        if (threadIdx.x == 0) place = found;
     }
     __syncthreads();
-    const int per = 2 * st.heads * (D / 8);
-    for (int u = tid; u < per * TOKENS; u += 256) {
-        const int tok = u / per, w = u - tok * per, head = w / (D / 8), c = w % (D / 8);
-        const PagedPlace at = place[tok];
-        if (at.page < 0) continue;
+    const PagedPlace at = place;
+    if (at.page < 0) return;
+    for (int u = threadIdx.x; u < 2 * st.heads * (D / 8); u += 256) {
+        const int head = u / (D / 8), c = u % (D / 8);
         const bool is_v = head >= st.heads;
         const int h = is_v ? head - st.heads : head;
         float x[8];
         paged_load8<D>(reinterpret_cast<const CT *>((is_v ? v_pool : k_pool) + paged_at(st, at.page, h)), st.page_shift, at.row, c, x);
-        io_store8((is_v ? v_out : k_out) + ((int64_t)(first + tok) * st.heads + h) * D + 8 * c, x);
+        io_store8((is_v ? v_out : k_out) + ((int64_t)blockIdx.x * st.heads + h) * D + 8 * c, x);
     }
 }
 
@@ -296,25 +286,18 @@ static int32_t check_io(skn_ctx *ctx, int32_t io) {
     return SKN_OK;
 }
 
-template <class CT, int D, class IO, int TOKENS> static cudaError_t append_with(const PagedStep &st, const PagedRows &r, cudaStream_t stream) {
-    const size_t smem = sizeof(CT) == 1 ? (size_t)TOKENS * st.heads * D * sizeof(float) : 0;
-    auto *kern = skn_paged_append_kernel<CT, D, IO, TOKENS>;
+template <class CT, int D, class IO> static cudaError_t append_launch(const PagedStep &st, const PagedRows &r, cudaStream_t stream) {
+    const size_t smem = sizeof(CT) == 1 ? (size_t)st.heads * D * sizeof(float) : 0;
+    auto *kern = skn_paged_append_kernel<CT, D, IO>;
     if (smem > 32000) {
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    kern<<<(st.n_tokens + TOKENS - 1) / TOKENS, TOKENS == 1 ? 128 : 256, smem, stream>>>(st, r);
+    kern<<<st.n_tokens, 128, smem, stream>>>(st, r);
     return cudaGetLastError();
 }
-template <class CT, int D, class IO> static cudaError_t append_launch(const PagedStep &st, const PagedRows &r, cudaStream_t stream) {
-    // (four tokens' staged keys of 4 bits have to fit shared memory: up to 96 kv heads of 128)
-    return st.n_tokens >= PAGED_LONG_STEP && (sizeof(CT) > 1 || st.heads * D <= 96 * 128) ? append_with<CT, D, IO, 4>(st, r, stream) : append_with<CT, D, IO, 1>(st, r, stream);
-}
 template <class CT, int D, class IO> static cudaError_t gather_launch(const PagedStep &st, const skn_paged *pc, void *k, void *v, cudaStream_t stream) {
-    if (st.n_tokens >= PAGED_LONG_STEP)
-        skn_paged_gather_kernel<CT, D, IO, 4><<<(st.n_tokens + 3) / 4, 256, 0, stream>>>(st, pc->k, pc->v, static_cast<IO *>(k), static_cast<IO *>(v));
-    else
-        skn_paged_gather_kernel<CT, D, IO, 1><<<st.n_tokens, 256, 0, stream>>>(st, pc->k, pc->v, static_cast<IO *>(k), static_cast<IO *>(v));
+    skn_paged_gather_kernel<CT, D, IO><<<st.n_tokens, 256, 0, stream>>>(st, pc->k, pc->v, static_cast<IO *>(k), static_cast<IO *>(v));
     return cudaGetLastError();
 }
 #define PAGED_BY_IO(fn, CT, D, ...) (io == SKN_KV_F32 ? fn<CT, D, float>(__VA_ARGS__) : fn<CT, D, __nv_bfloat16>(__VA_ARGS__))

@@ -30,7 +30,7 @@ template <class CT, int D> struct PpTraits {
     static constexpr int SLACK = 4;
     static constexpr float LIFT = BF ? 0.f : 11.f;                // exponent: fp16 weights up to 2^15 (see skn_paged_attn.cuh)
     // registers a thread of the softmax warpgroups, of the MMA / TMA / clearing warpgroup and of the unpacking one: at most the launch's, 384 x 168 or 512 x 128
-    static constexpr int REGS_SOFT = Q4 ? 176 : 208, REGS_MMA = Q4 ? 64 : 80, REGS_UNPACK = 96;
+    static constexpr int REGS_SOFT = Q4 ? 184 : 208, REGS_MMA = Q4 ? 64 : 80, REGS_UNPACK = 80;
     static_assert(128 * (2 * REGS_SOFT + REGS_MMA + (Q4 ? REGS_UNPACK : 0)) <= THREADS * (Q4 ? 128 : 168), "more than the launch has");
 };
 

@@ -361,11 +361,13 @@ typedef struct skn_paged_spec {
  * lengths[s]) are padding: they are not appended or gathered, and their attention output is zero.  Rows before token_start[0] and from
  * token_start[n_seqs] on belong to nobody and are left as they are.  Entries of pages that no call needs (beyond the
  * length, or outside every query's window) may hold anything.  The arrays are on the device for `_dev` calls, whose kernels check
- * what they use of them: a sequence or a page out of range is skipped, and the next skn_sync returns SKN_ERR_ARG. */
+ * what they use of them: the next skn_sync returns SKN_ERR_ARG where something is out of range.  A sequence whose rows do not lie in the step, are
+ * more than max_new, or whose length its table cannot hold, is left out (its outputs stay as they are); a page that is none is not touched,
+ * and what attention says of its sequence means nothing.  Other sequences of the step are not affected. */
 typedef struct skn_paged_batch {
-    int32_t n_seqs, n_tokens;        /* n_tokens: rows of k, v, q and out */
+    int32_t n_seqs, n_tokens;        /* at most 65535; n_tokens: rows of k, v, q and out, at most 2^24 */
     int32_t max_new;                 /* no sequence has more new tokens */
-    int32_t max_pages;               /* columns of the page table */
+    int32_t max_pages;               /* columns of the page table, at most 2^23 */
     const int32_t *page_table;       /* [n_seqs][max_pages] */
     const int32_t *token_start;      /* [n_seqs + 1], not decreasing */
     const int32_t *lengths;          /* [n_seqs] */
@@ -373,15 +375,17 @@ typedef struct skn_paged_batch {
 /* bytes of one pool of this specification (host arithmetic; the message of a refusal is read with skn_last_error(NULL)) */
 int32_t skn_paged_pool_bytes(const skn_paged_spec *spec, int64_t *bytes);
 /* k_pool_dev, v_pool_dev: device memory of skn_paged_pool_bytes bytes each, 16-byte aligned, that outlives the cache; or both NULL: the
- * cache allocates them, filled with zeros.  The workspace of attention is allocated here, so every `_dev` call below can be captured
- * into a CUDA graph; calls on one cache share it and have to be ordered on the device (one stream, or events). */
+ * cache allocates them, filled with zeros.  The workspace of attention (47 MB on a GPU of 148 SMs for head_dim 128, 25 MB for 64) is allocated here, so
+ * every `_dev` call below can be captured into a CUDA graph; calls on one cache share it and have to be ordered on the device (one stream, or
+ * events).  n_pages * n_kv_heads * page_tokens is at most 2^31 - 1. */
 int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_dev, void *v_pool_dev, skn_paged **out);
 int32_t skn_paged_destroy(skn_paged *pc);
 int32_t skn_paged_info(const skn_paged *pc, void **k_pool_dev, void **v_pool_dev, int64_t *pool_bytes);
 /* Append the step's keys and values, the keys rotated to their positions; q (optional) is rotated into q_out, which may be q.
- * `_dev`: at most 2^24 rows a step; io is the element type of k, v, q and q_out (SKN_KV_F32 or SKN_KV_BF16), a row [heads][head_dim]; strides are the elements from one
- * row to the next (rows of a joint projection need no copy).  Pointers and rows are 16-byte aligned.  A page that a step appends to belongs to
- * one of its sequences only.  The host form takes dense fp32 rows and answers every mistake before anything has run. */
+ * `_dev`: io is the element type of k, v, q and q_out (SKN_KV_F32 or SKN_KV_BF16), a row [heads][head_dim]; strides are the elements from one
+ * row to the next (rows of a joint projection need no copy).  Pointers and rows are 16-byte aligned.  Rows of nobody and padded rows of q_out stay
+ * as they are.  A row of a page is appended to by one of the step's sequences only.  The host form takes dense fp32 rows and answers every mistake
+ * before anything has run. */
 int32_t skn_paged_append(skn_paged *pc, const skn_paged_batch *batch, const float *k_host, const float *v_host, const float *q_host,
                          int32_t n_q_heads, float *q_out_host);
 int32_t skn_paged_append_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, const void *k_dev, int64_t k_stride, const void *v_dev,
@@ -392,8 +396,10 @@ int32_t skn_paged_gather(skn_paged *pc, const skn_paged_batch *batch, float *k_o
 int32_t skn_paged_gather_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, void *k_out_dev, void *v_out_dev);
 /* out = softmax(scale * q . K^T) . V of every row over the cached tokens at its own position and before: all of them (window 0), or the last
  * `window`, its own included, and the first `sinks` of the sequence.  Query head h reads kv head h / (n_q_heads / n_kv_heads).  What is not
- * visible has no influence, whatever it holds.  fp32 rows: fp32 accuracy.  bf16 rows: queries exact, softmax weights rounded to
- * fp16 (bf16 caches: bf16), fp32 sums. */
+ * visible has no influence, whatever it holds.  At most 64 query heads per kv head; out may not lie over q (rows side by side in
+ * wider ones are fine).  fp32 rows: fp32 accuracy.  bf16 rows: queries exact (down to 2^-38 of a row's largest), softmax weights rounded to fp16 (bf16
+ * caches: bf16), fp32 sums; in a step whose max_new times the query heads per kv head is above 32, the dequantised rows of a Q4_0 cache may be
+ * rounded to fp16 as well. */
 int32_t skn_paged_attn(skn_paged *pc, const skn_paged_batch *batch, const float *q_host, int32_t n_q_heads, float scale, int32_t window,
                        int32_t sinks, float *out_host);
 int32_t skn_paged_attn_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, const void *q_dev, int64_t q_stride, int32_t n_q_heads,

@@ -21,6 +21,11 @@
 // zero: in units with hidden keys, rows that nobody sees are cleared if they are not finite.  Whatever else goes wrong with such values
 // (a key that some rows see and others do not; an infinity that meets the two terms of a weight) leaves a result that is not finite,
 // and a segment with one is computed again straight from the definition (paged_redo).
+//
+// 16-bit caches are bound by HBM: 16 sequences of 8192 tokens, 32 / 8 heads of 128, 97 us for fp32 rows and 95 us for bf16 ones (5.5 and 5.7 TB/s, 0.86 of a copy's
+// rate), 48 sequences with a window of 4096 135 us (6.0 TB/s).  Q4_0 by its instructions: 64 sequences of 16384, bf16 rows, 393 us (3.1 TB/s; 59 % of the
+// issue slots, the ALU pipe at 51 %: masks, permutes and conversions of V), fp32 rows, with two terms of everything, half as fast.  One sequence of
+// 100 tokens is 8 us of latency.  Shares smaller than the CTAs that run at a time (twice as many) cost 95 -> 101 us: every share has a beginning.
 #pragma once
 #include "skn_paged.cuh"
 #include "skn_mma.cuh"
@@ -28,7 +33,9 @@
 
 #include <math.h>
 
-constexpr int PA_MAX_SEQS = 512;            // sequences whose work is shared out; more of them take a CTA per segment
+// Sequences whose work is shared out (their places are in shared memory); more of them take a CTA per segment.  300 sequences: of 1000 tokens each 195 us
+// shared out, 183 as CTAs; of 500 and one of 32768 133 us against 447.
+constexpr int PA_MAX_SEQS = 512;
 constexpr float PA_NONE = -1e30f;            // running maximum before the first score
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -290,7 +297,7 @@ template <class CT, int D, int NB, bool EX> struct PaTraits {
     static constexpr int UNIT = Q4 ? 32 : 16;
     static constexpr int NT = EX ? (BF ? 3 : 2) : 1;
     // A CTA of eight warps per SM; one row block of eight: CTAs of four, two per SM (Q4_0: four), so that one's queries, pages and results are under way
-    // while another computes
+    // while another computes (64 sequences of 300 tokens 36.9 -> 26.6 us, 16 of 8192 95 -> 96)
     static constexpr int WARPS = NB == 1 ? 4 : 8, THREADS = 32 * WARPS;
     static constexpr int ROW = Q4 ? D / 2 + D / 16 : 2 * D;
     static constexpr int HALF = (16 * ROW + 127) / 128 * 128;                     // 16 rows, where TMA may put them
@@ -374,7 +381,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             if (p.split) skn_pdl_wait();
             return;
         }
-        // fewer CTAs where each would get less than a unit per warp; short segments get one each (nothing to join)
+        // fewer CTAs where each would get less than a unit per warp; short segments get one each (nothing to join: 100 tokens of one sequence 18.5 -> 9.2 us)
         const long long segments = (run >> 40) * st.heads;
         const long long want = total <= 2 * WARPS * segments ? segments : (total + WARPS - 1) / WARPS;
         n_cta = want < (long long)gridDim.x ? (int)want : (int)gridDim.x;
@@ -1095,7 +1102,9 @@ cudaError_t skn_paged_prompt(skn_q4, const skn_paged *pc, const PagedAttn &p);
 
 // Up to 32 rows a sequence: shared out with the keys.  More: blocks of rows, bf16 on tcgen05, fp32 a CTA each; then the sequences of a step that
 // have few (the rows of one token or a little more: decoding beside prompts) follow in a launch of their own, which begins while the first one ends.
-// (512 tokens of a prompt beside 256 sequences of 2048 decoding, bf16, 32 / 8 heads of 128: all of them as blocks of 256 rows 643 us.)
+// (512 tokens of a prompt beside 256 sequences of 2048 decoding, bf16, 32 / 8 heads of 128: 356 us; all of them as blocks of 256 rows 643; both on their own
+// 30 and 329.)  Where the two kernels meet, fp16 pages, 4 query heads per kv head: 8 tokens (32 rows) here and 9 there, behind 512 cached ones 20.6
+// and 23.0 us, 4096: 41.0 and 34.9, 16384: 51.4 and 59.8; 32 sequences of 2048 88.7 and 90.6.
 template <class CT, int D, bool EX> static cudaError_t attn_by_rows(const skn_paged *pc, PagedAttn &p) {
     int64_t rows = (int64_t)p.st.max_new * p.group;
     p.above = 0;

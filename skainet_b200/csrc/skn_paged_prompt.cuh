@@ -1,22 +1,30 @@
-// Attention of prompts over the paged KV cache: bf16 rows, more than the 32 rows per kv head that the kernel of skn_paged_attn.cuh takes at a time.
+// Attention of prompts over the paged KV cache: bf16 rows, more of them per kv head than the kernel of skn_paged_attn.cuh takes at a time.
 //
 // 256 rows (tokens x query heads of one kv head) in two tiles of 128 against 128 keys at a time, on tcgen05: S = Q K^T and O += P V with S, O and P in tensor
 // memory (P in fp16, bf16 for bf16 caches, over its own S: the first operand of the second product), Q, K and V in shared memory with 128-byte swizzle, V
 // as the transposed second operand.  A thread of the two softmax warpgroups owns a row: its maximum and sum need no exchange.  The maximum moves only
 // when a weight would exceed 2^SLACK; O is then scaled where it is, by the same threads.  While one tile's softmax runs, the tensor cores work
-// on the other tile.  One warp issues the MMAs, one the TMA loads (a box per page, or 128 rows of larger ones).  Q4_0: a warpgroup turns quants into
-// fp16 (q - 8) d between the two.
+// on the other tile.  Weights are handed over in halves (of 64 keys); in quarters the waits cost more than the earlier start gives (a prompt of 8192
+// tokens 534 -> 585 us).  One warp issues the MMAs, one the TMA loads (a box per page, or 128 rows of larger ones).  Q4_0: a warpgroup turns quants
+// into fp16 (q - 8) d between the two.
 //
 // Work is shared out as in skn_paged_attn.cuh: the units (128 keys of a block of rows) of all blocks form one line, one contiguous share for each CTA;
-// blocks that lie in several shares are joined by the last of their CTAs to finish.
+// blocks that lie in several shares are joined by the last of their CTAs to finish.  One warp walks the line for all the others (each for itself
+// held its state in registers, which the softmax warps had to spill: 544 -> 512 us).
 //
 // Hidden rows of V (behind the last key that the block sees, before its window, on pages that were given back) are cleared in shared memory before the
 // product: a warp does it in the few units that have some.  A result that is not finite is computed again from the definition.
+//
+// Bound by the chain of a tile (scores, softmax, products, each waiting for the one before) at about half of what the exponentials and the products
+// would each take alone.  32 / 8 heads of 128, bf16: a prompt of 8192 tokens 495 us (1110 TFLOP/s, 0.66 of the measured burst), 512 tokens behind 16383 cached
+// ones 143 us (970), in 4 bits 182 us; heads of 64: 114 us (610 TFLOP/s: as many exponentials for half the products).  64 tokens alone: 12 us, of which
+// 7 before the first product (launch, the line, the first segment, queries).
 #pragma once
 #include "skn_paged_attn.cuh"
 
 constexpr int PP_ROWS = 256, PP_KEYS = 128;
-constexpr int PP_COST = 4;        // units that a block's start and end are worth on the line
+// units that a block's start and end are worth on the line (2: a prompt of 8192 tokens 705 us, 3: 593, 4: 512, 6: 507, 9: 519; 16 of 1024: 331, 310, 298, 309, 312)
+constexpr int PP_COST = 4;
 
 template <class CT, int D> struct PpTraits {
     static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
@@ -27,8 +35,9 @@ template <class CT, int D> struct PpTraits {
     static constexpr int HALF = (16 * (D / 2 + D / 16) + 127) / 128 * 128;
     static constexpr int RAW = Q4 ? 8 * HALF : 0, RAW_SLOTS = Q4 ? 4 : 0;
     static constexpr size_t SMEM = 1024 + 2 * TILE + (size_t)SLOTS * TILE + (size_t)RAW_SLOTS * RAW;
-    static constexpr int SLACK = 4;
-    static constexpr float LIFT = BF ? 0.f : 11.f;                // exponent: fp16 weights up to 2^15 (see skn_paged_attn.cuh)
+    // (a prompt of 8192 tokens: SLACK 0 561 us, 2 530, 4 505, 8 495)
+    static constexpr int SLACK = 8;
+    static constexpr float LIFT = BF ? 0.f : 7.f;                 // exponent: fp16 weights up to 2^15, so that one of 2^-31 of its row's largest is the last one there
     // registers a thread of the softmax warpgroups, of the MMA / TMA / clearing warpgroup and of the unpacking one: at most the launch's, 384 x 168 or 512 x 128
     static constexpr int REGS_SOFT = Q4 ? 184 : 208, REGS_MMA = Q4 ? 64 : 80, REGS_UNPACK = 80;
     static_assert(128 * (2 * REGS_SOFT + REGS_MMA + (Q4 ? REGS_UNPACK : 0)) <= THREADS * (Q4 ? 128 : 168), "more than the launch has");

@@ -148,7 +148,7 @@ class PagedKVCache:
         return stride[0] if n > 1 else heads * D
 
     def append_dev(self, batch: PagedBatch, k, v, q=None, q_out=None):
-        """rows may be parts of wider ones (a joint projection); q_out may be q"""
+        """rows may be parts of wider ones (a joint projection); q_out is q or lies elsewhere; its rows of nobody and padded rows stay as they are"""
         io, n, kv, dt, row = _io_of(k), batch.n_tokens, self.n_kv_heads, k.dtype, self._row_stride
         if batch.device != self.ctx.device:
             raise ValueError("the step's tensors are on the context's device and of one type")
@@ -174,7 +174,7 @@ class PagedKVCache:
             _raise(self.ctx.handle, rc)
 
     def attend_dev(self, batch: PagedBatch, q, out, scale: Optional[float] = None, window: int = 0, sinks: int = 0):
-        """out lies beside q, not over it"""
+        """q [n_tokens, n_q_heads, head_dim] (rotated) -> out, which may lie beside q in wider rows, but not over it; rows of nobody stay as they are"""
         io, n, heads, row = _io_of(q), batch.n_tokens, q.shape[1], self._row_stride
         if batch.device != self.ctx.device:
             raise ValueError("the step's tensors are on the context's device and of one type")

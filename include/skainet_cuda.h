@@ -375,7 +375,7 @@ typedef struct skn_paged_batch {
 /* bytes of one pool of this specification (host arithmetic; the message of a refusal is read with skn_last_error(NULL)) */
 int32_t skn_paged_pool_bytes(const skn_paged_spec *spec, int64_t *bytes);
 /* k_pool_dev, v_pool_dev: device memory of skn_paged_pool_bytes bytes each, 16-byte aligned, that outlives the cache; or both NULL: the
- * cache allocates them, filled with zeros.  The workspace of attention (47 MB on a GPU of 148 SMs for head_dim 128, 25 MB for 64) is allocated here, so
+ * cache allocates them, filled with zeros.  The workspace of attention (45 MB on a GPU of 148 SMs for head_dim 128, 23 MB for 64) is allocated here, so
  * every `_dev` call below can be captured into a CUDA graph; calls on one cache share it and have to be ordered on the device (one stream, or
  * events).  n_pages * n_kv_heads * page_tokens is at most 2^31 - 1. */
 int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_dev, void *v_pool_dev, skn_paged **out);

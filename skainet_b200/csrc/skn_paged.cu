@@ -462,7 +462,6 @@ int32_t skn_paged_destroy(skn_paged *pc) {
     if (pc->d_turns) cudaFree(pc->d_turns);
     if (pc->d_parts) cudaFree(pc->d_parts);
     if (pc->d_tickets) cudaFree(pc->d_tickets);
-    if (pc->d_again) cudaFree(pc->d_again);
     pc->magic = 0;
     delete pc;
     return SKN_OK;

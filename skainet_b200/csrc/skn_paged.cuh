@@ -26,7 +26,6 @@ struct skn_paged {
     float *d_parts;              // prompts: blocks of rows of two segments per SM; then (from prompt_parts on) decoding, two per CTA: [rows of a CTA's segment][head_dim + 4]:
     int64_t prompt_parts;        // output, maximum, sum
     unsigned *d_tickets;         // [2][2 n_parts], zero between launches
-    uint8_t *d_again;            // prompts: a PagedScratch per SM
 };
 constexpr int SKN_PAGED_PART_ROWS = 32;
 

@@ -43,11 +43,10 @@ cudaError_t skn_paged_attn_prepare(skn_paged *pc) {
     }
     pc->n_parts = 4 * pc->ctx->sm_count;
     const size_t row = (D + 4) * sizeof(float), decode_rows = (size_t)2 * pc->ctx->sm_count * SKN_PAGED_PART_ROWS, prompt_rows = (size_t)2 * pc->ctx->sm_count * PP_ROWS;
-    const size_t tickets = (size_t)4 * pc->n_parts * sizeof(unsigned), again = D == 64 ? sizeof(PagedScratch<64, 256>) : sizeof(PagedScratch<128, 256>);
+    const size_t tickets = (size_t)4 * pc->n_parts * sizeof(unsigned);
     pc->prompt_parts = (int64_t)(prompt_rows * (D + 4));
     if (e == cudaSuccess) e = cudaMalloc((void **)&pc->d_parts, (decode_rows + prompt_rows) * row);
     if (e == cudaSuccess) e = cudaMalloc((void **)&pc->d_tickets, tickets);
-    if (e == cudaSuccess) e = cudaMalloc((void **)&pc->d_again, again * pc->ctx->sm_count);
     if (e == cudaSuccess) e = cudaMemsetAsync(pc->d_tickets, 0, tickets, pc->ctx->stream);
     return e;
 }
@@ -63,7 +62,6 @@ int32_t skn_paged_attn_launch(skn_paged *pc, const skn_paged_batch *batch, int32
     // a window that reaches back over any table's tokens is none
     p.window = window >= (int64_t)batch->max_pages * pc->spec.page_tokens ? 0 : window;
     p.sinks = p.window ? sinks : 0;
-    p.scratch = pc->d_again;
     p.scale = scale * 1.4426950408889634f;
     p.parts = pc->d_parts;
     p.tickets = pc->d_tickets;

@@ -118,7 +118,6 @@ struct PagedAttn {
     int direct;                   // a CTA per segment: no sharing (rows in blocks of 8 NB)
     int above, upto;              // sequences of other numbers of rows (tokens x group) are left to another launch
     int split;                    // ... which follows this one, or is this one: it begins while that one ends
-    void *scratch;                // prompts: a PagedScratch for each CTA
     float *parts;
     unsigned *tickets;
 };
@@ -166,12 +165,13 @@ __device__ __forceinline__ int paged_slot(const PagedSegment &g, int cta) { retu
 
 // A segment from the definition, eight rows at a time: a thread per key for the scores, then a thread per dimension (and part of the keys) for the outputs
 // (THREADS of them, which `bar` brings together).  put(row, maximum (base 2), sum, this thread's dimension of the unnormalised output).
-// Eight rows share every load: a block of 256 rows that other roles of its CTA wait for is through its keys at some 15 us per thousand.
+// Eight rows share every load.  256 rows take 3.3 us a key: from 600 thousand keys of one CTA on the waits of the others of its warps (two seconds each) run out and
+// are reported.
 constexpr int PA_REDO = 8;
-template <int D, int THREADS> struct PagedScratch {
+template <int D, int THREADS> struct alignas(16) PagedScratch {
     float q[D][PA_REDO], w[THREADS][PA_REDO], red[THREADS / 32][PA_REDO];
     int page[THREADS];
-    uint8_t seen[THREADS];                               // a bit per row
+    uint8_t row[THREADS], seen[THREADS];                 // of its page; a bit per row of queries
 };
 template <class CT, int D, int THREADS, class IO, class Bar, class Put>
 __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &g, int unit, PagedScratch<D, THREADS> &sc, Bar bar, Put put) {
@@ -205,18 +205,23 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
                 const int page = paged_page(p.st, g.seq, key), row = key & ((1 << p.st.page_shift) - 1);
                 if (page >= 0) {
                     const CT *at = reinterpret_cast<const CT *>(p.k_pool + paged_at(p.st, page, g.head));
+#pragma unroll 4
                     for (int c = 0; c < D / 8; ++c) {
                         float x[8], y[PA_REDO] = {};
                         paged_load8<D>(at, p.st.page_shift, row, c, x);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
+                        for (int e = 0; e < 8; ++e) {
+                            float qs[PA_REDO];
+                            io_load8(sc.q[8 * c + e], qs);
 #pragma unroll
-                            for (int k = 0; k < PA_REDO; ++k) y[k] = fmaf(x[e], sc.q[8 * c + e][k], y[k]);
+                            for (int k = 0; k < PA_REDO; ++k) y[k] = fmaf(x[e], qs[k], y[k]);
+                        }
 #pragma unroll
                         for (int k = 0; k < PA_REDO; ++k) z[k] += y[k];
                     }
                 } else seen = 0;
                 sc.page[tid] = page;
+                sc.row[tid] = (uint8_t)row;
             }
             sc.seen[tid] = (uint8_t)seen;
 #pragma unroll
@@ -255,15 +260,26 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
                 for (int w = 0; w < THREADS / 32; ++w) l[k] += sc.red[w][k];
             }
             const int end = min(THREADS, g.u1 * unit - b);
-#pragma unroll 4
-            for (int j = tid / D; j < end; j += THREADS / D) {
-                const uint32_t which = sc.seen[j];       // a row of V that is hidden is not touched
-                const float v = which ? paged_load1<D>(reinterpret_cast<const CT *>(p.v_pool + paged_at(p.st, sc.page[j], g.head)), p.st.page_shift,
-                                                       key_of(b + j) & ((1 << p.st.page_shift) - 1), dim)
-                                      : 0.f;
+            for (int j0 = tid / D; j0 < end; j0 += 8 * (THREADS / D)) {      // eight rows of V on their way at once; one that is hidden is not touched
+                uint32_t which[8];
+                float v[8];
 #pragma unroll
-                for (int k = 0; k < PA_REDO; ++k)
-                    if (which >> k & 1) acc[k] = fmaf(sc.w[j][k], v, acc[k]);
+                for (int e = 0; e < 8; ++e) {
+                    const int j = j0 + e * (THREADS / D);
+                    which[e] = j < end ? sc.seen[j] : 0;
+                    v[e] = 0.f;
+                    if (which[e])
+                        v[e] = paged_load1<D>(reinterpret_cast<const CT *>(p.v_pool + paged_at(p.st, sc.page[j], g.head)), p.st.page_shift, sc.row[j], dim);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (!which[e]) continue;
+                    float ws[PA_REDO];
+                    io_load8(sc.w[j0 + e * (THREADS / D)], ws);
+#pragma unroll
+                    for (int k = 0; k < PA_REDO; ++k)
+                        if (which[e] >> k & 1) acc[k] = fmaf(ws[k], v[e], acc[k]);
+                }
             }
             bar();
         }
@@ -318,7 +334,7 @@ template <class CT, int D, int NB, bool EX> struct PaTraits {
     static constexpr int BODY = (RING > COMB ? RING : COMB);
     static constexpr int Q_BYTES = Q_SMEM ? NT * NB * KS * 32 * 8 : 0;
     static constexpr size_t SMEM = 1024 + BODY + Q_BYTES;
-    static_assert(ROWS * (D + 4) * 4 + sizeof(PagedScratch<D, THREADS>) <= BODY, "what a segment is computed again in lies over the ring too");
+    static_assert(ROWS * (D + 4) * 4 % 16 == 0 && ROWS * (D + 4) * 4 + sizeof(PagedScratch<D, THREADS>) <= BODY, "what a segment is computed again in lies over the ring too");
 };
 
 template <class CT, int D, int NB, bool EX>

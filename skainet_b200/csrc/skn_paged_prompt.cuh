@@ -201,6 +201,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     __shared__ uint32_t tmem_slot;
     __shared__ unsigned ticket;
     __shared__ int starts[THREADS + 1];
+    __shared__ PagedScratch<D, 256> scratch;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedStep &st = p.st;
 
@@ -523,7 +524,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             if (pp_any(!got)) more = false;
             if (pp_any(odd)) {
                 const PagedSegment again = now;      // (a copy: the address of the one that the loops use is not taken)
-                paged_redo<CT, D, 256, IO>(p, again, PP_KEYS, static_cast<PagedScratch<D, 256> *>(p.scratch)[blockIdx.x], [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
+                paged_redo<CT, D, 256, IO>(p, again, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
                     const int tr = (now.row0 + row) / p.group;
                     if (shared) {
                         if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;

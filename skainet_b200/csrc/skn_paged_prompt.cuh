@@ -104,8 +104,8 @@ __device__ __forceinline__ float pp_max3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// 2^x of two values, on the special-function units.  (16 a clock and SM take as long as the products do; but the warps are short of issue slots first:
-// three in eight by FMAs instead, a cubic in the fraction, 548 -> 606 us for a prompt of 8192 tokens.)
+// 2^x of two values, on the special-function units.  (16 a clock and SM take as long as the products do, but neither is busy for more than half of the time: one in
+// eight by a cubic in the fraction instead 534 -> 536 us for a prompt of 8192 tokens, three in eight 623.)
 __device__ __forceinline__ uint64_t pp_ex2_pair(uint64_t x) {
     float a, b;
     skn_unpack2(x, a, b);

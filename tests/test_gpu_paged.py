@@ -794,3 +794,40 @@ def test_two_contexts_at_once(ctx):
         assert torch.equal(out, first)
         cache.close()
     other.close()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "q4_0"])
+@pytest.mark.parametrize("group,window", [(3, 0), (8, 60), (12, 0), (40, 0)])
+def test_steps_of_prompts_and_single_tokens(ctx, io, dtype, group, window):
+    """in one step: prompts, portions of prompts, single tokens, sequences without a row, padded ones"""
+    kv, dim = 2, 64
+    step = Step(2, [50, 700, 3, 9, 260, 120, 2, 30], [50, 1, 3, 0, 1, 12, 4, 2], 16, padding=2)
+    cache, ref = filled(ctx, step, kv, dim, dtype, 3)
+    g = np.random.default_rng(group)
+    k, v = (g.standard_normal((step.n, kv, dim)).astype(np.float32) for _ in range(2))
+    q = bf16(g.standard_normal((step.n, kv * group, dim)))
+    cache.append(k, v, step.table, step.starts, step.lens)
+    ref.append(k, v, step.table, step.starts, step.lens)
+    given = bf16(g.standard_normal(q.shape))
+    want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125, window, 2, given=given)
+    out = run_attend(cache, step, q, io, given=given, window=window, sinks=2)
+    n = int(step.starts[-1])
+    assert np.array_equal(out[n:], given[n:])
+    check(out[:n], want[:n], mass[:n], reach[:n], io, dtype, True)
+    cache.close()
+
+
+def test_calls_without_their_parts(ctx):
+    step = Step(3, [40], [2], 16)
+    cache, _ = filled(ctx, step, 2, 64, "bf16", 3)
+    k = torch.zeros(2, 2, 64, device="cuda", dtype=torch.bfloat16)
+    q = torch.zeros(2, 4, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="q_out"):
+        cache.append_dev(step.batch(), k, k, q)
+    wide = skn.PagedBatch(torch.zeros(1, 2 ** 23 + 1, dtype=torch.int32, device="cuda"), torch.tensor([0, 2], dtype=torch.int32, device="cuda"),
+                          torch.tensor([2], dtype=torch.int32, device="cuda"), 2, 2)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="pages"):
+        cache.attend_dev(wide, q, torch.zeros_like(q))
+    cache.close()

@@ -17,7 +17,7 @@
 //
 // Bound by the chain of a tile (scores, softmax, products, each waiting for the one before) at about half of what the exponentials and the products
 // would each take alone.  32 / 8 heads of 128, bf16: a prompt of 8192 tokens 495 us (1110 TFLOP/s, 0.66 of the measured burst), 512 tokens behind 16383 cached
-// ones 143 us (970), in 4 bits 182 us; heads of 64: 114 us (610 TFLOP/s: as many exponentials for half the products).  64 tokens alone: 12 us, of which
+// ones 143 us (970), in 4 bits 182 us; heads of 64: 114 us (610 TFLOP/s: as many exponentials for half the products).  64 tokens alone: 15 us, of which
 // 7 before the first product (launch, the line, the first segment, queries).
 #pragma once
 #include "skn_paged_attn.cuh"

@@ -399,7 +399,7 @@ int32_t skn_paged_gather_dev(skn_paged *pc, const skn_paged_batch *batch, int32_
  * visible has no influence, whatever it holds.  At most 64 query heads per kv head; out may not lie over q (rows side by side in
  * wider ones are fine).  fp32 rows: fp32 accuracy.  bf16 rows: queries exact (down to 2^-38 of a row's largest), softmax weights rounded to fp16 (bf16
  * caches: bf16), fp32 sums; in a step whose max_new times the query heads per kv head is above 32, the dequantised rows of a Q4_0 cache may be
- * rounded to fp16 as well. */
+ * rounded to fp16 as well (rows that see a block with a value above 65504 are computed in fp32 instead, at about a hundredth of the speed). */
 int32_t skn_paged_attn(skn_paged *pc, const skn_paged_batch *batch, const float *q_host, int32_t n_q_heads, float scale, int32_t window,
                        int32_t sinks, float *out_host);
 int32_t skn_paged_attn_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, const void *q_dev, int64_t q_stride, int32_t n_q_heads,

@@ -13,7 +13,9 @@
 // held its state in registers, which the softmax warps had to spill: 544 -> 512 us).
 //
 // Hidden rows of V (behind the last key that the block sees, before its window, on pages that were given back) are cleared in shared memory before the
-// product: a warp does it in the few units that have some.  A result that is not finite is computed again from the definition.
+// product: a warp does it in the few units that have some.  A result that is not finite is computed again from the definition.  Q4_0: fp16 holds
+// (q - 8) d up to 65504, so |d| below 2^13.  A larger one would leave minus infinity for some scores, which looks like a hidden key's, so blocks with such a scale become NaN:
+// whoever sees them is computed again.
 //
 // Bound by the chain of a tile (scores, softmax, products, each waiting for the one before) at about half of what the exponentials and the products
 // would each take alone.  32 / 8 heads of 128, bf16: a prompt of 8192 tokens 495 us (1110 TFLOP/s, 0.66 of the measured burst), 512 tokens behind 16383 cached
@@ -812,7 +814,9 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
 #pragma unroll
                     for (int b = 0; b < NBLK; ++b) {
                         uint4 u = need ? *reinterpret_cast<const uint4 *>(src + (((b << box_shift) + in) << 4)) : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-                        const __half d = need ? *reinterpret_cast<const __half *>(src + (D / 2 << box_shift) + (in * NBLK + b) * 2) : __float2half_rn(0.f);
+                        __half_raw dr = {need ? *reinterpret_cast<const unsigned short *>(src + (D / 2 << box_shift) + (in * NBLK + b) * 2) : (unsigned short)0};
+                        if ((dr.x & 0x7000) == 0x7000) dr.x = 0x7FFF;        // from 2^13 on: see the head of this file
+                        const __half d = dr;
                         const __half2 d2 = __half2half2(d), off = __float2half2_rn(-1032.f);
                         const uint32_t ws[4] = {u.x, u.y, u.z, u.w};
                         uint32_t h[16];

@@ -1,0 +1,44 @@
+"""Paged KV cache on the GPU: values, steps and calls at the edges of what it takes, against the oracle in 64 bits (tolerances as in
+test_gpu_paged.py)."""
+import numpy as np
+import pytest
+import torch
+
+import skainet_b200 as skn
+from oracle import paged as oracle
+from test_gpu_paged import Step, bf16, run_attend, tolerance
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,news", [([300], [40]), ([300, 70], [1, 1]), ([2100, 40], [33, 20]), ([260], [260])])
+def test_keys_beyond_fp16_in_4_bits(ctx, io, dim, lens, news):
+    """A 4-bit block holds values up to 8 x 65504.  One dimension of every key is 1e5, of which queries of either sign (and of none) make scores of +-1e4; then
+    keys whose value beyond fp16 meets another one that brings the score back.  Every row's block is computed in fp32: no term for rows in fp16.  (No bound
+    on the norm: a score of 1e4 in fp32 is a multiple of 2^-10, by which a weight is off.)"""
+    kv, group, page = 2, 4, 32
+    for kind in range(2):
+        step = Step(5, lens, news, page)
+        cache = skn.PagedKVCache(ctx, step.n_pages, page, kv, dim, "q4_0")
+        ref = oracle.Pages(step.n_pages, page, kv, dim, "q4_0")
+        g = np.random.default_rng(dim + kind)
+        total = int(step.lens.sum())
+        k, v = (g.standard_normal((total, kv, dim)).astype(np.float32) for _ in range(2))
+        q = bf16(g.standard_normal((step.n, kv * group, dim)))
+        if kind == 0:
+            k[:, :, 5] = 1e5
+            q[:, :, 5] = np.array([-1, 1, -0.5, 0])[np.arange(kv * group) % 4]
+        else:                                              # -7e4 + 6e4 or -1e4
+            k[:, :, 5], k[:, :, 40] = 0, -1e4
+            k[::2, :, 5], k[::2, :, 40] = 7e4, 6e4
+            q[:, :, 5], q[:, :, 40] = -1, 1
+        cache.append(k, v, step.table, step.full, step.lens)
+        ref.append(k, v, step.table, step.full, step.lens)
+        want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+        assert np.isfinite(want).all() and np.abs(want).max() > 0.1
+        err = np.abs(run_attend(cache, step, q, io, scale=0.125) - want)
+        tol = tolerance(want, mass, reach, 0.0 if io == "f32" else 2.0 ** -11, 0.0, io)
+        assert np.all(err <= tol), f"largest excess {np.max(err / tol):.3g} at {np.unravel_index(np.argmax(err / tol), err.shape)}"
+        cache.close()

@@ -302,7 +302,9 @@ __device__ __noinline__ void paged_redo(const PagedAttn &p, const PagedSegment &
 template <class IO> __device__ __forceinline__ void paged_out4(const PagedAttn &p, const PagedSegment &g, int r, int d, int dims, float4 x, float sum) {
     const int t = (g.row0 + r) / p.group;
     IO *to = static_cast<IO *>(p.out) + (int64_t)(g.first + t) * p.out_stride + (g.head * p.group + (g.row0 + r) % p.group) * dims + d;
-    if (sum == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
+    // (no weight: zero for a row that sees nothing; a row at a position sees itself, so all of its scores were minus infinity, and 0 / 0 is NaN)
+    if (sum == 0.f && g.len - g.n + t < 0) x = make_float4(0.f, 0.f, 0.f, 0.f);
+    else if (sum == 0.f) x = make_float4(NAN, NAN, NAN, NAN);
     else x = make_float4(x.x / sum, x.y / sum, x.z / sum, x.w / sum);
     if constexpr (sizeof(IO) == 4) *reinterpret_cast<float4 *>(to) = x;
     else *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));

@@ -489,7 +489,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 if (ok) ok = tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane);
                 if (!(ok && got) && lane == 0) *st.status = SKN_ERR_TIMEOUT;
                 tc_fence_after();
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = 1.f / l;
+                const uint32_t none = now.len - now.n + t < 0 ? 0u : 0x7FFF7FFFu;      // without a weight: zero where nothing is seen, NaN where all scores were minus infinity
 #pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     float o[32];
@@ -510,7 +511,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     } else {
                         uint32_t y[16];
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) y[k] = l == 0.f ? 0u : pack_bf16(o[2 * k] * inv, o[2 * k + 1] * inv);
+                        for (int k = 0; k < 16; ++k) y[k] = l == 0.f ? none : pack_bf16(o[2 * k] * inv, o[2 * k + 1] * inv);
                         if (real) {
 #pragma unroll
                             for (int k = 0; k < 16; k += 8) pp_store32(out + c + 2 * k, y + k, wide);
@@ -536,7 +537,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         }
                     } else if (tid < D)
                         static_cast<IO *>(p.out)[(int64_t)(now.first + tr) * p.out_stride + (now.head * p.group + (now.row0 + row) % p.group) * D + tid] =
-                            __float2bfloat16_rn(rl == 0.f ? 0.f : acc / rl);
+                            __float2bfloat16_rn(rl != 0.f ? acc / rl : now.len - now.n + tr < 0 ? 0.f : NAN);
                 });
             }
             if (shared) {
@@ -550,7 +551,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     float top = PA_NONE, sum = 0.f;
                     for (int k = 0; k < now.n_parts; ++k) top = fmaxf(top, __ldcg(part_of(k) + D * PP_ROWS + R));
                     for (int k = 0; k < now.n_parts; ++k) sum = fmaf(__ldcg(part_of(k) + (D + 1) * PP_ROWS + R), exp2f(__ldcg(part_of(k) + D * PP_ROWS + R) - top), sum);
-                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    const float inv = 1.f / sum;
+                    const uint32_t none = now.len - now.n + t < 0 ? 0u : 0x7FFF7FFFu;
 #pragma unroll 1
                     for (int c = 0; c < D; c += 16) {
                         float4 o[4] = {};
@@ -575,8 +577,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         uint32_t y[8];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            y[2 * e] = pack_bf16(o[e].x * inv, o[e].y * inv);
-                            y[2 * e + 1] = pack_bf16(o[e].z * inv, o[e].w * inv);
+                            y[2 * e] = sum == 0.f ? none : pack_bf16(o[e].x * inv, o[e].y * inv);
+                            y[2 * e + 1] = sum == 0.f ? none : pack_bf16(o[e].z * inv, o[e].w * inv);
                         }
                         pp_store32(out + c, y, wide);
                     }

@@ -6,7 +6,7 @@ import torch
 
 import skainet_b200 as skn
 from oracle import paged as oracle
-from test_gpu_paged import Step, bf16, run_attend, tolerance
+from test_gpu_paged import Step, bf16, check, filled, run_attend, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,32 @@ def test_keys_beyond_fp16_in_4_bits(ctx, io, dim, lens, news):
         tol = tolerance(want, mass, reach, 0.0 if io == "f32" else 2.0 ** -11, 0.0, io)
         assert np.all(err <= tol), f"largest excess {np.max(err / tol):.3g} at {np.unravel_index(np.argmax(err / tol), err.shape)}"
         cache.close()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lens,news,some", [([40], [40], 10), ([70, 20], [1, 1], 70), ([3000], [60], 3000), ([3000, 5], [60, 1], 2970), ([9, 300], [12, 40], 6)])
+def test_scores_of_minus_infinity(ctx, io, dtype, lens, news, some):
+    """The first `some` keys hold minus infinity in one dimension: with a positive query their weights are zero, and 0 / 0 where all visible ones are such.
+    Rows at negative positions see nothing and are zero; with a query of the other sign (or of none) everything is NaN."""
+    kv, group, dim, page = 1, 4, 64, 16
+    step = Step(5, lens, news, page)
+    cache, ref = filled(ctx, step, kv, dim, dtype, 3)
+    g = np.random.default_rng(7)
+    n = int(np.maximum(step.lens, 0).sum())
+    k, v = (g.standard_normal((n, kv, dim)).astype(np.float32) for _ in range(2))
+    at = np.concatenate([np.arange(int(x)) for x in step.lens])
+    k[at < some, 0, 3] = -np.inf
+    q = bf16(g.standard_normal((step.n, kv * group, dim)))
+    q[:, :, 3] = np.array([1, 2, -1, 0.25])
+    cache.append(k, v, step.table, step.full, step.lens)
+    ref.append(k, v, step.table, step.full, step.lens)
+    with np.errstate(invalid="ignore"):
+        want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    out = run_attend(cache, step, q, io, scale=0.125)
+    odd = np.isnan(want)
+    assert odd[:, 2].any() and np.array_equal(np.isnan(out), odd)
+    reach[..., 0] = np.where(np.isfinite(reach[..., 0]), reach[..., 0], 0.125 * 6 * dim)      # |k| and |q| below 6, a product a dimension: no more for keys with a weight
+    rows = ~odd.any(axis=2)
+    check(out[rows], want[rows], mass[rows], reach[rows], io, dtype, max(news) > 1)
+    cache.close()

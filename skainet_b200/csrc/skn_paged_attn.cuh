@@ -36,7 +36,7 @@
 // Sequences whose work is shared out (their places are in shared memory); more of them take a CTA per segment.  300 sequences: of 1000 tokens each 195 us
 // shared out, 183 as CTAs; of 500 and one of 32768 133 us against 447.
 constexpr int PA_MAX_SEQS = 512;
-constexpr float PA_NONE = -1e30f;            // running maximum before the first score
+constexpr float PA_NONE = -3.402823466e38f;  // running maximum before the first score: the lowest number, so that no score is below it
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"

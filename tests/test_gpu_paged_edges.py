@@ -71,3 +71,31 @@ def test_scores_of_minus_infinity(ctx, io, dtype, lens, news, some):
     rows = ~odd.any(axis=2)
     check(out[rows], want[rows], mass[rows], reach[rows], io, dtype, max(news) > 1)
     cache.close()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype,key,query", [("bf16", 2.0 ** 40, 2.0 ** 75), ("f16", 2.0 ** 10, 2.0 ** 105), ("q4_0", 2.0 ** 10, 2.0 ** 105)])
+@pytest.mark.parametrize("lens,news", [([60], [1]), ([60, 30], [40, 1]), ([5000], [50]), ([5000, 9], [1, 1])])
+def test_scores_far_below_zero(ctx, io, dtype, key, query, lens, news):
+    """scores of about -1e33 and less, distances as large: every row is the value of the key that is least far below, which is drawn anew every 50 tokens"""
+    kv, group, dim, page = 2, 4, 64, 16
+    step = Step(5, lens, news, page)
+    cache = skn.PagedKVCache(ctx, step.n_pages, page, kv, dim, dtype)
+    ref = oracle.Pages(step.n_pages, page, kv, dim, dtype)
+    g = np.random.default_rng(3)
+    total = int(step.lens.sum())
+    k = np.zeros((total, kv, dim), dtype=np.float32)
+    at = np.concatenate([np.arange(int(x)) for x in step.lens])
+    k[:, :, 0] = key * (1 + ((at * 29 + 11) % 50)[:, None] / 64)                     # exact in every type
+    k[at >= 50, :, 0] = key * 2                                                       # ... and twice as far from the 50th on
+    v = g.standard_normal((total, kv, dim)).astype(np.float32)
+    q = np.zeros((step.n, kv * group, dim), dtype=np.float32)
+    q[:, :, 0] = -query
+    cache.append(k, v, step.table, step.full, step.lens)
+    ref.append(k, v, step.table, step.full, step.lens)
+    want, _, _ = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    assert np.abs(want).max() > 1
+    out = run_attend(cache, step, q, io, scale=0.125)
+    # one weight of one: an output is the value itself, rounded (bf16 rows) or summed and divided in fp32
+    assert np.all(np.abs(out - want) <= (2.0 ** -8 if io == "bf16" else 2.0 ** -20) * np.abs(want))
+    cache.close()

@@ -281,6 +281,11 @@ static int32_t check_heads(skn_ctx *ctx, const skn_paged *pc, int32_t n_q_heads)
     if (n_q_heads / pc->spec.n_kv_heads > 64) return skn_fail(ctx, SKN_ERR_SHAPE, "%d query heads per kv head; 64 at most", n_q_heads / pc->spec.n_kv_heads);
     return SKN_OK;
 }
+static int32_t check_mask(skn_ctx *ctx, float scale, int32_t window, int32_t sinks) {
+    if (window < 0 || sinks < 0) return skn_fail(ctx, SKN_ERR_ARG, "negative window or sinks");
+    if (!isfinite(scale * PAGED_LOG2E)) return skn_fail(ctx, SKN_ERR_ARG, "a scale of %g: times log2(e) it is no number", scale);
+    return SKN_OK;
+}
 static int32_t check_io(skn_ctx *ctx, int32_t io) {
     if (io != SKN_KV_F32 && io != SKN_KV_BF16) return skn_fail(ctx, SKN_ERR_TYPE, "rows are fp32 or bf16, not element type %d", io);
     return SKN_OK;
@@ -561,7 +566,7 @@ int32_t skn_paged_attn_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t 
     bool nothing;
     int32_t rc = check_io(ctx, io);
     if (rc || (rc = check_batch(ctx, batch, &nothing)) || (rc = check_heads(ctx, pc, n_q_heads))) return rc;
-    if (window < 0 || sinks < 0 || !isfinite(scale)) return skn_fail(ctx, SKN_ERR_ARG, "negative window or sinks, or a scale that is no number");
+    if ((rc = check_mask(ctx, scale, window, sinks))) return rc;
     if (nothing) return SKN_OK;
     const int64_t wq = (int64_t)n_q_heads * pc->spec.head_dim;
     if ((rc = check_rows(ctx, "q", q_dev, q_stride, wq, io)) || (rc = check_rows(ctx, "out", out_dev, out_stride, wq, io))) return rc;
@@ -584,7 +589,7 @@ int32_t skn_paged_attn(skn_paged *pc, const skn_paged_batch *batch, const float 
     bool nothing;
     int32_t rc = enter_host(pc, batch, &nothing);
     if (rc || (rc = check_heads(ctx, pc, n_q_heads))) return rc;
-    if (window < 0 || sinks < 0 || !isfinite(scale)) return skn_fail(ctx, SKN_ERR_ARG, "negative window or sinks, or a scale that is no number");
+    if ((rc = check_mask(ctx, scale, window, sinks))) return rc;
     if (nothing) return SKN_OK;
     if (!q_host || !out_host) return skn_fail(ctx, SKN_ERR_ARG, "NULL argument");
     if ((rc = check_tables(pc, batch, NEED_SEEN, window, sinks, false)) || batch->max_new == 0) return rc;

@@ -28,6 +28,7 @@ struct skn_paged {
     unsigned *d_tickets;         // [2][2 n_parts], zero between launches
 };
 constexpr int SKN_PAGED_PART_ROWS = 32;
+constexpr float PAGED_LOG2E = 1.4426950408889634f;        // scores are formed in base 2
 
 // A step as the kernels see it
 struct PagedStep {

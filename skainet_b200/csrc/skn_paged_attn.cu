@@ -62,7 +62,7 @@ int32_t skn_paged_attn_launch(skn_paged *pc, const skn_paged_batch *batch, int32
     // a window that reaches back over any table's tokens is none
     p.window = window >= (int64_t)batch->max_pages * pc->spec.page_tokens ? 0 : window;
     p.sinks = p.window ? sinks : 0;
-    p.scale = scale * 1.4426950408889634f;
+    p.scale = scale * PAGED_LOG2E;
     p.parts = pc->d_parts;
     p.tickets = pc->d_tickets;
     SKN_CUDA(pc->ctx, pc->spec.kv_dtype == SKN_KV_F16    ? skn_paged_attn_f16(pc, io, p)

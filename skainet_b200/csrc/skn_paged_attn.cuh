@@ -597,6 +597,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
             for (int c = 0; c < 2; ++c) {
                 const int src = 4 * (2 * t4 + c);
                 cs[nb][c] = __shfl_sync(0xffffffffu, f, src);
+                if (!(fabsf(cs[nb][c]) < INFINITY)) flags[0] = 1;       // scores of minus infinity would look like hidden keys': the segment is computed again
                 const int rc = 8 * nb + 2 * t4 + c;
                 pos[nb][c] = rc < g.rows ? g.len - g.n + (g.row0 + rc) / p.group : -1;
                 if constexpr (T::Q4) {

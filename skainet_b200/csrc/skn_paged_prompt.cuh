@@ -400,7 +400,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             const bool real = R < now.rows, used = tile * 128 < now.rows;
             const int t = (now.row0 + R) / p.group, pos = real ? now.len - now.n + t : -1;
             const float cs = cs_next;
-            float m = PA_NONE, l = 0.f;
+            float m = PA_NONE, l = cs < INFINITY ? 0.f : cs - cs;        // (a factor beyond fp32 makes scores of minus infinity, as of hidden keys: computed again)
             if (used && ok) {
                 const int ta = (now.row0 + tile * 128) / p.group, tb = (now.row0 + min(tile * 128 + 127, now.rows - 1)) / p.group;
                 const int pmin = now.len - now.n + ta, pmax = now.len - now.n + tb;

@@ -99,3 +99,42 @@ def test_scores_far_below_zero(ctx, io, dtype, key, query, lens, news):
     # one weight of one: an output is the value itself, rounded (bf16 rows) or summed and divided in fp32
     assert np.all(np.abs(out - want) <= (2.0 ** -8 if io == "bf16" else 2.0 ** -20) * np.abs(want))
     cache.close()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,news", [([60], [1]), ([60, 30], [40, 1]), ([3000, 9], [1, 1])])
+def test_queries_near_the_largest_number(ctx, io, lens, news):
+    """queries of -2^122 and 4-bit keys of 2^-17: scores of -2^102, though the factor between the quants' products and the scores is more than fp32 holds"""
+    kv, group, dim, page = 2, 4, 64, 16
+    step = Step(5, lens, news, page)
+    cache = skn.PagedKVCache(ctx, step.n_pages, page, kv, dim, "q4_0")
+    ref = oracle.Pages(step.n_pages, page, kv, dim, "q4_0")
+    g = np.random.default_rng(3)
+    total = int(step.lens.sum())
+    k = np.zeros((total, kv, dim), dtype=np.float32)
+    at = np.concatenate([np.arange(int(x)) for x in step.lens])
+    k[:, :, 0] = 2.0 ** -21 * (16 + (at * 29 + 11) % 50 + 50 * (at >= 50))[:, None]      # 8 times a multiple of 2^-24
+    v = g.standard_normal((total, kv, dim)).astype(np.float32)
+    q = np.zeros((step.n, kv * group, dim), dtype=np.float32)
+    q[:, :, 0] = -2.0 ** 122
+    cache.append(k, v, step.table, step.full, step.lens)
+    ref.append(k, v, step.table, step.full, step.lens)
+    want, _, _ = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    assert np.abs(want).max() > 1
+    out = run_attend(cache, step, q, io, scale=0.125)
+    # fp32: distances between scores of 2^98 and more leave one weight of one; equal keys none twice among the nearest
+    assert np.all(np.abs(out - want) <= (2.0 ** -8 if io == "bf16" else 2.0 ** -20) * np.abs(want))
+    cache.close()
+
+
+def test_scales_beyond_fp32_are_refused(ctx):
+    """scores are formed in base 2: the scale times log2(e) is a number too"""
+    step = Step(3, [40], [2], 16)
+    cache, _ = filled(ctx, step, 2, 64, "bf16", 3)
+    q = torch.zeros(2, 4, 64, device="cuda", dtype=torch.bfloat16)
+    for scale in (3e38, -3e38, float("inf")):
+        with pytest.raises(skn.SknError, match="scale"):
+            cache.attend(np.zeros((2, 4, 64), dtype=np.float32), step.table, step.starts, step.lens, scale=scale)
+        with pytest.raises(skn.SknError, match="scale"):
+            cache.attend_dev(step.batch(), q, torch.zeros_like(q), scale=scale)
+    cache.close()

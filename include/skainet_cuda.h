@@ -396,10 +396,15 @@ int32_t skn_paged_gather(skn_paged *pc, const skn_paged_batch *batch, float *k_o
 int32_t skn_paged_gather_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, void *k_out_dev, void *v_out_dev);
 /* out = softmax(scale * q . K^T) . V of every row over the cached tokens at its own position and before: all of them (window 0), or the last
  * `window`, its own included, and the first `sinks` of the sequence.  Query head h reads kv head h / (n_q_heads / n_kv_heads).  What is not
- * visible has no influence, whatever it holds (a row that sees nothing is zero; one whose scores are all minus infinity is NaN).  At most 64 query heads per kv head; out may not lie over q (rows side by side in
- * wider ones are fine).  fp32 rows: fp32 accuracy.  bf16 rows: queries exact (down to 2^-38 of a row's largest), softmax weights rounded to fp16 (bf16
- * caches: bf16), fp32 sums; in a step whose max_new times the query heads per kv head is above 32, the dequantised rows of a Q4_0 cache may be
- * rounded to fp16 as well (rows that see a block with a value above 65504 are computed in fp32 instead, at about a hundredth of the speed). */
+ * visible has no influence, whatever it holds (a row that sees nothing is zero; one whose scores are all minus infinity is NaN).  At most 64 query
+ * heads per kv head; out may not lie over q (rows side by side in wider ones are fine).
+ *   fp32 rows: fp32 accuracy.
+ *   bf16 rows: softmax weights rounded to fp16 (bf16 caches: bf16, the type that their product takes), fp32 sums.  Queries meet fp16 caches in multiples of 2^-38 of a row's
+ *     largest, Q4_0 caches of 2^-34, bf16 caches as they are.  In a step whose max_new times the query heads per kv head is above 32, the
+ *     dequantised rows of a Q4_0 cache may be rounded to fp16 as well (rows that see a block with a value above 65504 are computed in fp32 instead,
+ *     at about a hundredth of the speed).
+ *   Q4_0 caches: weights are multiplied by the values' scales before they are rounded, so that a key's part in a dimension may miss 2^-32 (fp32 rows: 2^-37) of the row's
+ *     largest weight times the largest value seen in any dimension. */
 int32_t skn_paged_attn(skn_paged *pc, const skn_paged_batch *batch, const float *q_host, int32_t n_q_heads, float scale, int32_t window,
                        int32_t sinks, float *out_host);
 int32_t skn_paged_attn_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, const void *q_dev, int64_t q_stride, int32_t n_q_heads,

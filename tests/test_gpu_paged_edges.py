@@ -138,3 +138,56 @@ def test_scales_beyond_fp32_are_refused(ctx):
         with pytest.raises(skn.SknError, match="scale"):
             cache.attend_dev(step.batch(), q, torch.zeros_like(q), scale=scale)
     cache.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_queries_beside_a_large_one(ctx, dim):
+    """Single tokens over 4 bits: queries of bf16 rows are multiples of 2^-34 of the row's largest there (2^-38 over other caches).  The largest meets zeros, the
+    others, around 2^-33 of it, keys of 1e4."""
+    for dtype, step_of in (("q4_0", -34), ("f16", -38)):
+        step = Step(5, [200, 17], [1, 1], 32)
+        kv, group = 2, 4
+        cache = skn.PagedKVCache(ctx, step.n_pages, 32, kv, dim, dtype)
+        ref = oracle.Pages(step.n_pages, 32, kv, dim, dtype)
+        g = np.random.default_rng(dim)
+        total = int(step.lens.sum())
+        k, v = (g.standard_normal((total, kv, dim)).astype(np.float32) for _ in range(2))
+        k[:, :, :32] = 0
+        k *= 1e4
+        q = g.integers(-6, 7, (step.n, kv * group, dim)) * np.exp2(20.0 + step_of)
+        q[:, :, 0] = 2.0 ** 20
+        q = bf16(q)
+        cache.append(k, v, step.table, step.full, step.lens)
+        ref.append(k, v, step.table, step.full, step.lens)
+        want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+        check(run_attend(cache, step, q, "bf16", scale=0.125), want, mass, reach, "bf16", dtype, False)
+        cache.close()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+def test_values_of_unequal_blocks(ctx, io):
+    """4 bits, single tokens: values of the first 32 dimensions are 2^20 times the others'.  A key's part may miss 2^-32 (2^-37) of the largest weight times the largest
+    value beside what the weights' own rounding takes."""
+    kv, group, dim, page = 2, 4, 128, 32
+    step = Step(5, [300, 21], [1, 1], page)
+    cache = skn.PagedKVCache(ctx, step.n_pages, page, kv, dim, "q4_0")
+    ref = oracle.Pages(step.n_pages, page, kv, dim, "q4_0")
+    g = np.random.default_rng(2)
+    total = int(step.lens.sum())
+    k, v = (g.standard_normal((total, kv, dim)).astype(np.float32) for _ in range(2))
+    v[:, :, :32] *= 2.0 ** 10
+    v[:, :, 32:] *= 2.0 ** -10
+    q = bf16(g.standard_normal((step.n, kv * group, dim)))
+    cache.append(k, v, step.table, step.full, step.lens)
+    ref.append(k, v, step.table, step.full, step.lens)
+    want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    out = run_attend(cache, step, q, io, scale=0.125)
+    most = np.empty((step.n, kv * group, 1))               # each row's largest weight of a sum of one
+    for s in range(step.n):
+        for h in range(kv * group):
+            z = ref.rows("k", s, int(step.lens[s]), step.table)[h // group] @ q[s, h].astype(np.float64) * 0.125
+            most[s, h] = 1 / np.exp(z - z.max()).sum()
+    miss = step.lens[:, None, None] * most * np.abs(ref.v).max() * 2.0 ** (-37 if io == "f32" else -32)
+    tol = tolerance(want, mass, reach, 0.0 if io == "f32" else 2.0 ** -11, 0.0, io) + miss
+    assert np.all(np.abs(out - want) <= tol)
+    cache.close()

@@ -289,6 +289,7 @@ int32_t skn_status_check(skn_ctx *ctx) {
     const int32_t st = *ctx->h_status;
     if (st != 0) {
         cudaMemsetAsync(ctx->d_status, 0, sizeof(int32_t), ctx->stream);
+        if (st == SKN_ERR_TIMEOUT && ctx->after_timeout) ctx->after_timeout(ctx);
         cudaStreamSynchronize(ctx->stream);
         return skn_fail(ctx, st, "a kernel reported device-side status %d (%s)", st,
                         st == SKN_ERR_TIMEOUT ? "a bounded wait ran out"

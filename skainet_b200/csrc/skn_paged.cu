@@ -2,6 +2,7 @@
 #include "skn_paged.cuh"
 
 #include <math.h>
+#include <pthread.h>
 #include <new>
 
 // ---- append -------------------------------------------------------------------------------------------------------------
@@ -401,6 +402,35 @@ static int32_t enter_host(skn_paged *pc, const skn_paged_batch *b, bool *nothing
     return SKN_OK;
 }
 
+// ---- after a wait that ran out ------------------------------------------------------------------------------------------------------
+// A prompt kernel that gives up leaves some of its joins' counters above zero, and the next launch, a captured one too, would join too early.  So
+// the report of a timeout, which every caller gets before it can trust a result again, zeroes the counters of the context's caches.
+static pthread_mutex_t caches_lock = PTHREAD_MUTEX_INITIALIZER;
+static skn_paged *caches;
+static void tickets_back(skn_ctx *ctx) {
+    pthread_mutex_lock(&caches_lock);
+    cudaDeviceSynchronize();                            // (graphs may run on other streams than the context's)
+    for (skn_paged *pc = caches; pc; pc = pc->next)
+        if (pc->ctx == ctx) cudaMemsetAsync(pc->d_tickets, 0, paged_ticket_bytes(pc), ctx->stream);
+    pthread_mutex_unlock(&caches_lock);
+}
+static void caches_add(skn_paged *pc) {
+    pthread_mutex_lock(&caches_lock);
+    pc->next = caches;
+    caches = pc;
+    pthread_mutex_unlock(&caches_lock);
+    pc->ctx->after_timeout = tickets_back;
+}
+static void caches_remove(const skn_paged *pc) {
+    pthread_mutex_lock(&caches_lock);
+    for (skn_paged **at = &caches; *at; at = &(*at)->next)
+        if (*at == pc) {
+            *at = pc->next;
+            break;
+        }
+    pthread_mutex_unlock(&caches_lock);
+}
+
 extern "C" {
 
 int32_t skn_paged_pool_bytes(const skn_paged_spec *spec, int64_t *bytes) {
@@ -450,12 +480,14 @@ int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_
         skn_paged_destroy(pc);
         return skn_check_cuda(ctx, e, "paged cache allocation");
     }
+    caches_add(pc);
     *out = pc;
     return SKN_OK;
 }
 
 int32_t skn_paged_destroy(skn_paged *pc) {
     if (!pc || pc->magic != SKN_MAGIC_PAGED) return skn_fail(nullptr, SKN_ERR_BAD_HANDLE, "bad paged cache handle");
+    caches_remove(pc);
     if (skn_ctx_ok(pc->ctx)) {
         cudaSetDevice(pc->ctx->device);
         cudaStreamSynchronize(pc->ctx->stream);

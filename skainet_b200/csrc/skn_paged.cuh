@@ -25,7 +25,8 @@ struct skn_paged {
     int n_parts;                 // CTAs that share a launch's work, at most
     float *d_parts;              // prompts: blocks of rows of two segments per SM; then (from prompt_parts on) decoding, two per CTA: [rows of a CTA's segment][head_dim + 4]:
     int64_t prompt_parts;        // output, maximum, sum
-    unsigned *d_tickets;         // [2][2 n_parts], zero between launches
+    unsigned *d_tickets;         // [2][2 n_parts], zero between launches (a launch that gave up: from the report of it on, skn_paged.cu)
+    skn_paged *next;             // of all caches
 };
 constexpr int SKN_PAGED_PART_ROWS = 32;
 constexpr float PAGED_LOG2E = 1.4426950408889634f;        // scores are formed in base 2
@@ -127,6 +128,8 @@ template <int D, class CT> __device__ __forceinline__ float paged_load1(const CT
     }
 }
 #endif
+
+static inline size_t paged_ticket_bytes(const skn_paged *pc) { return (size_t)4 * pc->n_parts * sizeof(unsigned); }
 
 bool skn_paged_ok(const skn_paged *pc);
 cudaError_t skn_paged_attn_prepare(skn_paged *pc);

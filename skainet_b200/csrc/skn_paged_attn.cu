@@ -43,7 +43,7 @@ cudaError_t skn_paged_attn_prepare(skn_paged *pc) {
     }
     pc->n_parts = 4 * pc->ctx->sm_count;
     const size_t row = (D + 4) * sizeof(float), decode_rows = (size_t)2 * pc->ctx->sm_count * SKN_PAGED_PART_ROWS, prompt_rows = (size_t)2 * pc->ctx->sm_count * PP_ROWS;
-    const size_t tickets = (size_t)4 * pc->n_parts * sizeof(unsigned);
+    const size_t tickets = paged_ticket_bytes(pc);
     pc->prompt_parts = (int64_t)(prompt_rows * (D + 4));
     if (e == cudaSuccess) e = cudaMalloc((void **)&pc->d_parts, (decode_rows + prompt_rows) * row);
     if (e == cudaSuccess) e = cudaMalloc((void **)&pc->d_tickets, tickets);

@@ -1,11 +1,14 @@
 """Paged KV cache on the GPU: values, steps and calls at the edges of what it takes, against the oracle in 64 bits (tolerances as in
 test_gpu_paged.py)."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import skainet_b200 as skn
 from oracle import paged as oracle
+from skainet_b200.parallel import Exchange
 from test_gpu_paged import Step, bf16, check, filled, run_attend, tolerance
 
 pytestmark = pytest.mark.gpu
@@ -191,3 +194,49 @@ def test_values_of_unequal_blocks(ctx, io):
     tol = tolerance(want, mass, reach, 0.0 if io == "f32" else 2.0 ** -11, 0.0, io) + miss
     assert np.all(np.abs(out - want) <= tol)
     cache.close()
+
+
+def _counters(cache):
+    """device address and bytes of a cache's join counters: among the pointers of its structure, the only allocation of 64 bytes an SM"""
+    cuda = ctypes.CDLL("libcuda.so.1")
+    words = (ctypes.c_uint64 * 152).from_address(cache.handle.value)
+    size = 64 * torch.cuda.get_device_properties(0).multi_processor_count
+    for w in words:
+        base, n = ctypes.c_uint64(), ctypes.c_size_t()
+        if w and cuda.cuMemGetAddressRange_v2(ctypes.byref(base), ctypes.byref(n), ctypes.c_uint64(w)) == 0 and base.value == w and n.value == size:
+            return cuda, w, size
+    raise AssertionError("no counters")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "q4_0"])
+def test_a_cache_is_whole_after_a_wait_that_ran_out(dtype):
+    """A kernel that gives up leaves counters of its joins as they are (here: written by the host).  The report of a wait that ran out, of any kernel of the
+    context, sets them back, so that the next step is right."""
+    c0, c1 = skn.Context(0), skn.Context(0)
+    c0.set_wait_limit_ms(50)
+    ex = Exchange.connect_local([c0, c1], 4096)
+    caches = []
+    for lens, news, io in (([5000, 40], [50, 1], "bf16"), ([5000, 3], [1, 1], "f32")):
+        step = Step(5, lens, news, 32)
+        cache, _ = filled(c0, step, 2, 128, dtype, 5)
+        q = bf16(np.random.default_rng(1).standard_normal((step.n, 8, 128)))
+        caches.append((cache, step, q, io, run_attend(cache, step, q, io)))
+    for cache, *_ in caches:
+        cuda, at, size = _counters(cache)
+        back = (ctypes.c_uint32 * (size // 4))()
+        torch.cuda.synchronize()
+        assert cuda.cuMemcpyDtoH_v2(back, ctypes.c_uint64(at), ctypes.c_size_t(size)) == 0 and not any(back)
+        assert cuda.cuMemsetD32_v2(ctypes.c_uint64(at), ctypes.c_uint32(2 ** 31), ctypes.c_size_t(size // 4)) == 0
+    part, out = torch.ones(1024, device="cuda"), torch.zeros(1024, device="cuda")
+    torch.cuda.synchronize()
+    ex[0].all_reduce(part, None, out, 1024)                 # of two ranks the other one never joins
+    with pytest.raises(skn.SknError, match="bounded wait"):
+        c0.sync()
+    for cache, step, q, io, want in caches:
+        for _ in range(3):
+            assert np.array_equal(run_attend(cache, step, q, io), want)
+        cache.close()
+    for e in ex:
+        e.close()
+    c0.close()
+    c1.close()

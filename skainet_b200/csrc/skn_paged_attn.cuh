@@ -165,8 +165,7 @@ __device__ __forceinline__ int paged_slot(const PagedSegment &g, int cta) { retu
 
 // A segment from the definition, eight rows at a time: a thread per key for the scores, then a thread per dimension (and part of the keys) for the outputs
 // (THREADS of them, which `bar` brings together).  put(row, maximum (base 2), sum, this thread's dimension of the unnormalised output).
-// Eight rows share every load.  256 rows take 3.3 us a key: from 600 thousand keys of one CTA on the waits of the others of its warps (two seconds each) run out and
-// are reported.
+// Eight rows share every load: 256 rows take 3.3 us a key.
 constexpr int PA_REDO = 8;
 template <int D, int THREADS> struct alignas(16) PagedScratch {
     float q[D][PA_REDO], w[THREADS][PA_REDO], red[THREADS / 32][PA_REDO];

@@ -28,6 +28,10 @@ constexpr int PP_ROWS = 256, PP_KEYS = 128;
 // units that a block's start and end are worth on the line (2: a prompt of 8192 tokens 705 us, 3: 593, 4: 512, 6: 507, 9: 519; 16 of 1024: 331, 310, 298, 309, 312)
 constexpr int PP_COST = 4;
 
+// A segment that is computed again takes 3.3 us a key, and the CTA's other warps wait for two seconds: longer ones than this are left to the end of the
+// share, up to PP_LATE - 1 of them (with more, 600 thousand keys of the next one are too many: the call reports that a wait ran out)
+constexpr int PP_LATE_UNITS = 512, PP_LATE = 32;
+
 template <class CT, int D> struct PpTraits {
     static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
     static constexpr int THREADS = Q4 ? 512 : 384;                // two softmax warpgroups, one of MMA / TMA / clearing, one of unpacking
@@ -112,6 +116,80 @@ __device__ __forceinline__ uint64_t pp_ex2_pair(uint64_t x) {
     float a, b;
     skn_unpack2(x, a, b);
     return skn_pack2(pp_ex2(a), pp_ex2(b));
+}
+
+// This thread's row R of a block from the parts that its CTAs left; none: what a row without a weight is
+template <int D> __device__ __forceinline__ void pp_join(float *parts, const PagedSegment &now, int R, __nv_bfloat16 *out, uint32_t none, bool wide) {
+    auto part_of = [&](int k) { return parts + (int64_t)paged_slot(now, now.c0 + min(k, now.n_parts - 1)) * PP_ROWS * (D + 4); };
+    float top = PA_NONE, sum = 0.f;
+    for (int k = 0; k < now.n_parts; ++k) top = fmaxf(top, __ldcg(part_of(k) + D * PP_ROWS + R));
+    for (int k = 0; k < now.n_parts; ++k) sum = fmaf(__ldcg(part_of(k) + (D + 1) * PP_ROWS + R), exp2f(__ldcg(part_of(k) + D * PP_ROWS + R) - top), sum);
+    const float inv = 1.f / sum;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {
+        float4 o[4] = {};
+        for (int k = 0; k < now.n_parts; k += 4) {       // four parts' loads on their way at once
+            float4 y[4][4];
+            float f[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                f[b] = k + b < now.n_parts ? exp2f(__ldcg(part_of(k + b) + D * PP_ROWS + R) - top) : 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[b][e] = __ldcg(reinterpret_cast<const float4 *>(part_of(k + b)) + (c / 4 + e) * PP_ROWS + R);
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                if (f[b] != 0.f)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[e].x = fmaf(y[b][e].x, f[b], o[e].x); o[e].y = fmaf(y[b][e].y, f[b], o[e].y);
+                        o[e].z = fmaf(y[b][e].z, f[b], o[e].z); o[e].w = fmaf(y[b][e].w, f[b], o[e].w);
+                    }
+        }
+        uint32_t y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            y[2 * e] = sum == 0.f ? none : pack_bf16(o[e].x * inv, o[e].y * inv);
+            y[2 * e + 1] = sum == 0.f ? none : pack_bf16(o[e].z * inv, o[e].w * inv);
+        }
+        pp_store32(out + c, y, wide);
+    }
+}
+// Blocks with a result that is not finite, from the definition, by the softmax warps (out of line: nothing of it in the others' registers)
+template <class CT, int D>
+__device__ __noinline__ void pp_again(const PagedAttn &p, const PagedSegment *list, int n, PagedScratch<D, 256> &scratch, unsigned &ticket) {
+    using IO = __nv_bfloat16;
+    const int tid = threadIdx.x;
+    pp_bar();                                    // (the list is there)
+    for (int i = 0; i < n; ++i) {
+        const PagedSegment now = list[i];
+        const bool shared = now.n_parts > 1;
+        float *const part = p.parts + (int64_t)now.slot * PP_ROWS * (D + 4);
+        paged_redo<CT, D, 256, IO>(p, now, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p, &now](int row, float rm, float rl, float acc) {
+            const int t = (now.row0 + row) / p.group;
+            if (shared) {
+                if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;
+                if (tid == 0) {
+                    part[D * PP_ROWS + row] = rm + PpTraits<CT, D>::LIFT;      // (its weights are not lifted)
+                    part[(D + 1) * PP_ROWS + row] = rl;
+                }
+            } else if (tid < D)
+                static_cast<IO *>(p.out)[(int64_t)(now.first + t) * p.out_stride + (now.head * p.group + (now.row0 + row) % p.group) * D + tid] =
+                    __float2bfloat16_rn(rl != 0.f ? acc / rl : now.len - now.n + t < 0 ? 0.f : NAN);
+        });
+        if (!shared) continue;
+        __threadfence();
+        pp_bar();
+        if (tid == 0) ticket = atomicInc(&p.tickets[paged_slot(now, now.c0)], (unsigned)now.n_parts - 1);
+        pp_bar();
+        if (ticket == (unsigned)now.n_parts - 1 && tid < now.rows) {
+            __threadfence();
+            const int t = (now.row0 + tid) / p.group;
+            IO *const out = static_cast<IO *>(p.out) + (int64_t)(now.first + t) * p.out_stride + (now.head * p.group + (now.row0 + tid) % p.group) * D;
+            pp_join<D>(p.parts, now, tid, out, now.len - now.n + t < 0 ? 0u : 0x7FFF7FFFu, false);
+        }
+        pp_bar();
+    }
 }
 
 // A CTA's share of the line, segment by segment: one warp walks it ahead of the others and leaves the segments in shared memory
@@ -204,6 +282,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     __shared__ unsigned ticket;
     __shared__ int starts[THREADS + 1];
     __shared__ PagedScratch<D, 256> scratch;
+    __shared__ alignas(16) PagedSegment late[PP_LATE];        // to be computed again
+    __shared__ int n_late;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedStep &st = p.st;
 
@@ -229,6 +309,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         }
         skn_fence_mbar_init();
         found[0] = -1;
+        n_late = 0;
     }
 
     if (p.split) skn_pdl_launch_dependents();        // the launch for short sequences may take the SMs that this one leaves
@@ -526,19 +607,15 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             }
             if (pp_any(!got)) more = false;
             if (pp_any(odd)) {
-                const PagedSegment again = now;      // (a copy: the address of the one that the loops use is not taken)
-                paged_redo<CT, D, 256, IO>(p, again, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
-                    const int tr = (now.row0 + row) / p.group;
-                    if (shared) {
-                        if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;
-                        if (tid == 0) {
-                            part[D * PP_ROWS + row] = rm + T::LIFT;      // (its weights are not lifted)
-                            part[(D + 1) * PP_ROWS + row] = rl;
-                        }
-                    } else if (tid < D)
-                        static_cast<IO *>(p.out)[(int64_t)(now.first + tr) * p.out_stride + (now.head * p.group + (now.row0 + row) % p.group) * D + tid] =
-                            __float2bfloat16_rn(rl != 0.f ? acc / rl : now.len - now.n + tr < 0 ? 0.f : NAN);
-                });
+                const int k = n_late;
+                const bool later = now.u1 - now.u0 > PP_LATE_UNITS && k < PP_LATE - 1;
+                pp_bar();                            // (n_late is read)
+                if (tid == 0) {
+                    late[k] = now;
+                    if (later) n_late = k + 1;
+                }
+                if (!later) pp_again<CT, D>(p, late + k, 1, scratch, ticket);
+                continue;
             }
             if (shared) {
                 __threadfence();
@@ -547,45 +624,13 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 pp_bar();
                 if (ticket == (unsigned)now.n_parts - 1 && real) {
                     __threadfence();
-                    auto part_of = [&](int k) { return p.parts + (int64_t)paged_slot(now, now.c0 + min(k, now.n_parts - 1)) * PP_ROWS * (D + 4); };
-                    float top = PA_NONE, sum = 0.f;
-                    for (int k = 0; k < now.n_parts; ++k) top = fmaxf(top, __ldcg(part_of(k) + D * PP_ROWS + R));
-                    for (int k = 0; k < now.n_parts; ++k) sum = fmaf(__ldcg(part_of(k) + (D + 1) * PP_ROWS + R), exp2f(__ldcg(part_of(k) + D * PP_ROWS + R) - top), sum);
-                    const float inv = 1.f / sum;
-                    const uint32_t none = now.len - now.n + t < 0 ? 0u : 0x7FFF7FFFu;
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {
-                        float4 o[4] = {};
-                        for (int k = 0; k < now.n_parts; k += 4) {       // four parts' loads on their way at once
-                            float4 y[4][4];
-                            float f[4];
-#pragma unroll
-                            for (int b = 0; b < 4; ++b) {
-                                f[b] = k + b < now.n_parts ? exp2f(__ldcg(part_of(k + b) + D * PP_ROWS + R) - top) : 0.f;
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) y[b][e] = __ldcg(reinterpret_cast<const float4 *>(part_of(k + b)) + (c / 4 + e) * PP_ROWS + R);
-                            }
-#pragma unroll
-                            for (int b = 0; b < 4; ++b)
-                                if (f[b] != 0.f)
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        o[e].x = fmaf(y[b][e].x, f[b], o[e].x); o[e].y = fmaf(y[b][e].y, f[b], o[e].y);
-                                        o[e].z = fmaf(y[b][e].z, f[b], o[e].z); o[e].w = fmaf(y[b][e].w, f[b], o[e].w);
-                                    }
-                        }
-                        uint32_t y[8];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            y[2 * e] = sum == 0.f ? none : pack_bf16(o[e].x * inv, o[e].y * inv);
-                            y[2 * e + 1] = sum == 0.f ? none : pack_bf16(o[e].z * inv, o[e].w * inv);
-                        }
-                        pp_store32(out + c, y, wide);
-                    }
+                    pp_join<D>(p.parts, now, R, out, now.len - now.n + t < 0 ? 0u : 0x7FFF7FFFu, wide);
                 }
                 pp_bar();                            // (the ticket is read)
             }
         }
+        pp_bar();
+        if (n_late) pp_again<CT, D>(p, late, n_late, scratch, ticket);       // (no other warp waits any more)
     }
     // ---- MMAs: warp 8 --------------------------------------------------------------------------------------------------------
     else if (warp < 12) {

@@ -240,3 +240,32 @@ def test_a_cache_is_whole_after_a_wait_that_ran_out(dtype):
         e.close()
     c0.close()
     c1.close()
+
+
+def test_segments_that_take_seconds_to_compute_again(ctx):
+    """An infinity that every row sees, in front of 650 thousand keys: the blocks' second computation takes about two seconds, which the other warps of their CTAs
+    wait for.  Rows against the formula in 64 bits by torch; exponentials and weights as for fp32 rows of long sums, outputs rounded to bf16."""
+    kv, group, dim, page, n, new = 8, 64, 64, 128, 650_000, 76
+    pages = -(-n // page)
+    pools = [torch.randn(pages, kv, page, dim, device="cuda").to(torch.float16) for _ in range(2)]
+    pools[1][0, :, 0, 3] = float("inf")
+    cache = skn.PagedKVCache(ctx, pages, page, kv, dim, "f16", pools=pools)
+    b = skn.PagedBatch(torch.arange(pages, dtype=torch.int32, device="cuda")[None], torch.tensor([0, new], dtype=torch.int32, device="cuda"),
+                       torch.tensor([n], dtype=torch.int32, device="cuda"), new, new)
+    q = (8 * torch.randn(new, kv * group, dim, device="cuda")).bfloat16()
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    cache.attend_dev(b, q, out, scale=0.125)
+    ctx.sync()
+    assert (out[..., 3] == float("inf")).all()
+    for row, head in ((0, 0), (40, 200), (75, 511)):
+        k, v = (p[:, head // group].reshape(-1, dim)[:n - new + row + 1].double() for p in pools)
+        z = k @ q[row, head].double() * 0.125
+        w = torch.softmax(z, 0)
+        keep = torch.arange(dim) != 3
+        want, mass = (w @ v)[keep], (w @ v.abs())[keep]
+        reach = 0.125 * (k.abs() @ q[row, head].double().abs()).max()
+        # sums of 650 thousand weights, 256 at a time: 2540 roundings of 2^-24 at worst
+        tol = mass * (torch.expm1(2 * 2.0 ** -19 * reach) + 2.0 ** -18 + 2540 * 2.0 ** -24) + 2.0 ** -8 * want.abs()
+        assert ((out[row, head].double()[keep] - want).abs() <= tol).all()
+    cache.close()

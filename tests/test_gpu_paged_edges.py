@@ -243,9 +243,9 @@ def test_a_cache_is_whole_after_a_wait_that_ran_out(dtype):
 
 
 def test_segments_that_take_seconds_to_compute_again(ctx):
-    """An infinity that every row sees, in front of 650 thousand keys: the blocks' second computation takes about two seconds, which the other warps of their CTAs
-    wait for.  Rows against the formula in 64 bits by torch; exponentials and weights as for fp32 rows of long sums, outputs rounded to bf16."""
-    kv, group, dim, page, n, new = 8, 64, 64, 128, 650_000, 76
+    """An infinity that every row sees, in front of two million keys: the blocks' second computation takes seconds, longer than the other warps of their CTAs
+    wait.  Rows against the formula in 64 bits by torch; exponentials and weights as for fp32 rows of long sums, outputs rounded to bf16."""
+    kv, group, dim, page, n, new = 8, 64, 64, 128, 2_000_000, 76
     pages = -(-n // page)
     pools = [torch.randn(pages, kv, page, dim, device="cuda").to(torch.float16) for _ in range(2)]
     pools[1][0, :, 0, 3] = float("inf")
@@ -265,7 +265,7 @@ def test_segments_that_take_seconds_to_compute_again(ctx):
         keep = torch.arange(dim) != 3
         want, mass = (w @ v)[keep], (w @ v.abs())[keep]
         reach = 0.125 * (k.abs() @ q[row, head].double().abs()).max()
-        # sums of 650 thousand weights, 256 at a time: 2540 roundings of 2^-24 at worst
-        tol = mass * (torch.expm1(2 * 2.0 ** -19 * reach) + 2.0 ** -18 + 2540 * 2.0 ** -24) + 2.0 ** -8 * want.abs()
+        # sums of two million weights, 256 at a time: 7813 roundings of 2^-24 at worst
+        tol = mass * (torch.expm1(2 * 2.0 ** -19 * reach) + 2.0 ** -18 + 7813 * 2.0 ** -24) + 2.0 ** -8 * want.abs()
         assert ((out[row, head].double()[keep] - want).abs() <= tol).all()
     cache.close()

@@ -381,7 +381,8 @@ int32_t skn_paged_pool_bytes(const skn_paged_spec *spec, int64_t *bytes);
 int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_dev, void *v_pool_dev, skn_paged **out);
 int32_t skn_paged_destroy(skn_paged *pc);
 int32_t skn_paged_info(const skn_paged *pc, void **k_pool_dev, void **v_pool_dev, int64_t *pool_bytes);
-/* Append the step's keys and values, the keys rotated to their positions; q (optional) is rotated into q_out, which may be q.
+/* Append the step's keys and values, the keys rotated to their positions; q (optional) is rotated into q_out, which may be q
+ * (the same rows), but lies over no other part of q, k and v.
  * `_dev`: io is the element type of k, v, q and q_out (SKN_KV_F32 or SKN_KV_BF16), a row [heads][head_dim]; strides are the elements from one
  * row to the next (rows of a joint projection need no copy).  Pointers and rows are 16-byte aligned.  Rows of nobody and padded rows of q_out stay
  * as they are.  A row of a page is appended to by one of the step's sequences only.  The host form takes dense fp32 rows and answers every mistake
@@ -391,7 +392,7 @@ int32_t skn_paged_append(skn_paged *pc, const skn_paged_batch *batch, const floa
 int32_t skn_paged_append_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, const void *k_dev, int64_t k_stride, const void *v_dev,
                              int64_t v_stride, const void *q_dev, int64_t q_stride, int32_t n_q_heads, void *q_out_dev, int64_t q_out_stride);
 /* The reverse of append: the cached rows at the positions of the step's tokens (all tokens of a sequence, where token_start says so), dense
- * [n_tokens][n_kv_heads][head_dim], fp32 (host) or io (device). */
+ * [n_tokens][n_kv_heads][head_dim], fp32 (host) or io (device); K's rows do not lie over V's. */
 int32_t skn_paged_gather(skn_paged *pc, const skn_paged_batch *batch, float *k_out_host, float *v_out_host);
 int32_t skn_paged_gather_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t io, void *k_out_dev, void *v_out_dev);
 /* out = softmax(scale * q . K^T) . V of every row over the cached tokens at its own position and before: all of them (window 0), or the last

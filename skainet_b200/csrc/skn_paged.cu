@@ -277,6 +277,15 @@ static int32_t check_rows(skn_ctx *ctx, const char *what, const void *p, int64_t
     if (stride < width) return skn_fail(ctx, SKN_ERR_SHAPE, "%s: rows of %lld elements are %lld apart", what, (long long)width, (long long)stride);
     return SKN_OK;
 }
+// whether rows of a and b meet in memory (side by side in wider rows of one length they do not)
+static bool rows_meet(int64_t n, int32_t io, const void *a, int64_t a_stride, int64_t a_width, const void *b, int64_t b_stride, int64_t b_width) {
+    const int64_t size = io == SKN_KV_F32 ? 4 : 2;
+    const uintptr_t p = (uintptr_t)a, q = (uintptr_t)b;
+    if (p >= q + ((n - 1) * b_stride + b_width) * size || q >= p + ((n - 1) * a_stride + a_width) * size) return false;
+    if (a_stride != b_stride) return true;
+    const int64_t row = a_stride * size, behind = q >= p ? (int64_t)((q - p) % (uintptr_t)row) : (row - (int64_t)((p - q) % (uintptr_t)row)) % row;
+    return behind < a_width * size || behind + b_width * size > row;
+}
 static int32_t check_heads(skn_ctx *ctx, const skn_paged *pc, int32_t n_q_heads) {
     if (n_q_heads < 1 || n_q_heads % pc->spec.n_kv_heads) return skn_fail(ctx, SKN_ERR_SHAPE, "Shapes do not align.");
     if (n_q_heads / pc->spec.n_kv_heads > 64) return skn_fail(ctx, SKN_ERR_SHAPE, "%d query heads per kv head; 64 at most", n_q_heads / pc->spec.n_kv_heads);
@@ -527,6 +536,12 @@ int32_t skn_paged_append_dev(skn_paged *pc, const skn_paged_batch *batch, int32_
         if ((rc = check_heads(ctx, pc, n_q_heads)) || (rc = check_rows(ctx, "q", q_dev, q_stride, wq, io)) ||
             (rc = check_rows(ctx, "q_out", q_out_dev, q_out_stride, wq, io)))
             return rc;
+        // tokens are turned side by side: only a row's own place may be written to
+        const int32_t n = batch->n_tokens;
+        if ((q_out_dev != q_dev || (q_out_stride != q_stride && n > 1)) && rows_meet(n, io, q_dev, q_stride, wq, q_out_dev, q_out_stride, wq))
+            return skn_fail(ctx, SKN_ERR_ARG, "q_out lies over q, but is not q");
+        if (rows_meet(n, io, k_dev, k_stride, w, q_out_dev, q_out_stride, wq) || rows_meet(n, io, v_dev, v_stride, w, q_out_dev, q_out_stride, wq))
+            return skn_fail(ctx, SKN_ERR_ARG, "q_out lies over k or v");
     }
     SKN_CUDA(ctx, cudaSetDevice(ctx->device));
     return append_run(pc, batch, io, PagedRows{k_dev, v_dev, q_dev, q_out_dev, k_stride, v_stride, q_stride, q_out_stride, q_dev ? n_q_heads : 0,
@@ -564,6 +579,8 @@ int32_t skn_paged_gather_dev(skn_paged *pc, const skn_paged_batch *batch, int32_
     int32_t rc = check_io(ctx, io);
     if (rc || (rc = check_batch(ctx, batch, &nothing)) || nothing) return rc;
     if ((rc = check_rows(ctx, "k_out", k_out_dev, 16, 0, io)) || (rc = check_rows(ctx, "v_out", v_out_dev, 16, 0, io))) return rc;
+    const int64_t w = (int64_t)pc->spec.n_kv_heads * pc->spec.head_dim;
+    if (rows_meet(batch->n_tokens, io, k_out_dev, w, w, v_out_dev, w, w)) return skn_fail(ctx, SKN_ERR_ARG, "k_out lies over v_out");
     SKN_CUDA(ctx, cudaSetDevice(ctx->device));
     SKN_CUDA(ctx, PAGED_BY_TYPE(gather_launch, paged_step(pc, batch), pc, k_out_dev, v_out_dev, ctx->stream));
     return SKN_OK;
@@ -603,12 +620,7 @@ int32_t skn_paged_attn_dev(skn_paged *pc, const skn_paged_batch *batch, int32_t 
     const int64_t wq = (int64_t)n_q_heads * pc->spec.head_dim;
     if ((rc = check_rows(ctx, "q", q_dev, q_stride, wq, io)) || (rc = check_rows(ctx, "out", out_dev, out_stride, wq, io))) return rc;
     // outputs are written while other rows' queries are still to be read, and a query is asked for again where a result is not finite
-    const int64_t size = io == SKN_KV_F32 ? 4 : 2, n = batch->n_tokens - 1;
-    const uintptr_t qa = (uintptr_t)q_dev, oa = (uintptr_t)out_dev, q_end = qa + (n * q_stride + wq) * size, o_end = oa + (n * out_stride + wq) * size;
-    if (qa < o_end && oa < q_end) {
-        const int64_t apart = q_stride == out_stride ? (int64_t)((qa > oa ? qa - oa : oa - qa) % (uintptr_t)(q_stride * size)) : 0;
-        if (q_stride != out_stride || apart < wq * size || apart > (q_stride - wq) * size) return skn_fail(ctx, SKN_ERR_ARG, "out lies over q");
-    }
+    if (rows_meet(batch->n_tokens, io, q_dev, q_stride, wq, out_dev, out_stride, wq)) return skn_fail(ctx, SKN_ERR_ARG, "out lies over q");
     SKN_CUDA(ctx, cudaSetDevice(ctx->device));
     return skn_paged_attn_launch(pc, batch, io, q_dev, q_stride, n_q_heads, scale, window, window ? sinks : 0, out_dev, out_stride);
 }

@@ -269,3 +269,46 @@ def test_segments_that_take_seconds_to_compute_again(ctx):
         tol = mass * (torch.expm1(2 * 2.0 ** -19 * reach) + 2.0 ** -18 + 7813 * 2.0 ** -24) + 2.0 ** -8 * want.abs()
         assert ((out[row, head].double()[keep] - want).abs() <= tol).all()
     cache.close()
+
+
+def test_rows_written_over_others_are_refused(ctx):
+    """queries that are turned into a place of which other rows are still read, rows that are gathered over one another; beside one another is right"""
+    kv, H, dim = 2, 4, 64
+    step = Step(3, [40, 30], [2, 3], 16)
+    cache, _ = filled(ctx, step, kv, dim, "bf16", 3, rot=64)
+    b, n = step.batch(), step.n
+    wide = torch.randn(n + 1, 2 * H + 2 * kv, dim, device="cuda").bfloat16()
+    flat = wide.view(-1)
+    q, k, v = wide[:n, :H], wide[:n, H:H + kv], wide[:n, H + kv:H + 2 * kv]
+    over_q = [wide[1:, :H], wide[:n, 1:H + 1][:, :H], flat[:n * H * dim].view(n, H, dim)]
+    for out in over_q:
+        with pytest.raises(skn.SknError, match="over q"):
+            cache.append_dev(b, k.clone(), v.clone(), q, out)
+    for out in (wide[:n, H:2 * H], wide[:n, H + kv:2 * H + kv], wide[:n, H + 1:2 * H + 1], flat[n * dim:n * dim + n * H * dim].view(n, H, dim)):
+        with pytest.raises(skn.SknError, match="over k or v"):
+            cache.append_dev(b, k, v, q.clone(), out)
+    dense = torch.zeros(2 * n * kv * dim, device="cuda")
+    at = [dense[i * dim:i * dim + n * kv * dim].view(n, kv, dim) for i in (0, 1, n * kv - 1, n * kv)]
+    for i, j in ((0, 0), (0, 1), (0, 2), (2, 0), (1, 3)):
+        with pytest.raises(skn.SknError, match="over v_out"):
+            cache.gather_dev(b, at[i], at[j])
+    torch.cuda.synchronize()
+    own = torch.zeros(n, H, dim, device="cuda").bfloat16()
+    beside = wide[:n, H + 2 * kv:]
+    was = wide.clone()
+    torch.cuda.synchronize()
+    cache.append_dev(b, k, v, q, own)
+    cache.append_dev(b, k, v, q, beside)
+    cache.gather_dev(b, at[0], at[3])
+    cache.append_dev(b, k, v, q, q)
+    ctx.sync()
+    assert torch.equal(own, beside) and torch.equal(own, q) and torch.equal(wide[:n, H:H + 2 * kv], was[:n, H:H + 2 * kv]) and torch.equal(wide[n], was[n])
+    assert torch.equal(at[3], v.float())
+    one = Step(3, [40], [1], 16)                           # one row: no other one that its stride could meet
+    b1 = one.batch()
+    q1 = wide[:1, :H].clone()
+    torch.cuda.synchronize()
+    cache.append_dev(b1, k[:1], v[:1], wide[:1, :H], wide[:1, :H])
+    cache.append_dev(b1, k[:1], v[:1], q1, q1.view(-1).as_strided((1, H, dim), (2 * H * dim, dim, 1)))
+    ctx.sync()
+    cache.close()

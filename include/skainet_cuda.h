@@ -366,7 +366,7 @@ typedef struct skn_paged_spec {
  * and what attention says of its sequence means nothing.  Other sequences of the step are not affected. */
 typedef struct skn_paged_batch {
     int32_t n_seqs, n_tokens;        /* at most 65535; n_tokens: rows of k, v, q and out, at most 2^24 */
-    int32_t max_new;                 /* no sequence has more new tokens */
+    int32_t max_new;                 /* no sequence has more new tokens (more than n_tokens says no more than n_tokens) */
     int32_t max_pages;               /* columns of the page table, at most 2^23 */
     const int32_t *page_table;       /* [n_seqs][max_pages] */
     const int32_t *token_start;      /* [n_seqs + 1], not decreasing */

@@ -40,7 +40,8 @@ struct PagedStep {
     int32_t *status;
 };
 static inline PagedStep paged_step(const skn_paged *pc, const skn_paged_batch *b) {
-    return PagedStep{b->page_table, b->token_start, b->lengths, b->n_seqs, b->n_tokens, b->max_new, b->max_pages,
+    // (no sequence has more rows than the step: a bound that says nothing makes no larger grid)
+    return PagedStep{b->page_table, b->token_start, b->lengths, b->n_seqs, b->n_tokens, b->max_new < b->n_tokens ? b->max_new : b->n_tokens, b->max_pages,
                      pc->spec.n_kv_heads, pc->page_shift, pc->spec.n_pages, pc->head_bytes, pc->ctx->d_status};
 }
 

@@ -9,7 +9,7 @@ import torch
 import skainet_b200 as skn
 from oracle import paged as oracle
 from skainet_b200.parallel import Exchange
-from test_gpu_paged import Step, bf16, check, filled, run_attend, tolerance
+from test_gpu_paged import IO, Step, bf16, check, filled, run_attend, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -311,4 +311,31 @@ def test_rows_written_over_others_are_refused(ctx):
     cache.append_dev(b1, k[:1], v[:1], wide[:1, :H], wide[:1, :H])
     cache.append_dev(b1, k[:1], v[:1], q1, q1.view(-1).as_strided((1, H, dim), (2 * H * dim, dim, 1)))
     ctx.sync()
+    cache.close()
+
+
+@pytest.mark.parametrize("dtype,io", [("f16", "f32"), ("bf16", "bf16"), ("q4_0", "bf16")])
+@pytest.mark.parametrize("news", [[1, 1, 0], [20, 1, 3]])
+def test_a_bound_of_new_tokens_that_says_nothing(ctx, dtype, io, news):
+    """max_new is an upper bound: the largest number is taken as the step's rows, by the choice of the kernel and by its grid"""
+    kv, group, dim = 2, 8, 64
+    step = Step(3, [400, 90, 30], news, 16, padding=2)
+    cache, ref = filled(ctx, step, kv, dim, dtype, 3)
+    g = np.random.default_rng(3)
+    k, v = (g.standard_normal((step.n, kv, dim)).astype(np.float32) for _ in range(2))
+    q = bf16(g.standard_normal((step.n, kv * group, dim)))
+    t = [torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda() for a in (step.table, step.starts, step.lens)]
+    kd, vd, qd = (torch.from_numpy(a).cuda().to(IO[io]) for a in (k, v, q))
+    out = torch.zeros_like(qd)
+    b = skn.PagedBatch(*t, step.n, 2 ** 31 - 1)
+    kr, vr = kd.float().cpu().numpy(), vd.float().cpu().numpy()
+    ref.append(kr, vr, step.table, step.starts, step.lens)
+    want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    torch.cuda.synchronize()
+    cache.append_dev(b, kd, vd)
+    cache.attend_dev(b, qd, out)
+    ctx.sync()
+    n = int(step.starts[-1])
+    check(out.float().cpu().numpy()[:n], want[:n], mass[:n], reach[:n], io, dtype, True)
+    assert not out[n:].any()
     cache.close()

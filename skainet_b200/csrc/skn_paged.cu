@@ -243,7 +243,7 @@ static int32_t check_spec(skn_ctx *ctx, const skn_paged_spec *s) {
     if (!s) return skn_fail(ctx, SKN_ERR_ARG, "NULL specification");
     if (s->kv_dtype != SKN_KV_F16 && s->kv_dtype != SKN_KV_BF16 && s->kv_dtype != SKN_KV_Q4_0)
         return skn_fail(ctx, SKN_ERR_TYPE, "a paged cache holds fp16, bf16 or Q4_0, not element type %d", s->kv_dtype);
-    if (s->n_kv_heads < 1 || s->n_kv_heads > 256 || s->n_pages < 1) return skn_fail(ctx, SKN_ERR_ARG, "pages and heads (at most 256) must be positive");
+    if (s->n_kv_heads < 1 || s->n_kv_heads > PAGED_MAX_HEADS || s->n_pages < 1) return skn_fail(ctx, SKN_ERR_ARG, "pages and heads (at most %d) must be positive", PAGED_MAX_HEADS);
     if (s->head_dim != 64 && s->head_dim != 128) return skn_fail(ctx, SKN_ERR_SHAPE, "head_dim must be 64 or 128 (got %d)", s->head_dim);
     if (s->page_tokens != 16 && s->page_tokens != 32 && s->page_tokens != 64 && s->page_tokens != 128)
         return skn_fail(ctx, SKN_ERR_SHAPE, "a page holds 16, 32, 64 or 128 tokens, not %d", s->page_tokens);
@@ -301,11 +301,12 @@ static int32_t check_io(skn_ctx *ctx, int32_t io) {
     return SKN_OK;
 }
 
-template <class CT, int D, class IO> static cudaError_t append_launch(const PagedStep &st, const PagedRows &r, cudaStream_t stream) {
+template <class CT, int D, class IO> static cudaError_t append_launch(const PagedStep &st, const PagedRows &r, int device, cudaStream_t stream) {
     const size_t smem = sizeof(CT) == 1 ? (size_t)st.heads * D * sizeof(float) : 0;
     auto *kern = skn_paged_append_kernel<CT, D, IO>;
     if (smem > 32000) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        static uint64_t done = 0;
+        const cudaError_t e = paged_attributes(kern, (size_t)PAGED_MAX_HEADS * D * sizeof(float), device, &done);
         if (e != cudaSuccess) return e;
     }
     kern<<<st.n_tokens, 128, smem, stream>>>(st, r);
@@ -323,7 +324,7 @@ template <class CT, int D, class IO> static cudaError_t gather_launch(const Page
                                         : PAGED_BY_DIM(fn, skn_q4, __VA_ARGS__))
 
 static int32_t append_run(skn_paged *pc, const skn_paged_batch *b, int32_t io, const PagedRows &r) {
-    SKN_CUDA(pc->ctx, PAGED_BY_TYPE(append_launch, paged_step(pc, b), r, pc->ctx->stream));
+    SKN_CUDA(pc->ctx, PAGED_BY_TYPE(append_launch, paged_step(pc, b), r, pc->ctx->device, pc->ctx->stream));
     return SKN_OK;
 }
 

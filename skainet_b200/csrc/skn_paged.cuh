@@ -29,6 +29,7 @@ struct skn_paged {
     skn_paged *next;             // of all caches
 };
 constexpr int SKN_PAGED_PART_ROWS = 32;
+constexpr int PAGED_MAX_HEADS = 256;         // kv heads
 constexpr float PAGED_LOG2E = 1.4426950408889634f;        // scores are formed in base 2
 
 // A step as the kernels see it
@@ -127,6 +128,15 @@ template <int D, class CT> __device__ __forceinline__ float paged_load1(const CT
         const int q = p[((((d >> 5) << page_shift) + r) << 4) + (d & 15)] >> (d & 16 ? 4 : 0) & 15;
         return (float)(q - 8) * __half2float(*reinterpret_cast<const __half *>(p + ((D / 2) << page_shift) + (r * (D / 32) + (d >> 5)) * 2));
     }
+}
+
+// a kernel's largest dynamic shared memory, once per kernel and device (`done`: a bit each; setting it twice does no harm, but two contexts share the
+// setting: it is the most that any cache asks for)
+template <class K> static cudaError_t paged_attributes(K *kern, size_t smem, int device, uint64_t *done) {
+    if (device < 64 && __atomic_load_n(done, __ATOMIC_RELAXED) >> device & 1) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && device < 64) __atomic_fetch_or(done, (uint64_t)1 << device, __ATOMIC_RELAXED);
+    return e;
 }
 #endif
 

@@ -1087,13 +1087,6 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
-// once per kernel and device (`done`: a bit each; setting it twice does no harm)
-template <class K> static cudaError_t paged_attributes(K *kern, size_t smem, int device, uint64_t *done) {
-    if (device < 64 && __atomic_load_n(done, __ATOMIC_RELAXED) >> device & 1) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess && device < 64) __atomic_fetch_or(done, (uint64_t)1 << device, __ATOMIC_RELAXED);
-    return e;
-}
 template <class CT, int D, int NB, bool EX> static cudaError_t attn_launch(const skn_paged *pc, const PagedAttn &p) {
     using T = PaTraits<CT, D, NB, EX>;
     auto *kern = skn_paged_attn_kernel<CT, D, NB, EX>;

@@ -1,6 +1,7 @@
 """Paged KV cache on the GPU: values, steps and calls at the edges of what it takes, against the oracle in 64 bits (tolerances as in
 test_gpu_paged.py)."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -339,3 +340,46 @@ def test_a_bound_of_new_tokens_that_says_nothing(ctx, dtype, io, news):
     check(out.float().cpu().numpy()[:n], want[:n], mass[:n], reach[:n], io, dtype, True)
     assert not out[n:].any()
     cache.close()
+
+
+@pytest.mark.parametrize("dtype", ["q4_0", "bf16"])
+@pytest.mark.parametrize("heads", [63, 64, 256])
+def test_many_kv_heads(ctx, dtype, heads):
+    dim, page = 128, 16
+    step = Step(3, [33, 5, 20], [3, 5, 1], page)
+    cache, ref = filled(ctx, step, heads, dim, dtype, 3, rot=64, pairs="halves")
+    g = np.random.default_rng(heads)
+    k, v = (g.standard_normal((step.n, heads, dim)).astype(np.float32) for _ in range(2))
+    q = g.standard_normal((step.n, heads, dim)).astype(np.float32)
+    cache.append(k, v, step.table, step.starts, step.lens)
+    ref.append(k, v, step.table, step.starts, step.lens)
+    kk, vv = cache.gather(step.table, step.full, step.lens)
+    for s in range(3):
+        a, b = step.full[s], step.full[s + 1]
+        assert np.array_equal(kk[a:b].transpose(1, 0, 2), ref.rows("k", s, b - a, step.table))
+        assert np.array_equal(vv[a:b].transpose(1, 0, 2), ref.rows("v", s, b - a, step.table))
+    want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.1)
+    check(run_attend(cache, step, q, "f32", scale=0.1), want, mass, reach, "f32", dtype, False)
+    cache.close()
+
+
+def test_caches_of_many_and_of_few_heads_at_once():
+    """two threads, each with a context of its own, append to 4-bit caches of 256 and of 64 heads: neither takes shared memory away from the other's launches"""
+    def work(heads, out):
+        try:
+            with skn.Context(0) as c:
+                cache = skn.PagedKVCache(c, 2, 16, heads, 128, "q4_0")
+                k = np.random.default_rng(heads).standard_normal((1, heads, 128)).astype(np.float32)
+                for _ in range(2000):
+                    cache.append(k, k, [[0]], [0, 1], [1])
+                cache.close()
+        except Exception as e:                              # told by the main thread
+            out.append(e)
+
+    failed = []
+    threads = [threading.Thread(target=work, args=(h, failed)) for h in (256, 64)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed

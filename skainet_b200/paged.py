@@ -34,6 +34,8 @@ class PagedBatch:
         for t, shape in ((page_table, (n, page_table.shape[-1])), (token_start, (n + 1,)), (lengths, (n,))):
             if tuple(t.shape) != shape or not str(t.dtype).endswith("int32") or not t.is_contiguous() or not t.is_cuda:
                 raise ValueError("page_table [n, max_pages], token_start [n + 1] and lengths [n] are dense int32 device tensors")
+        if not page_table.device.index == token_start.device.index == lengths.device.index:
+            raise ValueError("page_table, token_start and lengths are on one device")
         self._keep = page_table, token_start, lengths
         self.device = page_table.device.index
         self.n_seqs, self.n_tokens, self.max_new, self.max_pages = n, int(n_tokens), int(max_new), int(page_table.shape[1])

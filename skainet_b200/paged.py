@@ -43,10 +43,15 @@ class PagedBatch:
         self._ref = ctypes.byref(self._c)
 
 
+def _int32(a) -> np.ndarray:
+    a = np.asarray(a)
+    if a.size and (a.dtype.kind not in "biuf" or not (np.floor(a) == a).all() or a.min() < -2 ** 31 or a.max() >= 2 ** 31):
+        raise ValueError("page_table, token_start and lengths are numbers of int32")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
 def _host_batch(page_table, token_start, lengths, n_tokens):
-    table = np.ascontiguousarray(page_table, dtype=np.int32)
-    starts = np.ascontiguousarray(token_start, dtype=np.int32)
-    lens = np.ascontiguousarray(lengths, dtype=np.int32)
+    table, starts, lens = _int32(page_table), _int32(token_start), _int32(lengths)
     if table.ndim != 2 or lens.shape != (table.shape[0],) or starts.shape != (table.shape[0] + 1,):
         raise ValueError("Shapes do not align.")
     new = int(np.diff(starts.astype(np.int64)).max(initial=0))

@@ -363,7 +363,8 @@ typedef struct skn_paged_spec {
  * length, or outside every query's window) may hold anything.  The arrays are on the device for `_dev` calls, whose kernels check
  * what they use of them: the next skn_sync returns SKN_ERR_ARG where something is out of range.  A sequence whose rows do not lie in the step, are
  * more than max_new, or whose length its table cannot hold, is left out (its outputs stay as they are); a page that is none is not touched,
- * and what attention says of its sequence means nothing.  Other sequences of the step are not affected. */
+ * and what attention says of its sequence means nothing.  Other sequences of the step are not affected, but where token_start goes back, append
+ * and gather may leave out rows of others too. */
 typedef struct skn_paged_batch {
     int32_t n_seqs, n_tokens;        /* at most 65535; n_tokens: rows of k, v, q and out, at most 2^24 */
     int32_t max_new;                 /* no sequence has more new tokens (more than n_tokens says no more than n_tokens) */

@@ -69,6 +69,12 @@ struct PagedRows {                                     // rows of the step's tok
     uint8_t *k_pool, *v_pool;
 };
 
+// Row ranges that go back: the search above may miss every row of such a sequence, so each CTA looks at some by itself, with a warp that does not search
+__device__ __forceinline__ void paged_order(const PagedStep &st) {
+    for (int s = blockIdx.x * 32 + (threadIdx.x & 31); s < st.n_seqs; s += gridDim.x * 32)
+        if (st.starts[s] > st.starts[s + 1]) *st.status = SKN_ERR_ARG;
+}
+
 struct PagedPlace { int pos, page, row; };             // of a token: its position (negative: nowhere), page (negative: none) and row of the page
 // by a whole warp
 __device__ __forceinline__ PagedPlace paged_place(const PagedStep &st, int i) {
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(128, 8) skn_paged_append_kernel(const PagedSte
     if (tid < 32) {
         const PagedPlace found = paged_place(st, blockIdx.x);
         if (tid == 0) place = found;
-    }
+    } else if (tid < 64) paged_order(st);
     __syncthreads();
     const PagedPlace at = place;
     if (at.pos < 0) return;
@@ -222,7 +228,7 @@ __global__ void __launch_bounds__(256) skn_paged_gather_kernel(const PagedStep s
     if (threadIdx.x < 32) {
         const PagedPlace found = paged_place(st, blockIdx.x);
         if (threadIdx.x == 0) place = found;
-    }
+    } else if (threadIdx.x < 64) paged_order(st);
     __syncthreads();
     const PagedPlace at = place;
     if (at.page < 0) return;

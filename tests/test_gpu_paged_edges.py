@@ -383,3 +383,19 @@ def test_caches_of_many_and_of_few_heads_at_once():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def test_sequences_out_of_order_are_reported(ctx):
+    """row ranges that go back are reported by every call of the step, whether or not one of its rows is looked for among them"""
+    step = Step(3, [40, 9, 20, 20, 30], [5, 0, 0, 0, 3], 16)
+    cache, _ = filled(ctx, step, 2, 64, "f16", 3)
+    b = step.batch(starts=np.array([0, 5, 3, 3, 3, 8], dtype=np.int32), n=8)          # the second sequence: rows 5 to 3
+    k, q = torch.zeros(8, 2, 64, device="cuda"), torch.zeros(8, 4, 64, device="cuda")
+    out, kk, vv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(k)
+    torch.cuda.synchronize()
+    for call in (lambda: cache.append_dev(b, k, k), lambda: cache.gather_dev(b, kk, vv), lambda: cache.attend_dev(b, q, out)):
+        call()
+        with pytest.raises(skn.SknError, match="out of range"):
+            ctx.sync()
+        ctx.sync()
+    cache.close()

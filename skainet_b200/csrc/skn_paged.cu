@@ -468,6 +468,8 @@ int32_t skn_paged_create(skn_ctx *ctx, const skn_paged_spec *spec, void *k_pool_
         return skn_fail(ctx, SKN_ERR_SHAPE, "%d pages of %d tokens and %d heads are more than 2^31 rows", spec->n_pages, spec->page_tokens, spec->n_kv_heads);
     if (!k_pool_dev != !v_pool_dev) return skn_fail(ctx, SKN_ERR_ARG, "one pool is NULL");
     if (((uintptr_t)k_pool_dev | (uintptr_t)v_pool_dev) & 15) return skn_fail(ctx, SKN_ERR_ALIGN, "pools must be 16-byte aligned");
+    const uintptr_t ka = (uintptr_t)k_pool_dev, va = (uintptr_t)v_pool_dev;
+    if (k_pool_dev && (ka < va ? va - ka : ka - va) < (uintptr_t)pool_bytes_of(spec)) return skn_fail(ctx, SKN_ERR_ARG, "one pool lies over the other");
     skn_paged *pc = new (std::nothrow) skn_paged();
     if (!pc) return skn_fail(ctx, SKN_ERR_OOM, "host allocation failed");
     pc->magic = SKN_MAGIC_PAGED;

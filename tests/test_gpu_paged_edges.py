@@ -399,3 +399,13 @@ def test_sequences_out_of_order_are_reported(ctx):
             ctx.sync()
         ctx.sync()
     cache.close()
+
+
+def test_pools_over_one_another_are_refused(ctx):
+    n = skn.PagedKVCache.pool_bytes(4, 16, 2, 64, "f16")
+    memory = torch.zeros(2 * n, dtype=torch.uint8, device="cuda")
+    for a, b in ((0, 0), (0, n - 16), (n, 16)):
+        with pytest.raises(skn.SknError, match="over the other"):
+            skn.PagedKVCache(ctx, 4, 16, 2, 64, "f16", pools=(memory[a:a + n], memory[b:b + n]))
+    for a, b in ((0, n), (n, 0)):
+        skn.PagedKVCache(ctx, 4, 16, 2, 64, "f16", pools=(memory[a:a + n], memory[b:b + n])).close()

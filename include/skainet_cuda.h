@@ -401,8 +401,9 @@ int32_t skn_paged_gather_dev(skn_paged *pc, const skn_paged_batch *batch, int32_
  * visible has no influence, whatever it holds (a row that sees nothing is zero; one whose scores are all minus infinity is NaN).  At most 64 query
  * heads per kv head; out may not lie over q (rows side by side in wider ones are fine).
  *   fp32 rows: fp32 accuracy.
- *   bf16 rows: softmax weights rounded to fp16 (bf16 caches: bf16, the type that their product takes), fp32 sums.  Queries meet fp16 caches in multiples of 2^-38 of a row's
- *     largest, Q4_0 caches of 2^-34, bf16 caches as they are.  In a step whose max_new times the query heads per kv head is above 32, the
+ *   bf16 rows: fp32 sums.  Softmax weights are rounded to fp16; over bf16 caches to bf16, which is the type that their product takes, or to two terms of it (2^-16) in steps whose
+ *     max_new times the query heads per kv head is 32 or less.  Queries meet fp16 caches in multiples of 2^-38 of a row's largest, Q4_0 caches of 2^-34, bf16 caches as
+ *     they are.  In a step whose max_new times the query heads per kv head is above 32, the
  *     dequantised rows of a Q4_0 cache may be rounded to fp16 as well (rows that see a block with a value above 65504 are computed in fp32 instead,
  *     at about a hundredth of the speed).
  *   Q4_0 caches: weights are multiplied by the values' scales before they are rounded, so that a key's part in a dimension may miss 2^-32 (fp32 rows: 2^-37) of the row's

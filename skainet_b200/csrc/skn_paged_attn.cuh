@@ -8,7 +8,9 @@
 // A unit.  Each of a CTA's eight warps takes every eighth unit through a ring of its own, filled by TMA.  S^T = K q^T with mma.sync (m16n8k16: 16 keys
 // x 8 rows): keys are the operand of 16 so that up to eight query heads waste nothing.  Scores go through one running maximum per row that
 // moves only when a weight would exceed 2^SLACK (one vote a unit instead of six shuffles).  Weights are transposed by movmatrix into the second
-// operand of O^T = V^T p^T.  fp32 rows: queries and weights as sums of two fp16 (fp16 and Q4_0 caches) or three bf16 terms.
+// operand of O^T = V^T p^T.  A product takes operands of one type, the cache's (Q4_0: fp16).  fp32 rows: queries and weights as sums of two fp16 (fp16 and Q4_0 caches) or three
+// bf16 terms.  bf16 rows: queries in one term, weights in one of fp16, whose rounding an output's own hides (relative errors of 1.66e-3 either way), or in two of bf16: with one
+// 2.2e-3, 48 sequences with a window of 4096 133 us instead of 134.
 // The tensor cores cut their sums off instead of rounding them, so for these rows the small terms have an accumulator of their own, the large ones
 // two for the scores, and a unit's output is formed from zero and added in fp32.
 //
@@ -63,7 +65,7 @@ template <class CT> __device__ __forceinline__ void mma_as(float (&c)[4], const 
     if constexpr (std::is_same<CT, __nv_bfloat16>::value) mma_bf16(c, a, b0, b1);
     else mma_f16(c, a, b0, b1);
 }
-// o += a b, b in NT terms; fp32 rows: from zero, small terms first, and then added
+// o += a b, b in NT terms, small ones first; fp32 rows: from zero, and then added
 template <class CT, bool EX, int NT> __device__ __forceinline__ void pa_add(float (&o)[4], const uint32_t (&a)[4], const uint32_t (&b)[NT][2]) {
     if constexpr (EX) {
         float x[4];
@@ -72,8 +74,10 @@ template <class CT, bool EX, int NT> __device__ __forceinline__ void pa_add(floa
         for (int n = NT - 2; n >= 0; --n) mma_as<CT>(x, a, b[n][0], b[n][1]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) o[c] += x[c];
-    } else
-        mma_as<CT>(o, a, b[0][0], b[0][1]);
+    } else {
+#pragma unroll
+        for (int n = NT - 1; n >= 0; --n) mma_as<CT>(o, a, b[n][0], b[n][1]);
+    }
 }
 __device__ __forceinline__ uint32_t movm(uint32_t x) {
     uint32_t y;
@@ -312,7 +316,8 @@ template <class IO> __device__ __forceinline__ void paged_out4(const PagedAttn &
 template <class CT, int D, int NB, bool EX> struct PaTraits {
     static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
     static constexpr int UNIT = Q4 ? 32 : 16;
-    static constexpr int NT = EX ? (BF ? 3 : 2) : 1;
+    static constexpr int NT = EX ? (BF ? 3 : 2) : 1;                              // ... of a query
+    static constexpr int WT = EX ? NT : BF ? 2 : 1;                               // terms of a weight
     // A CTA of eight warps per SM; one row block of eight: CTAs of four, two per SM (Q4_0: four), so that one's queries, pages and results are under way
     // while another computes (64 sequences of 300 tokens 36.9 -> 26.6 us, 16 of 8192 95 -> 96)
     static constexpr int WARPS = NB == 1 ? 4 : 8, THREADS = 32 * WARPS;
@@ -344,7 +349,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                       const __grid_constant__ CUtensorMap mks, const __grid_constant__ CUtensorMap mvs) {
     using T = PaTraits<CT, D, NB, EX>;
     using IO = typename std::conditional<EX, float, __nv_bfloat16>::type;
-    constexpr int UNIT = T::UNIT, NT = T::NT, KS = T::KS, STAGES = T::STAGES, ROWS = T::ROWS, NBLK = D / 32, WARPS = T::WARPS, THREADS = T::THREADS;
+    constexpr int UNIT = T::UNIT, NT = T::NT, WT = T::WT, KS = T::KS, STAGES = T::STAGES, ROWS = T::ROWS, NBLK = D / 32, WARPS = T::WARPS, THREADS = T::THREADS;
     extern __shared__ uint8_t raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     uint2 *qf = reinterpret_cast<uint2 *>(ring + T::BODY);
@@ -916,14 +921,14 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                         }
                     }
                 } else {
-                    uint32_t pb[NB][NT][2];
+                    uint32_t pb[NB][WT][2];
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        uint32_t a[NT], c[NT];
-                        terms_of<CT, NT>(s[nb][0], s[nb][1], a);
-                        terms_of<CT, NT>(s[nb][2], s[nb][3], c);
+                        uint32_t a[WT], c[WT];
+                        terms_of<CT, WT>(s[nb][0], s[nb][1], a);
+                        terms_of<CT, WT>(s[nb][2], s[nb][3], c);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
+                        for (int n = 0; n < WT; ++n) {
                             pb[nb][n][0] = movm(a[n]);
                             pb[nb][n][1] = movm(c[n]);
                         }
@@ -936,7 +941,7 @@ skn_paged_attn_kernel(const __grid_constant__ PagedAttn p, const __grid_constant
                         uint32_t a[4];
                         ldsm4t(a, base + (c >> 3) * 2048 + (((c & 7) ^ (row & 7)) << 4));
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) pa_add<CT, EX, NT>(o[i][nb], a, pb[nb]);
+                        for (int nb = 0; nb < NB; ++nb) pa_add<CT, EX, WT>(o[i][nb], a, pb[nb]);
                     }
                 }
             }

@@ -409,3 +409,24 @@ def test_pools_over_one_another_are_refused(ctx):
             skn.PagedKVCache(ctx, 4, 16, 2, 64, "f16", pools=(memory[a:a + n], memory[b:b + n]))
     for a, b in ((0, n), (n, 0)):
         skn.PagedKVCache(ctx, 4, 16, 2, 64, "f16", pools=(memory[a:a + n], memory[b:b + n])).close()
+
+
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 8), (64, 16), (128, 32)])
+def test_weights_of_single_tokens_over_bf16(ctx, dim, group):
+    """values that nearly cancel: an output's own rounding is small beside that of weights in bf16.  Two terms leave 2^-8 of 2^-8 of a weight."""
+    kv = 2
+    step = Step(5, [2, 5, 33, 300], [1, 1, 1, 1], 16)
+    cache = skn.PagedKVCache(ctx, step.n_pages, 16, kv, dim, "bf16")
+    ref = oracle.Pages(step.n_pages, 16, kv, dim, "bf16")
+    g = np.random.default_rng(dim)
+    total = int(step.lens.sum())
+    k, v = (g.standard_normal((total, kv, dim)).astype(np.float32) for _ in range(2))
+    at = np.concatenate([np.arange(int(x)) for x in step.lens])
+    v = (np.where(at % 2, -8, 8)[:, None, None] + v).astype(np.float32)
+    q = bf16(0.2 * g.standard_normal((step.n, kv * group, dim)))
+    cache.append(k, v, step.table, step.full, step.lens)
+    ref.append(k, v, step.table, step.full, step.lens)
+    want, mass, reach = ref.attend(q, step.table, step.starts, step.lens, 0.125)
+    err = np.abs(run_attend(cache, step, q, "bf16", scale=0.125) - want)
+    assert np.all(err <= tolerance(want, mass, reach, 2.0 ** -16, 0.0, "bf16"))
+    cache.close()

@@ -289,7 +289,7 @@ int32_t skn_status_check(skn_ctx *ctx) {
     const int32_t st = *ctx->h_status;
     if (st != 0) {
         cudaMemsetAsync(ctx->d_status, 0, sizeof(int32_t), ctx->stream);
-        if (st == SKN_ERR_TIMEOUT && ctx->after_timeout) ctx->after_timeout(ctx);
+        if (ctx->after_failure) ctx->after_failure(ctx);        // (whatever it says: one word holds the last of several reports, of which one may be a timeout)
         cudaStreamSynchronize(ctx->stream);
         return skn_fail(ctx, st, "a kernel reported device-side status %d (%s)", st,
                         st == SKN_ERR_TIMEOUT ? "a bounded wait ran out"

@@ -69,7 +69,7 @@ struct skn_ctx {
     // (entry points call one another); a second thread gets SKN_ERR_BUSY
     uint64_t owner;
     int owner_depth;
-    void (*after_timeout)(skn_ctx *);   // sets back what a kernel that gave up leaves behind (paged caches' counters); NULL: nothing
+    void (*after_failure)(skn_ctx *);   // after a report: sets back what a kernel that gave up leaves behind (paged caches' counters); NULL: nothing
     uint64_t entries, quiet_at;  // calls that claimed the context, and the last one after which nothing was left on its stream
     char err[512];
 };

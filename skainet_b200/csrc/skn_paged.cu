@@ -420,7 +420,7 @@ static int32_t enter_host(skn_paged *pc, const skn_paged_batch *b, bool *nothing
 
 // ---- after a wait that ran out ------------------------------------------------------------------------------------------------------
 // A prompt kernel that gives up leaves some of its joins' counters above zero, and the next launch, a captured one too, would join too early.  So
-// the report of a timeout, which every caller gets before it can trust a result again, zeroes the counters of the context's caches.
+// a report of the status, which every caller gets before it can trust a result again, zeroes the counters of the context's caches.
 static pthread_mutex_t caches_lock = PTHREAD_MUTEX_INITIALIZER;
 static skn_paged *caches;
 static void tickets_back(skn_ctx *ctx) {
@@ -435,7 +435,7 @@ static void caches_add(skn_paged *pc) {
     pc->next = caches;
     caches = pc;
     pthread_mutex_unlock(&caches_lock);
-    pc->ctx->after_timeout = tickets_back;
+    pc->ctx->after_failure = tickets_back;
 }
 static void caches_remove(const skn_paged *pc) {
     pthread_mutex_lock(&caches_lock);

@@ -430,3 +430,22 @@ def test_weights_of_single_tokens_over_bf16(ctx, dim, group):
     err = np.abs(run_attend(cache, step, q, "bf16", scale=0.125) - want)
     assert np.all(err <= tolerance(want, mass, reach, 2.0 ** -16, 0.0, "bf16"))
     cache.close()
+
+
+def test_a_timeout_behind_another_report_sets_a_cache_back(ctx):
+    """the status word holds the last of several reports: here rows out of range, after counters were left above zero"""
+    step = Step(5, [5000, 40], [50, 1], 32)
+    cache, _ = filled(ctx, step, 2, 128, "bf16", 5)
+    q = bf16(np.random.default_rng(1).standard_normal((step.n, 8, 128)))
+    want = run_attend(cache, step, q, "bf16")
+    cuda, at, size = _counters(cache)
+    torch.cuda.synchronize()
+    assert cuda.cuMemsetD32_v2(ctypes.c_uint64(at), ctypes.c_uint32(2 ** 31), ctypes.c_size_t(size // 4)) == 0
+    k = torch.zeros(step.n, 2, 128, device="cuda")
+    torch.cuda.synchronize()
+    cache.gather_dev(step.batch(lens=[9000, 40]), k, torch.zeros_like(k))
+    with pytest.raises(skn.SknError, match="out of range"):
+        ctx.sync()
+    for _ in range(2):
+        assert np.array_equal(run_attend(cache, step, q, "bf16"), want)
+    cache.close()

@@ -29,10 +29,6 @@ constexpr int PP_ROWS = 256, PP_KEYS = 128;
 // units that a block's start and end are worth on the line (2: a prompt of 8192 tokens 705 us, 3: 593, 4: 512, 6: 507, 9: 519; 16 of 1024: 331, 310, 298, 309, 312)
 constexpr int PP_COST = 4;
 
-// A segment that is computed again takes 3.3 us a key, and the CTA's other warps wait for two seconds: longer ones than this are left to the end of the
-// share, up to PP_LATE - 1 of them (with more, 600 thousand keys of the next one are too many: the call reports that a wait ran out)
-constexpr int PP_LATE_UNITS = 512, PP_LATE = 32;
-
 template <class CT, int D> struct PpTraits {
     static constexpr bool Q4 = sizeof(CT) == 1, BF = std::is_same<CT, __nv_bfloat16>::value;
     static constexpr int THREADS = Q4 ? 512 : 384;                // two softmax warpgroups, one of MMA / TMA / clearing, one of unpacking
@@ -119,79 +115,9 @@ __device__ __forceinline__ uint64_t pp_ex2_pair(uint64_t x) {
     return skn_pack2(pp_ex2(a), pp_ex2(b));
 }
 
-// This thread's row R of a block from the parts that its CTAs left; none: what a row without a weight is
-template <int D> __device__ __forceinline__ void pp_join(float *parts, const PagedSegment &now, int R, __nv_bfloat16 *out, uint32_t none, bool wide) {
-    auto part_of = [&](int k) { return parts + (int64_t)paged_slot(now, now.c0 + min(k, now.n_parts - 1)) * PP_ROWS * (D + 4); };
-    float top = PA_NONE, sum = 0.f;
-    for (int k = 0; k < now.n_parts; ++k) top = fmaxf(top, __ldcg(part_of(k) + D * PP_ROWS + R));
-    for (int k = 0; k < now.n_parts; ++k) sum = fmaf(__ldcg(part_of(k) + (D + 1) * PP_ROWS + R), exp2f(__ldcg(part_of(k) + D * PP_ROWS + R) - top), sum);
-    const float inv = 1.f / sum;
-#pragma unroll 1
-    for (int c = 0; c < D; c += 16) {
-        float4 o[4] = {};
-        for (int k = 0; k < now.n_parts; k += 4) {       // four parts' loads on their way at once
-            float4 y[4][4];
-            float f[4];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                f[b] = k + b < now.n_parts ? exp2f(__ldcg(part_of(k + b) + D * PP_ROWS + R) - top) : 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[b][e] = __ldcg(reinterpret_cast<const float4 *>(part_of(k + b)) + (c / 4 + e) * PP_ROWS + R);
-            }
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-                if (f[b] != 0.f)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        o[e].x = fmaf(y[b][e].x, f[b], o[e].x); o[e].y = fmaf(y[b][e].y, f[b], o[e].y);
-                        o[e].z = fmaf(y[b][e].z, f[b], o[e].z); o[e].w = fmaf(y[b][e].w, f[b], o[e].w);
-                    }
-        }
-        uint32_t y[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            y[2 * e] = sum == 0.f ? none : pack_bf16(o[e].x * inv, o[e].y * inv);
-            y[2 * e + 1] = sum == 0.f ? none : pack_bf16(o[e].z * inv, o[e].w * inv);
-        }
-        pp_store32(out + c, y, wide);
-    }
-}
-// Blocks with a result that is not finite, from the definition, by the softmax warps (out of line: nothing of it in the others' registers)
-template <class CT, int D>
-__device__ __noinline__ void pp_again(const PagedAttn &p, const PagedSegment *list, int n, PagedScratch<D, 256> &scratch, unsigned &ticket) {
-    using IO = __nv_bfloat16;
-    const int tid = threadIdx.x;
-    pp_bar();                                    // (the list is there)
-    for (int i = 0; i < n; ++i) {
-        const PagedSegment now = list[i];
-        const bool shared = now.n_parts > 1;
-        float *const part = p.parts + (int64_t)now.slot * PP_ROWS * (D + 4);
-        paged_redo<CT, D, 256, IO>(p, now, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p, &now](int row, float rm, float rl, float acc) {
-            const int t = (now.row0 + row) / p.group;
-            if (shared) {
-                if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;
-                if (tid == 0) {
-                    part[D * PP_ROWS + row] = rm + PpTraits<CT, D>::LIFT;      // (its weights are not lifted)
-                    part[(D + 1) * PP_ROWS + row] = rl;
-                }
-            } else if (tid < D)
-                static_cast<IO *>(p.out)[(int64_t)(now.first + t) * p.out_stride + (now.head * p.group + (now.row0 + row) % p.group) * D + tid] =
-                    __float2bfloat16_rn(rl != 0.f ? acc / rl : now.len - now.n + t < 0 ? 0.f : NAN);
-        });
-        if (!shared) continue;
-        __threadfence();
-        pp_bar();
-        if (tid == 0) ticket = atomicInc(&p.tickets[paged_slot(now, now.c0)], (unsigned)now.n_parts - 1);
-        pp_bar();
-        if (ticket == (unsigned)now.n_parts - 1 && tid < now.rows) {
-            __threadfence();
-            const int t = (now.row0 + tid) / p.group;
-            IO *const out = static_cast<IO *>(p.out) + (int64_t)(now.first + t) * p.out_stride + (now.head * p.group + (now.row0 + tid) % p.group) * D;
-            pp_join<D>(p.parts, now, tid, out, now.len - now.n + t < 0 ? 0u : 0x7FFF7FFFu, false);
-        }
-        pp_bar();
-    }
-}
+// The kernel's waits: two seconds are enough for anything but a segment that is computed again (3.3 us a key), for which the other warps wait.  A minute is 18 million keys.
+constexpr uint64_t PP_WAIT_NS = 60000000000ull;
+__device__ __forceinline__ bool pp_wait(uint64_t *bar, uint32_t parity, int lane) { return tc_wait_warp<PP_WAIT_NS>(bar, parity, lane); }
 
 // A CTA's share of the line, segment by segment: one warp walks it ahead of the others and leaves the segments in shared memory
 struct PpWalk {
@@ -283,8 +209,6 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     __shared__ unsigned ticket;
     __shared__ int starts[THREADS + 1];
     __shared__ PagedScratch<D, 256> scratch;
-    __shared__ alignas(16) PagedSegment late[PP_LATE];        // to be computed again
-    __shared__ int n_late;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const PagedStep &st = p.st;
 
@@ -310,7 +234,6 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         }
         skn_fence_mbar_init();
         found[0] = -1;
-        n_late = 0;
     }
 
     if (p.split) skn_pdl_launch_dependents();        // the launch for short sequences may take the SMs that this one leaves
@@ -411,7 +334,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
     bool got = true;                                 // no wait for a segment has run out
     auto take = [&] {                                // the next segment, by a whole warp
         const uint32_t i = n_taken & 3;
-        got = got && tc_wait_warp(&seg_full[i], n_taken >> 2 & 1, lane);
+        got = got && pp_wait(&seg_full[i], n_taken >> 2 & 1, lane);
         if (!got) return false;
         g = seg_ring[i];
         __syncwarp();
@@ -489,7 +412,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
 
                 for (int j = 0; j < now.u1 - now.u0; ++j, ++n_units) {
                     const int i = now.u0 + j, k0 = (i < now.span.a ? i : i + now.span.gap) * PP_KEYS;
-                    if (!tc_wait_warp(&s_full[tile], n_units & 1, lane)) { ok = false; break; }
+                    if (!pp_wait(&s_full[tile], n_units & 1, lane)) { ok = false; break; }
                     tc_fence_after();
                     float v[PP_KEYS];
 #pragma unroll
@@ -520,7 +443,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                         m = fresh;
                         l *= fix;
                         if (j > 0) {
-                            if (!tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane)) { ok = false; break; }
+                            if (!pp_wait(&pv_done[tile], (n_units - 1) & 1, lane)) { ok = false; break; }
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < D; c += 32) {
@@ -568,7 +491,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             IO *const out = static_cast<IO *>(p.out) + (int64_t)(now.first + t) * p.out_stride + (now.head * p.group + (now.row0 + R) % p.group) * D;
             bool odd = false;
             if (used) {
-                if (ok) ok = tc_wait_warp(&pv_done[tile], (n_units - 1) & 1, lane);
+                if (ok) ok = pp_wait(&pv_done[tile], (n_units - 1) & 1, lane);
                 if (!(ok && got) && lane == 0) *st.status = SKN_ERR_TIMEOUT;
                 tc_fence_after();
                 const float inv = 1.f / l;
@@ -608,15 +531,19 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             }
             if (pp_any(!got)) more = false;
             if (pp_any(odd)) {
-                const int k = n_late;
-                const bool later = now.u1 - now.u0 > PP_LATE_UNITS && k < PP_LATE - 1;
-                pp_bar();                            // (n_late is read)
-                if (tid == 0) {
-                    late[k] = now;
-                    if (later) n_late = k + 1;
-                }
-                if (!later) pp_again<CT, D>(p, late + k, 1, scratch, ticket);
-                continue;
+                const PagedSegment again = now;      // (a copy: the address of the one that the loops use is not taken)
+                paged_redo<CT, D, 256, IO>(p, again, PP_KEYS, scratch, [] { pp_bar(); }, [=, &p](int row, float rm, float rl, float acc) {
+                    const int tr = (now.row0 + row) / p.group;
+                    if (shared) {
+                        if (tid < D) part[((tid / 4) * PP_ROWS + row) * 4 + (tid & 3)] = acc;
+                        if (tid == 0) {
+                            part[D * PP_ROWS + row] = rm + T::LIFT;      // (its weights are not lifted)
+                            part[(D + 1) * PP_ROWS + row] = rl;
+                        }
+                    } else if (tid < D)
+                        static_cast<IO *>(p.out)[(int64_t)(now.first + tr) * p.out_stride + (now.head * p.group + (now.row0 + row) % p.group) * D + tid] =
+                            __float2bfloat16_rn(rl != 0.f ? acc / rl : now.len - now.n + tr < 0 ? 0.f : NAN);
+                });
             }
             if (shared) {
                 __threadfence();
@@ -625,13 +552,45 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 pp_bar();
                 if (ticket == (unsigned)now.n_parts - 1 && real) {
                     __threadfence();
-                    pp_join<D>(p.parts, now, R, out, now.len - now.n + t < 0 ? 0u : 0x7FFF7FFFu, wide);
+                    auto part_of = [&](int k) { return p.parts + (int64_t)paged_slot(now, now.c0 + min(k, now.n_parts - 1)) * PP_ROWS * (D + 4); };
+                    float top = PA_NONE, sum = 0.f;
+                    for (int k = 0; k < now.n_parts; ++k) top = fmaxf(top, __ldcg(part_of(k) + D * PP_ROWS + R));
+                    for (int k = 0; k < now.n_parts; ++k) sum = fmaf(__ldcg(part_of(k) + (D + 1) * PP_ROWS + R), exp2f(__ldcg(part_of(k) + D * PP_ROWS + R) - top), sum);
+                    const float inv = 1.f / sum;
+                    const uint32_t none = now.len - now.n + t < 0 ? 0u : 0x7FFF7FFFu;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        float4 o[4] = {};
+                        for (int k = 0; k < now.n_parts; k += 4) {       // four parts' loads on their way at once
+                            float4 y[4][4];
+                            float f[4];
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                f[b] = k + b < now.n_parts ? exp2f(__ldcg(part_of(k + b) + D * PP_ROWS + R) - top) : 0.f;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) y[b][e] = __ldcg(reinterpret_cast<const float4 *>(part_of(k + b)) + (c / 4 + e) * PP_ROWS + R);
+                            }
+#pragma unroll
+                            for (int b = 0; b < 4; ++b)
+                                if (f[b] != 0.f)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        o[e].x = fmaf(y[b][e].x, f[b], o[e].x); o[e].y = fmaf(y[b][e].y, f[b], o[e].y);
+                                        o[e].z = fmaf(y[b][e].z, f[b], o[e].z); o[e].w = fmaf(y[b][e].w, f[b], o[e].w);
+                                    }
+                        }
+                        uint32_t y[8];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            y[2 * e] = sum == 0.f ? none : pack_bf16(o[e].x * inv, o[e].y * inv);
+                            y[2 * e + 1] = sum == 0.f ? none : pack_bf16(o[e].z * inv, o[e].w * inv);
+                        }
+                        pp_store32(out + c, y, wide);
+                    }
                 }
                 pp_bar();                            // (the ticket is read)
             }
         }
-        pp_bar();
-        if (n_late) pp_again<CT, D>(p, late, n_late, scratch, ticket);       // (no other warp waits any more)
     }
     // ---- MMAs: warp 8 --------------------------------------------------------------------------------------------------------
     else if (warp < 12) {
@@ -663,8 +622,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         while (ok && take()) {
             const int n = g.u1 - g.u0, tiles = g.rows > 128 ? 2 : 1;
             int k_slot = slot;
-            for (int x = 0; x < tiles && ok; ++x) ok = tc_wait_warp(&q_full[x], segs[x] & 1, lane);
-            ok = ok && tc_wait_warp(&full[slot], parity, lane);
+            for (int x = 0; x < tiles && ok; ++x) ok = pp_wait(&q_full[x], segs[x] & 1, lane);
+            ok = ok && pp_wait(&full[slot], parity, lane);
             if (!ok) break;
             tc_fence_after();
             for (int x = 0; x < tiles; ++x) scores(x, slot);
@@ -673,15 +632,15 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             step();
             for (int j = 0; j < n && ok; ++j) {
                 const int v_slot = slot;
-                ok = tc_wait_warp(T::Q4 ? &full[slot] : &clean[slot], parity, lane);
+                ok = pp_wait(T::Q4 ? &full[slot] : &clean[slot], parity, lane);
                 step();
                 const bool more = j + 1 < n;
                 k_slot = slot;
                 const uint32_t va = skn_smem_u32(ring + v_slot * TILE);
                 for (int x = 0; x < tiles && ok; ++x) {
                     for (int h = 0; h < 2 && ok; ++h) {          // the weights come in halves
-                        ok = tc_wait_warp(&p_full[2 * x + h], units[x] & 1, lane);
-                        if (ok && j == 0 && h == 0 && segs[x] > 0) ok = tc_wait_warp(&o_free[x], (segs[x] - 1) & 1, lane);
+                        ok = pp_wait(&p_full[2 * x + h], units[x] & 1, lane);
+                        if (ok && j == 0 && h == 0 && segs[x] > 0) ok = pp_wait(&o_free[x], (segs[x] - 1) & 1, lane);
                         if (!ok) break;
                         tc_fence_after();
                         if (tc_elect()) {
@@ -698,7 +657,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     if (!ok) break;
                     ++units[x];
                     if (more) {
-                        if (x == 0) ok = tc_wait_warp(&full[k_slot], parity, lane);
+                        if (x == 0) ok = pp_wait(&full[k_slot], parity, lane);
                         if (!ok) break;
                         tc_fence_after();
                         scores(x, k_slot);
@@ -739,7 +698,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 for (int kv = 0; kv < 2 && ok; ++kv) {
                     const CUtensorMap *map = kv ? &mv : &mk;
                     if constexpr (!T::Q4) {
-                        if (loads >= (uint32_t)SLOTS) ok = tc_wait_warp(&empty[slot], parity ^ 1, lane);
+                        if (loads >= (uint32_t)SLOTS) ok = pp_wait(&empty[slot], parity ^ 1, lane);
                         if (!ok) break;
                         uint8_t *dst = ring + slot * TILE;
                         if (lane == 0) {
@@ -757,7 +716,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                             parity ^= 1;
                         }
                     } else {
-                        if (loads >= 4) ok = tc_wait_warp(&raw_empty[slot], parity ^ 1, lane);
+                        if (loads >= 4) ok = pp_wait(&raw_empty[slot], parity ^ 1, lane);
                         if (!ok) break;
                         uint8_t *dst = raw_ring + slot * T::RAW + ((b << box_shift) >> 4) * T::HALF;
                         if (lane == 0) {
@@ -801,7 +760,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
             const int seen_from = p.window ? max(0, max(0, pmin) - p.window + 1) : 0;
             for (int j = 0; j < g.u1 - g.u0 && ok; ++j) {
                 step();                              // K
-                ok = tc_wait_warp(&full[slot], parity, lane);
+                ok = pp_wait(&full[slot], parity, lane);
                 if (!ok) break;
                 if (pp_hides(p, g, j)) {
                     const int i = g.u0 + j, k0 = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS;
@@ -826,7 +785,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
         for (bool more = true; more; ++k) {
             more = pp_next(p, w, g);
             if (!more) g.rows = 0;
-            if (k >= 4 && !tc_wait_warp(&seg_empty[k & 3], (k >> 2 & 1) ^ 1, lane)) {
+            if (k >= 4 && !pp_wait(&seg_empty[k & 3], (k >> 2 & 1) ^ 1, lane)) {
                 ok = false;
                 break;
             }
@@ -853,8 +812,8 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                 const int i = g.u0 + j, key = (i < g.span.a ? i : i + g.span.gap) * PP_KEYS + row;
                 const bool need = key <= pmax && (key >= seen_from || key < p.sinks);
                 for (int kv = 0; kv < 2; ++kv) {
-                    ok = tc_wait_warp(&raw_full[raw], raw_parity, lane);
-                    if (ok && tiles >= (uint32_t)SLOTS) ok = tc_wait_warp(&empty[slot], parity ^ 1, lane);
+                    ok = pp_wait(&raw_full[raw], raw_parity, lane);
+                    if (ok && tiles >= (uint32_t)SLOTS) ok = pp_wait(&empty[slot], parity ^ 1, lane);
                     if (!ok) break;
                     const int box_shift = min(st.page_shift, 5), in = row & ((1 << box_shift) - 1);
                     const uint8_t *src = raw_ring + raw * T::RAW + ((row - in) >> 4) * T::HALF;

@@ -48,8 +48,9 @@ __device__ __forceinline__ uint64_t skn_globaltimer_ns() {
     return t;
 }
 
-// Bounded wait: gives up after ~2 s of wall time and returns false.  The caller records
+// Bounded wait: gives up after LIMIT_NS (~2 s) of wall time and returns false.  The caller records
 // the failure in the status word and skips the work that depended on the data.
+template <uint64_t LIMIT_NS = 2000000000ull>
 __device__ __forceinline__ bool skn_mbar_wait(uint64_t *bar, uint32_t parity) {
     if (skn_mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = skn_globaltimer_ns();
@@ -57,7 +58,7 @@ __device__ __forceinline__ bool skn_mbar_wait(uint64_t *bar, uint32_t parity) {
 #pragma unroll 1
         for (int i = 0; i < 1024; ++i)
             if (skn_mbar_try_wait(bar, parity)) return true;
-        if (skn_globaltimer_ns() - t0 > 2000000000ull) return false;
+        if (skn_globaltimer_ns() - t0 > LIMIT_NS) return false;
     }
 }
 

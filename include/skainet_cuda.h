@@ -248,7 +248,7 @@ int32_t skn_kv_create(skn_ctx *ctx, int32_t batch, int32_t n_kv_heads, int32_t h
 #define SKN_KV_F32 0
 #define SKN_KV_F16 1
 #define SKN_KV_Q8_0 2
-#define SKN_KV_BF16 3 /* position-addressed caches only (skn_kv_create_by_position) */
+#define SKN_KV_BF16 3 /* position-addressed caches (skn_kv_create_by_position) and paged ones; rows of skn_paged_* calls */
 int32_t skn_kv_create_typed(skn_ctx *ctx, int32_t batch, int32_t n_kv_heads, int32_t head_dim, int32_t capacity,
                             int32_t kv_dtype, skn_kvcache **out);
 /* A position-addressed cache: the token at position p of sequence b occupies slot p % capacity of

@@ -9,9 +9,9 @@
 // A CTA takes one token.  Where it goes is looked up and the sines and cosines of its position are formed once, in shared memory (in 64 bits: the angle of
 // a far position, and keys that land next to a border of the cache's rounding); its threads take 16 dimensions of a head at a time, eight and the
 // eight they turn with, so that the rotation may happen in place.  The rows are requested a unit ahead, the first before all that.
-// Bound by HBM from a few thousand tokens on.  8192 tokens of 32 + 2 x 8 heads of 128, all of them turned: bf16 rows and cache 36.9 us (5.5 TB/s), fp32 rows and
-// a cache of 4 bits 63.1 us (5.5 TB/s); with requests behind the sines 96 us for the first; with four tokens to a CTA of 256 threads 41.4 and 68.3 us, no faster
-// for any smaller step (512 tokens 8.6 us instead of 8.1), and the same for the way back (20.5 us instead of 19.0).  Alone, a token is 3 us of latency.
+// Bound by HBM from a few thousand tokens on.  8192 tokens of 32 + 2 x 8 heads of 128, all of them turned: bf16 rows and cache 37.3 us (5.4 TB/s), fp32 rows and
+// a cache of 4 bits 62.6 us (5.5 TB/s); with requests behind the sines 96 us for the first; with four tokens to a CTA of 256 threads 41.4 and 68.3 us, no faster
+// for any smaller step (512 tokens 8.6 us instead of 8.1).  Alone, a token is 3 us of latency.
 
 // sequence of row i: the last one that starts at or before it (-1: none).  Every warp counts the starts for itself: 32 of them at even distances, then
 // those between two of these.  (One after the other, 32 at a time, they are a chain of loads as long as the batch.)
@@ -222,6 +222,8 @@ __global__ void __launch_bounds__(128, 8) skn_paged_append_kernel(const PagedSte
 }
 
 // ---- gather ---------------------------------------------------------------------------------------------------------------
+// A CTA takes one token here too: 8192 of 2 x 8 heads of 128 to fp32 rows from bf16 21.6 us (4.7 TB/s), from 4 bits 20.7 us (3.7 TB/s: the look-up and the loads of a token
+// follow one another)
 template <class CT, int D, class IO>
 __global__ void __launch_bounds__(256) skn_paged_gather_kernel(const PagedStep st, const uint8_t *k_pool, const uint8_t *v_pool, IO *k_out, IO *v_out) {
     __shared__ PagedPlace place;

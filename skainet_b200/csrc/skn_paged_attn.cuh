@@ -5,7 +5,7 @@
 // unequal lengths keeps every SM at work to the end; a segment that lies in several CTAs leaves partial results (maximum, sum,
 // unnormalised output), which the last of them to finish joins in order.
 //
-// A unit.  Each of a CTA's eight warps takes every eighth unit through a ring of its own, filled by TMA.  S^T = K q^T with mma.sync (m16n8k16: 16 keys
+// A unit.  Each of a CTA's warps (four for up to eight rows, else eight) takes every fourth or eighth unit through a ring of its own, filled by TMA.  S^T = K q^T with mma.sync (m16n8k16: 16 keys
 // x 8 rows): keys are the operand of 16 so that up to eight query heads waste nothing.  Scores go through one running maximum per row that
 // moves only when a weight would exceed 2^SLACK (one vote a unit instead of six shuffles).  Weights are transposed by movmatrix into the second
 // operand of O^T = V^T p^T.  A product takes operands of one type, the cache's (Q4_0: fp16).  fp32 rows: queries and weights as sums of two fp16 (fp16 and Q4_0 caches) or three
@@ -24,10 +24,10 @@
 // (a key that some rows see and others do not; an infinity that meets the two terms of a weight) leaves a result that is not finite,
 // and a segment with one is computed again straight from the definition (paged_redo).
 //
-// 16-bit caches are bound by HBM: 16 sequences of 8192 tokens, 32 / 8 heads of 128, 97 us for fp32 rows and 95 us for bf16 ones (5.5 and 5.7 TB/s, 0.86 of a copy's
-// rate), 48 sequences with a window of 4096 135 us (6.0 TB/s).  Q4_0 by its instructions: 64 sequences of 16384, bf16 rows, 393 us (3.1 TB/s; 59 % of the
-// issue slots, the ALU pipe at 51 %: masks, permutes and conversions of V), fp32 rows, with two terms of everything, half as fast.  One sequence of
-// 100 tokens is 8 us of latency.  Shares smaller than the CTAs that run at a time (twice as many) cost 95 -> 101 us: every share has a beginning.
+// 16-bit caches are bound by HBM: 16 sequences of 8192 tokens, 32 / 8 heads of 128, fp16 pages 97 us for fp32 rows and 95 us for bf16 ones (5.5 and 5.7 TB/s, 0.86 of a copy's
+// rate), bf16 pages 99 and 96, 48 sequences with a window of 4096 134 us (6.0 TB/s).  Q4_0: 64 sequences of 16384, bf16 rows, 393 us (3.1 TB/s; 62 % of the
+// issue slots, the ALU pipe at 57 %: masks, permutes and conversions of V; neither is at its end), 16 of 8192 71 us, with fp32 rows, two terms of everything, 103.  One sequence
+// of 100 tokens is 8 us of latency, 1024 of one's 4100 20 us in a graph.  Shares smaller than the CTAs that run at a time (twice as many) cost 95 -> 101 us: every share has a beginning.
 #pragma once
 #include "skn_paged.cuh"
 #include "skn_mma.cuh"
@@ -35,8 +35,8 @@
 
 #include <math.h>
 
-// Sequences whose work is shared out (their places are in shared memory); more of them take a CTA per segment.  300 sequences: of 1000 tokens each 195 us
-// shared out, 183 as CTAs; of 500 and one of 32768 133 us against 447.
+// Sequences whose work is shared out: as many as have room for their places in shared memory; a step of more takes a CTA per segment.  That is the room's border, not one of
+// speed: 300 sequences of 1000 tokens each take 195 us shared out and 183 as CTAs, 510 of 500 and one of 32768 198 us, 600 and that one (as CTAs) 558.
 constexpr int PA_MAX_SEQS = 512;
 constexpr float PA_NONE = -3.402823466e38f;  // running maximum before the first score: the lowest number, so that no score is below it
 

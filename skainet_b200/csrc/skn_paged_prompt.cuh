@@ -11,7 +11,7 @@
 //
 // Work is shared out as in skn_paged_attn.cuh: the units (128 keys of a block of rows) of all blocks form one line, one contiguous share for each CTA;
 // blocks that lie in several shares are joined by the last of their CTAs to finish.  One warp walks the line for all the others (each for itself
-// held its state in registers, which the softmax warps had to spill: 544 -> 512 us).
+// held its state in registers, which the softmax warps had to spill: 544 -> 512 us; the kernel of Q4_0, at 128 registers, still spills 140 bytes).
 //
 // Hidden rows of V (behind the last key that the block sees, before its window, on pages that were given back) are cleared in shared memory before the
 // product: a warp does it in the few units that have some.  A result that is not finite is computed again from the definition.  Q4_0: fp16 holds
@@ -20,7 +20,7 @@
 //
 // Bound by the chain of a tile (scores, softmax, products, each waiting for the one before) at about half of what the exponentials and the products
 // would each take alone.  32 / 8 heads of 128, bf16: a prompt of 8192 tokens 495 us (1110 TFLOP/s, 0.66 of the measured burst), 512 tokens behind 16383 cached
-// ones 143 us (970), in 4 bits 182 us; heads of 64: 114 us (610 TFLOP/s: as many exponentials for half the products).  64 tokens alone: 15 us, of which
+// ones 145 us (960), in 4 bits 182 us; heads of 64: 113 us (615 TFLOP/s: as many exponentials for half the products).  64 tokens alone: 15 us, of which
 // 7 before the first product (launch, the line, the first segment, queries).
 #pragma once
 #include "skn_paged_attn.cuh"
@@ -96,12 +96,6 @@ __device__ __forceinline__ void pp_store32(__nv_bfloat16 *to, const uint32_t *y,
         reinterpret_cast<uint4 *>(to)[1] = make_uint4(y[4], y[5], y[6], y[7]);
     }
 }
-__device__ __forceinline__ float pp_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ float pp_max3(float a, float b, float c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -112,7 +106,7 @@ __device__ __forceinline__ float pp_max3(float a, float b, float c) {
 __device__ __forceinline__ uint64_t pp_ex2_pair(uint64_t x) {
     float a, b;
     skn_unpack2(x, a, b);
-    return skn_pack2(pp_ex2(a), pp_ex2(b));
+    return skn_pack2(pa_ex2(a), pa_ex2(b));
 }
 
 // The kernel's waits: two seconds are enough for anything but a segment that is computed again (3.3 us a key), for which the other warps wait.  A minute is 18 million keys.
@@ -439,7 +433,7 @@ skn_paged_prompt_kernel(const __grid_constant__ PagedAttn p, const __grid_consta
                     if (top != top) l = top;
                     top *= cs;
                     if (__any_sync(0xffffffffu, top > m + (float)T::SLACK)) {
-                        const float fresh = fmaxf(m, top), fix = pp_ex2(m - fresh);
+                        const float fresh = fmaxf(m, top), fix = pa_ex2(m - fresh);
                         m = fresh;
                         l *= fix;
                         if (j > 0) {

@@ -340,7 +340,8 @@ int32_t skn_attn_causal_dev(skn_kvcache *kv, const float *q_dev, int32_t n_q_hea
  *   SKN_KV_Q4_0: quants [head_dim / 32][page_tokens][16 bytes], then scales [page_tokens][head_dim / 32] fp16.  Per 32 dims, with m their
  *     value of largest size (the first of equals): d = m / -8, q = trunc(x * fp32(1 / d) + 8.5) in 64 bits, at most 15, read back as
  *     (q - 8) * fp16(d); byte j holds q[j] and, in its upper half, q[j + 16] (GGUF's Q4_0).  An all-zero block has d = 0.
- * Rows are rounded once, to nearest even, from fp32.  Rotated keys are formed in 64 bits and rounded to fp32 first. */
+ * Rows are rounded once, to nearest even, from fp32.  Rotated keys are formed in 64 bits and rounded to fp32 first,
+ * rotated queries formed in 64 bits and rounded once. */
 typedef struct skn_paged skn_paged;
 #define SKN_KV_Q4_0 4       /* paged caches only */
 #define SKN_ROT_ADJACENT 0  /* dimension 2 i turns with 2 i + 1 */

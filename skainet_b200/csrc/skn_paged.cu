@@ -7,7 +7,8 @@
 
 // ---- append -------------------------------------------------------------------------------------------------------------
 // A CTA takes one token.  Where it goes is looked up and the sines and cosines of its position are formed once, in shared memory (in 64 bits: the angle of
-// a far position, and keys that land next to a border of the cache's rounding); its threads take 16 dimensions of a head at a time, eight and the
+// a far position, and keys that land next to a border of the cache's rounding; queries too: with fp32 sines they are off by 3.8e-8 instead of their own rounding's
+// 2.5e-8, and six prompts of 7500 tokens in bf16 take 36.5 us instead of 37.5); its threads take 16 dimensions of a head at a time, eight and the
 // eight they turn with, so that the rotation may happen in place.  The rows are requested a unit ahead, the first before all that.
 // Bound by HBM from a few thousand tokens on.  8192 tokens of 32 + 2 x 8 heads of 128, all of them turned: bf16 rows and cache 37.3 us (5.4 TB/s), fp32 rows and
 // a cache of 4 bits 62.6 us (5.5 TB/s); with requests behind the sines 96 us for the first; with four tokens to a CTA of 256 threads 41.4 and 68.3 us, no faster
@@ -91,19 +92,19 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedStep &st, int i) {
     return at;
 }
 
-// eight dimensions and the eight they turn with, by fp32 or (keys) fp64 sines; c: the unit of 16.  Pair 8 c + i lies at [i][c]: the units of a
+// eight dimensions and the eight they turn with, in 64 bits; c: the unit of 16.  Pair 8 c + i lies at [i][c]: the units of a
 // head are neighbouring lanes (at [8 c + i] they met in the same banks: with four tokens to a CTA 8192 of them took 52 us instead of 43)
-template <int UNITS, class F2, class F> __device__ __forceinline__ void paged_turn(float (&x)[8], float (&y)[8], const F2 *turn, int c, bool halves) {
+template <int UNITS> __device__ __forceinline__ void paged_turn(float (&x)[8], float (&y)[8], const double2 *turn, int c, bool halves) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (halves) {
-            const F2 t = turn[j * UNITS + c];
-            const F a = x[j], b = y[j];
+            const double2 t = turn[j * UNITS + c];
+            const double a = x[j], b = y[j];
             x[j] = (float)(a * t.x - b * t.y);
             y[j] = (float)(a * t.y + b * t.x);
         } else if (!(j & 1)) {
-            const F2 t = turn[(j >> 1) * UNITS + c], w = turn[(4 + (j >> 1)) * UNITS + c];
-            const F x0 = x[j], x1 = x[j + 1], y0 = y[j], y1 = y[j + 1];
+            const double2 t = turn[(j >> 1) * UNITS + c], w = turn[(4 + (j >> 1)) * UNITS + c];
+            const double x0 = x[j], x1 = x[j + 1], y0 = y[j], y1 = y[j + 1];
             x[j] = (float)(x0 * t.x - x1 * t.y);
             x[j + 1] = (float)(x0 * t.y + x1 * t.x);
             y[j] = (float)(y0 * w.x - y1 * w.y);
@@ -140,7 +141,6 @@ __global__ void __launch_bounds__(128, 8) skn_paged_append_kernel(const PagedSte
     constexpr int THREADS = 128, UNITS = D / 16;
     extern __shared__ float staged[];                  // Q4: the rotated keys, [heads][D]
     __shared__ double2 turn[D / 2];
-    __shared__ float2 turn32[D / 2];
     __shared__ PagedPlace place;
     const int tid = threadIdx.x, n_units = (r.q_heads + (Q4 ? 1 : 2) * st.heads) * UNITS;
     const int64_t t = blockIdx.x;
@@ -176,9 +176,7 @@ __global__ void __launch_bounds__(128, 8) skn_paged_append_kernel(const PagedSte
     for (int i = tid; i < r.rot / 2; i += THREADS) {
         double2 x;
         sincospi((double)at.pos * r.turns[i], &x.y, &x.x);
-        const int to = (i & 7) * UNITS + (i >> 3);
-        turn[to] = x;
-        turn32[to] = make_float2((float)x.x, (float)x.y);
+        turn[(i & 7) * UNITS + (i >> 3)] = x;
     }
     __syncthreads();
     for (int u = tid; u < n_units; u += THREADS) {
@@ -189,10 +187,7 @@ __global__ void __launch_bounds__(128, 8) skn_paged_append_kernel(const PagedSte
         y.get(yf);
         request(u + THREADS);
         if (head >= 0 && at.page < 0) continue;
-        if (turned) {
-            if (head < 0) paged_turn<UNITS, float2, float>(xf, yf, turn32, c, r.halves);
-            else paged_turn<UNITS, double2, double>(xf, yf, turn, c, r.halves);
-        }
+        if (turned) paged_turn<UNITS>(xf, yf, turn, c, r.halves);
         if (head < 0) {
             IO *to = static_cast<IO *>(r.q_out) + t * r.q_out_stride + (head + r.q_heads) * D;
             io_store8(to + 8 * a, xf);

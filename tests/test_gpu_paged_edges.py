@@ -449,3 +449,18 @@ def test_a_timeout_behind_another_report_sets_a_cache_back(ctx):
     for _ in range(2):
         assert np.array_equal(run_attend(cache, step, q, "bf16"), want)
     cache.close()
+
+
+@pytest.mark.parametrize("pairs", ["adjacent", "halves"])
+def test_queries_are_turned_in_64_bits(ctx, pairs):
+    """one rounding to fp32, near and far positions; the angle of a position has 2^-50 of it"""
+    dim, kv, H = 128, 1, 5
+    step = Step(3, [5, 200, 70001], [5, 9, 20], 128)
+    cache = skn.PagedKVCache(ctx, step.n_pages, 128, kv, dim, "bf16", rot_dims=96, rot_pairs=pairs)
+    g = np.random.default_rng(5)
+    q = (g.standard_normal((step.n, H, dim)) * np.exp2(g.integers(-9, 9, (step.n, H, dim)))).astype(np.float32)
+    k = g.standard_normal((step.n, kv, dim)).astype(np.float32)
+    got = cache.append(k, k, step.table, step.starts, step.lens, q)
+    want = oracle.rotate(q, [p for _, p in oracle.positions(step.starts, step.lens)], 96, 10000.0, pairs)
+    assert np.all(np.abs(got - want) <= 2.0 ** -24 * np.abs(want) + 70001 * 2.0 ** -50 * np.abs(q).max(axis=2, keepdims=True))
+    cache.close()

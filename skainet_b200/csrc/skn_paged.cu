@@ -10,8 +10,8 @@
 // a far position, and keys that land next to a border of the cache's rounding; queries too: with fp32 sines they are off by 3.8e-8 instead of their own rounding's
 // 2.5e-8, and six prompts of 7500 tokens in bf16 take 36.5 us instead of 37.5); its threads take 16 dimensions of a head at a time, eight and the
 // eight they turn with, so that the rotation may happen in place.  The rows are requested a unit ahead, the first before all that.
-// Bound by HBM from a few thousand tokens on.  8192 tokens of 32 + 2 x 8 heads of 128, all of them turned: bf16 rows and cache 37.3 us (5.4 TB/s), fp32 rows and
-// a cache of 4 bits 62.6 us (5.5 TB/s); with requests behind the sines 96 us for the first; with four tokens to a CTA of 256 threads 41.4 and 68.3 us, no faster
+// Bound by HBM from a few thousand tokens on.  8192 tokens of 32 + 2 x 8 heads of 128, all of them turned: bf16 rows and cache 37.5 us (5.4 TB/s), fp32 rows and
+// a cache of 4 bits 62.7 us (5.5 TB/s); with requests behind the sines 96 us for the first; with four tokens to a CTA of 256 threads 41.4 and 68.3 us, no faster
 // for any smaller step (512 tokens 8.6 us instead of 8.1).  Alone, a token is 3 us of latency.
 
 // sequence of row i: the last one that starts at or before it (-1: none).  Every warp counts the starts for itself: 32 of them at even distances, then

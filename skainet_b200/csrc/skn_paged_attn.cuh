@@ -25,7 +25,7 @@
 // and a segment with one is computed again straight from the definition (paged_redo).
 //
 // 16-bit caches are bound by HBM: 16 sequences of 8192 tokens, 32 / 8 heads of 128, fp16 pages 97 us for fp32 rows and 95 us for bf16 ones (5.5 and 5.7 TB/s, 0.86 of a copy's
-// rate), bf16 pages 99 and 96, 48 sequences with a window of 4096 134 us (6.0 TB/s).  Q4_0: 64 sequences of 16384, bf16 rows, 393 us (3.1 TB/s; 62 % of the
+// rate), bf16 pages 99 and 96, 48 sequences with a window of 4096 134 us (6.0 TB/s).  Q4_0: 64 sequences of 16384, bf16 rows, 393 us (3.1 TB/s; 60 % of the
 // issue slots, the ALU pipe at 57 %: masks, permutes and conversions of V; neither is at its end), 16 of 8192 71 us, with fp32 rows, two terms of everything, 103.  One sequence
 // of 100 tokens is 8 us of latency, 1024 of one's 4100 20 us in a graph.  Shares smaller than the CTAs that run at a time (twice as many) cost 95 -> 101 us: every share has a beginning.
 #pragma once
